@@ -11,7 +11,7 @@ import os
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent.parent / "csrc" / "libpim_b200.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 F32, BF16, I32, I64 = 0, 1, 2, 3
 PROJ_PLAIN, PROJ_ROPE_KV, PROJ_SILU_MUL = 0, 1, 2
@@ -117,6 +117,71 @@ EXPORTS.update({
     "pim_aten_matmul": ([_PV, _PV, _PV, c_vp], c_i32),
     "pim_aten_sdpa": ([_PV, _PV, _PV, _PV, _PV, ctypes.c_double, c_i32, c_vp], c_i32),
     "pim_aten_embedding": ([_PV, _PV, _PV, c_vp, c_vp], c_i32),
+})
+
+
+class PagedKV(ctypes.Structure):
+    """Mirror of ``pim_paged_kv``."""
+
+    _fields_ = [("k_pages", c_vp), ("v_pages", c_vp), ("page_stride", c_i64), ("table", c_vp), ("table_stride", c_i64),
+                ("rows", c_i32), ("max_pages", c_i32), ("num_pages", c_i32), ("page_size", c_i32), ("kv_heads", c_i32),
+                ("head_dim", c_i32)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """Mirror of ``pim_paged_append_args``."""
+
+    _fields_ = [("kv", PagedKV), ("q", c_vp), ("k", c_vp), ("v", c_vp), ("q_stride", c_i64), ("k_stride", c_i64),
+                ("v_stride", c_i64), ("k_head_stride", c_i64), ("v_head_stride", c_i64), ("q_out", c_vp),
+                ("q_out_stride", c_i64), ("rope_cos", c_vp), ("rope_sin", c_vp), ("max_pos", c_i32),
+                ("q_heads", c_i32), ("pair_order", c_i32), ("tokens", c_i64), ("starts", c_vp), ("lengths", c_vp),
+                ("positions", c_vp), ("lengths_out", c_vp), ("positions_out", c_vp), ("slot_positions", c_vp),
+                ("weights", c_vp), ("state_row_stride", c_i64), ("state_head_stride", c_i64), ("err_flag", c_vp)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``pim_paged_attention_args``."""
+
+    _fields_ = [("kv", PagedKV), ("q", c_vp), ("out", c_vp), ("q_stride", c_i64), ("out_stride", c_i64),
+                ("lengths", c_vp), ("q_heads", c_i32), ("scale", c_f32), ("weights", c_vp),
+                ("weights_row_stride", c_i64), ("weights_head_stride", c_i64), ("err_flag", c_vp)]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """Mirror of ``pim_paged_evict_args``."""
+
+    _fields_ = [("kv", PagedKV), ("lengths", c_vp), ("positions", c_vp), ("weights", c_vp), ("slot_positions", c_vp),
+                ("weights_out", c_vp), ("slot_positions_out", c_vp), ("lengths_out", c_vp), ("state_row_stride", c_i64),
+                ("state_head_stride", c_i64), ("budget", c_i32), ("recent", c_i32), ("sink", c_i32),
+                ("err_flag", c_vp)]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """Mirror of ``pim_beam_select_args``."""
+
+    _fields_ = [("logits", c_vp), ("logits_stride", c_i64), ("scores", c_vp), ("done", c_vp), ("scores_out", c_vp),
+                ("parents", c_vp), ("tokens", c_vp), ("done_out", c_vp), ("batch", c_i32), ("beams", c_i32),
+                ("beams_out", c_i32), ("vocab", c_i32), ("eos", c_i32), ("pad", c_i32)]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    """Mirror of ``pim_beam_reorder_args``."""
+
+    _fields_ = [("pages", c_vp), ("block_stride", c_i64), ("page_stride", c_i64), ("table", c_vp), ("table_out", c_vp),
+                ("table_stride", c_i64), ("lengths", c_vp), ("parents", c_vp), ("batch", c_i32), ("beams", c_i32),
+                ("num_blocks", c_i32), ("max_pages", c_i32), ("num_pages", c_i32), ("page_size", c_i32),
+                ("kv_heads", c_i32), ("head_dim", c_i32), ("err_flag", c_vp)]
+
+
+EXPORTS.update({
+    "pim_paged_append": ([ctypes.POINTER(PagedAppendArgs), c_i32, c_vp], c_i32),
+    "pim_paged_attention": ([ctypes.POINTER(PagedAttentionArgs), c_i32, c_vp, c_i64, c_vp], c_i32),
+    "pim_paged_attention_workspace_bytes": ([ctypes.POINTER(PagedAttentionArgs), c_i32], c_i64),
+    "pim_paged_evict": ([ctypes.POINTER(PagedEvictArgs), c_i32, c_vp, c_i64, c_vp], c_i32),
+    "pim_paged_evict_workspace_bytes": ([ctypes.POINTER(PagedEvictArgs), c_i32], c_i64),
+    "pim_beam_select": ([ctypes.POINTER(BeamSelectArgs), c_i32, c_vp, c_i64, c_vp], c_i32),
+    "pim_beam_select_workspace_bytes": ([ctypes.POINTER(BeamSelectArgs), c_i32], c_i64),
+    "pim_beam_reorder": ([ctypes.POINTER(BeamReorderArgs), c_i32, c_vp], c_i32),
 })
 
 

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define PIM_ABI_VERSION 13
+#define PIM_ABI_VERSION 14
 
 enum pim_dtype { PIM_F32 = 0, PIM_BF16 = 1, PIM_I32 = 2, PIM_I64 = 3 };
 enum pim_status { PIM_OK = 0, PIM_EINVAL = 1, PIM_ECUDA = 2, PIM_EUNSUPPORTED = 3 };
@@ -353,6 +353,175 @@ int pim_fill_normal(void* out, int64_t n, int32_t dtype, uint64_t seed, float st
 /* Constant fill (e.g. RMSNorm weights = 1).  No reference counterpart. */
 int pim_fill_const(void* out, int64_t n, int32_t dtype, float value, void* stream);
 
+
+/* ---- paged KV cache ------------------------------------------------------------
+ * A KV cache whose memory follows the tokens: pages of page_size slots, and per sequence
+ * (row) a table of the pages that hold its slots 0, 1, 2, ... in order.  It stands beside
+ * the contiguous [max_seq, head_dim] blocks of memory/kv_layout.py (pim_attention, the
+ * KV append of pim_projection) for sequences of different lengths, for caches of bounded
+ * size and for beams that share their prompt.  No counterpart in the reference, whose
+ * cache is static.
+ *
+ * Every entry point below checks its arguments on the host before any CUDA call and
+ * bounds-checks what it reads from device memory (lengths, positions, page ids, parents):
+ * a bad value raises *err_flag (device int32, may be NULL) and the access it stands for is
+ * left out, as stated at each.  Rows may share pages only where an entry point says so.
+ * Nothing here keeps state between calls: workspaces are scratch (no initial contents,
+ * none expected afterwards); calls that overlap on the GPU must not share one. */
+typedef struct pim_paged_kv {
+  void* k_pages;            /* page p, head h, slot i, dim d at p * page_stride + (h * page_size + i) * head_dim + d */
+  void* v_pages;            /* the same layout */
+  int64_t page_stride;      /* elements between pages: at least kv_heads * page_size * head_dim */
+  const int32_t* table;     /* [rows, table_stride]: page ids, 0 <= id < num_pages where a row has slots */
+  int64_t table_stride;     /* elements between rows, at least max_pages */
+  int32_t rows;             /* sequences */
+  int32_t max_pages;        /* table entries of a row: a row holds at most max_pages * page_size slots */
+  int32_t num_pages;
+  int32_t page_size;        /* 8, 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;         /* 32, 64 or 128 */
+} pim_paged_kv;
+
+typedef struct pim_paged_append_args {
+  pim_paged_kv kv;
+  const void* q;            /* token t, head h, dim d at t * q_stride + h * head_dim + d; NULL: no q */
+  const void* k;
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;                /* elements between tokens */
+  int64_t k_head_stride, v_head_stride;                /* elements between heads of k and of v */
+  void* q_out;              /* token t at t * q_out_stride; may be q itself (same stride, no pair_order) */
+  int64_t q_out_stride;
+  const float* rope_cos;    /* [max_pos, head_dim / 2]; both NULL: no rotation */
+  const float* rope_sin;
+  int32_t max_pos;
+  int32_t q_heads;          /* with q; any number */
+  int32_t pair_order;       /* 1: element 2j of a head is dim j and 2j + 1 is dim j + head_dim / 2 (the row order of
+                               qkv_proj.weight, as pim_projection PLAIN leaves it); outputs are in dim order */
+  int64_t tokens;
+  const int32_t* starts;    /* [rows + 1]: row b has tokens starts[b] .. starts[b + 1) (0 or more); NULL: token b is
+                               row b's only one, tokens == rows.  Tokens behind starts[rows] are left out. */
+  const int32_t* lengths;   /* [rows] slots in use: the row's tokens go to slots lengths[b], lengths[b] + 1, ... */
+  const int32_t* positions; /* [rows] position of the row's first new token; NULL: lengths */
+  int32_t* lengths_out;     /* [rows] lengths + new tokens (not `lengths` itself); may be NULL */
+  int32_t* positions_out;   /* [rows] positions + new tokens (not `positions` itself); may be NULL */
+  int32_t* slot_positions;  /* eviction state, both or neither: [rows, kv_heads, slots] position of each slot's */
+  float* weights;           /* token (set) and its accumulated attention weight (set to 0) */
+  int64_t state_row_stride, state_head_stride;         /* elements, of both state arrays */
+  int32_t* err_flag;
+} pim_paged_append_args;
+
+/* New tokens into the pages of their rows, for every head of a layer: k rotated to its
+ * position (RoPE, halves rotated against one another as in pim_projection ROPE_KV,
+ * computed in fp32 and rounded once), v as it is; q rotated into q_out.  Replaces
+ * PIMStaticKVCache.update (memory/kv_layout.py:187-205) over pages.  A token whose slot,
+ * page or position is out of range raises *err_flag and is left out. */
+int pim_paged_append(const pim_paged_append_args* a, int32_t dtype, void* stream);
+
+typedef struct pim_paged_attention_args {
+  pim_paged_kv kv;
+  const void* q;            /* [rows, q_heads, head_dim], q_stride elements between rows */
+  void* out;                /* the same shape, out_stride elements between rows */
+  int64_t q_stride, out_stride;
+  const int32_t* lengths;   /* [rows] slots the row's token attends to (its own included); 0: the output row is 0 */
+  int32_t q_heads;          /* a multiple of kv_heads */
+  float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+  float* weights;           /* [rows, kv_heads, slots], weights_*_stride elements: every slot's probability, summed over
+                               the query heads of its group, is added to it; NULL: not asked for */
+  int64_t weights_row_stride, weights_head_stride;
+  int32_t* err_flag;
+} pim_paged_attention_args;
+
+/* Attention of one new token per row over its pages: the decode form of pim_attention over
+ * a paged cache, with query groups that share a kv head reading it once.  Rows may share
+ * pages.  A length outside [0, max_pages * page_size] is clamped and a page id out of
+ * range hides its slots; both raise *err_flag.  fp32 scores, softmax and sums; the output
+ * is rounded once.  The result does not depend on timing: no atomics. */
+int pim_paged_attention(const pim_paged_attention_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+/* Bytes of the workspace of a call with these arguments (its lengths are not read); -1 for
+ * arguments that pim_paged_attention refuses. */
+int64_t pim_paged_attention_workspace_bytes(const pim_paged_attention_args* a, int32_t dtype);
+
+typedef struct pim_paged_evict_args {
+  pim_paged_kv kv;
+  const int32_t* lengths;          /* [rows] slots in use */
+  const int32_t* positions;        /* [rows] position of the row's next token (tokens seen so far) */
+  const float* weights;            /* [rows, kv_heads, slots] accumulated attention weights */
+  const int32_t* slot_positions;   /* [rows, kv_heads, slots] positions of the slots' tokens */
+  float* weights_out;              /* the state after eviction; each may be its input (in place) or apart */
+  int32_t* slot_positions_out;
+  int32_t* lengths_out;            /* [rows]; not `lengths` itself */
+  int64_t state_row_stride, state_head_stride;          /* elements, of all four state arrays */
+  int32_t budget;                  /* slots kept per row and head, at least 1 */
+  int32_t recent, sink;            /* tokens at position >= positions - recent or < sink stay; recent + sink <= budget */
+  int32_t* err_flag;
+} pim_paged_evict_args;
+
+/* Cuts every row of more than `budget` slots down to `budget`, each head by itself: the
+ * newest `recent` tokens and the first `sink` ones stay, then those of the largest weight
+ * (of equal ones the lower slot; a NaN weight ranks below every number).  Kept tokens at
+ * slots >= budget move, K, V and state, into the slots < budget that became free, the
+ * first into the first; all others stay where they are.  Attention does not depend on the
+ * order of slots (K is rotated already) and slot_positions says which token a slot holds.
+ * Slots >= lengths_out are left as they were.  Rows must not share pages.  A length out of
+ * range is clamped and a row with a page id out of range moves nothing there; both raise
+ * *err_flag.  No counterpart in the reference. */
+int pim_paged_evict(const pim_paged_evict_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int64_t pim_paged_evict_workspace_bytes(const pim_paged_evict_args* a, int32_t dtype);
+
+typedef struct pim_beam_select_args {
+  const void* logits;       /* [batch, beams, vocab], logits_stride elements between beams (batch-major) */
+  int64_t logits_stride;
+  const float* scores;      /* [batch, beams] log-probability of each beam so far */
+  const int32_t* done;      /* [batch, beams] non-zero: the beam has ended; NULL: none has */
+  float* scores_out;        /* [batch, beams_out], best first */
+  int32_t* parents;         /* [batch, beams_out] beam (0 .. beams - 1) that each continues */
+  int32_t* tokens;          /* [batch, beams_out] */
+  int32_t* done_out;        /* [batch, beams_out] the parent had ended or the token is `eos`; may be NULL */
+  int32_t batch, beams;     /* beams <= 64 */
+  int32_t beams_out;        /* <= 64 */
+  int32_t vocab;
+  int32_t eos;              /* -1: no such token */
+  int32_t pad;              /* the token a beam that has ended continues with, 0 <= pad < vocab */
+} pim_beam_select_args;
+
+/* One step of beam search, per batch entry: the beams_out largest of
+ * scores[w] + logits[w][t] - log(sum_u exp(logits[w][u])) over beams w and tokens t, ties to the
+ * lowest w * vocab + t; a beam that has ended offers one candidate, `pad` at its score.  A
+ * logit that is not finite is no candidate and no part of the sum; a beam whose score is
+ * not finite offers none.  Where fewer than beams_out candidates are left, the rest get
+ * score -inf, parent 0, token `pad`, done 1.  Candidates of one beam are compared by their
+ * logits, those of different beams by their scores in fp64; scores_out is rounded once.
+ * Stands beside pim_argmax (greedy sampling, docs/spec.md:1552-1556). */
+int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int64_t pim_beam_select_workspace_bytes(const pim_beam_select_args* a, int32_t dtype);
+
+typedef struct pim_beam_reorder_args {
+  void* pages;              /* num_blocks blocks (each layer's K and V), block_stride elements apart, of pages laid */
+  int64_t block_stride;     /* out as in pim_paged_kv */
+  int64_t page_stride;
+  const int32_t* table;     /* [batch * beams, table_stride], the beams before */
+  int32_t* table_out;       /* the beams after (apart from `table`); max_pages entries of a row are written */
+  int64_t table_stride;     /* of both */
+  const int32_t* lengths;   /* [batch] slots in use, the same for every beam of an entry */
+  const int32_t* parents;   /* [batch, beams] as pim_beam_select gives them */
+  int32_t batch, beams;     /* beams <= 64 */
+  int32_t num_blocks;
+  int32_t max_pages, num_pages, page_size, kv_heads, head_dim;
+  int32_t* err_flag;
+} pim_beam_reorder_args;
+
+/* Reordering of the beams' cache states after pim_beam_select, through the page table: new
+ * beam j shares its parent's full pages.  The partly filled page cannot be shared, since
+ * both beams will append to it: a parent's first child takes the parent's, and each further
+ * child's is a copy (of the slots in use, in every block) in the page of a beam that has no
+ * child, so that no copy reads a page that another writes and no page is needed or lost.
+ * Entries behind the slots in use (reserved pages) stay with the beam's index.  The partly
+ * filled and reserved pages of the beams of an entry must differ.  A parent, length or page
+ * id out of range raises *err_flag: that entry's beams then keep their own tables. */
+int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, void* stream);
 
 /* ---- aten-level operations -------------------------------------------------------
  * For graphs compiled at aten granularity by the reference's own passes (torch.export,

@@ -14,7 +14,8 @@ Modules and what each restates:
   (comm/lowering.py:38-194): sequential in-dtype sums in rank order,
   merges by global range;
 * ``kernels``    -- NumPy kernel stubs for every op of the step graph, with
-  the bf16 rounding points of HF ``LlamaForCausalLM``.
+  the bf16 rounding points of HF ``LlamaForCausalLM``;
+* ``paged``      -- the paged-cache operators in fp64 (no reference counterpart).
 
 Parity is pinned by golden vectors generated from the reference itself
 (tests/golden/make_golden.py): the comm-plan segment tables, the redistribute

@@ -1,0 +1,659 @@
+"""The paged-cache operators against fp64 statements of the same formulas (GPU).
+
+Tolerances are derived, not tuned: the last rounding costs half a step of the type (``eps / 2`` of the value), and what
+comes before it is bounded by the arithmetic stated in ``oracle.paged.attention`` or beside the check.  Pages, tables and
+state outside what an operator may touch are compared bit for bit, and slots beyond a row's length hold NaN, so that a
+kernel which reads them shows.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"float32": 2.0**-24, "bfloat16": 2.0**-8}
+EXP = {"float32": 2.0**-21, "bfloat16": 2.0**-17}
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _tdt(dt):
+    torch = _torch()
+    return {"float32": torch.float32, "bfloat16": torch.bfloat16}[dt]
+
+
+def _host(t):
+    """fp64 copy of a device tensor (exact for every type used here)."""
+    torch = _torch()
+    torch.cuda.synchronize()
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def _ints(a):
+    return _torch().tensor(np.asarray(a), dtype=_torch().int32, device="cuda")
+
+
+class Pool:
+    """Pages of rows with the given numbers of slots in use, in shuffled order; unused slots and pages hold NaN."""
+
+    def __init__(self, lengths, *, heads, ps, hd, dt, seed=0, room=0, spare=3, k_scale=1.0):
+        torch = _torch()
+        rng = np.random.default_rng(seed)
+        need = [-(-(n + room) // ps) for n in lengths]
+        self.width = max(max(need), 1)
+        total = sum(need) + spare
+        order = rng.permutation(total).astype(np.int32)
+        table = np.full((len(lengths), self.width), order[-1] if spare else 0, np.int32)
+        at = 0
+        for b, m in enumerate(need):
+            table[b, :m] = order[at:at + m]
+            at += m
+        self.table_np, self.lengths_np = table, np.asarray(lengths, np.int32)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+
+        def pages(scale):
+            p = torch.full((total, heads, ps, hd), float("nan"), device="cuda", dtype=_tdt(dt))
+            for b, n in enumerate(lengths):
+                for i in range(need[b]):
+                    m = min(ps, n - i * ps)
+                    if m > 0:
+                        p[table[b, i], :, :m] = (scale * torch.randn(heads, m, hd, device="cuda", generator=g)).to(p.dtype)
+            return p
+
+        self.k, self.v = pages(k_scale), pages(1.0)
+        self.table, self.lengths = _ints(table), _ints(lengths)
+        self.ps = ps
+        self.slots = self.width * ps
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------------
+
+def _attention_case(lengths, group, heads, ps, hd, dt, seed=0, track=False, scale=None, k_scale=1.0):
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    pool = Pool(lengths, heads=heads, ps=ps, hd=hd, dt=dt, seed=seed, k_scale=k_scale)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    q = torch.randn(len(lengths), heads * group, hd, device="cuda", generator=g).to(_tdt(dt))
+    out = torch.full_like(q, float("nan"))
+    w0 = None
+    if track:
+        w0 = torch.rand(len(lengths), heads, pool.slots + 3, device="cuda", generator=g)[..., :pool.slots]
+    weights = None if w0 is None else w0.clone(memory_format=torch.preserve_format)
+    op = PagedAttention(q, pool.k, pool.v, pool.table, pool.lengths, out, weights=weights, scale=scale)
+    return pool, q, out, w0, weights, op
+
+
+def _check_attention(pool, q, out, w0, weights, dt, scale=None, lengths=None):
+    lengths = pool.lengths_np if lengths is None else lengths
+    want = ref.attention(_host(q), _host(pool.k), _host(pool.v), pool.table_np, lengths, scale, EXP[dt])
+    got = _host(out)
+    heads = pool.k.shape[1]
+    for b, (o, p, bound, rel) in enumerate(want):
+        tol = HALF[dt] * np.abs(o) + bound + 1e-30
+        off = np.abs(got[b] - o)
+        assert (off <= tol).all(), (b, lengths[b], float((off / tol).max()), float(off.max()))
+        if weights is None:
+            continue
+        n = lengths[b]
+        got_w, old = _host(weights[b]), _host(w0[b])
+        add = p.reshape(heads, p.shape[0] // heads, n).sum(1)
+        # one rounding of the sum and one per head added to it
+        tol = (1 + p.shape[0] // heads) * 2.0**-24 * (old[:, :n] + add) + rel * add
+        assert (np.abs(got_w[:, :n] - (old[:, :n] + add)) <= tol).all(), b
+        assert np.array_equal(got_w[:, n:], old[:, n:])
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("group,heads,ps", [(1, 3, 16), (2, 2, 8), (4, 1, 32), (7, 2, 64), (8, 1, 16), (12, 1, 128),
+                                            (16, 2, 16), (33, 1, 8)])
+def test_attention_groups_and_dims(group, heads, ps, hd, dt, track):
+    lengths = [1, 0, 7, 8, 9, 63, 64, 65, 130, 257, 0, 513]
+    pool, q, out, w0, weights, op = _attention_case(lengths, group, heads, ps, hd, dt, track=track)
+    assert op() is out
+    _check_attention(pool, q, out, w0, weights, dt)
+    op.check()
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("lengths", [[1], [130], [0], [0, 0, 5, 0], [4097], [2, 9001, 1, 3000], [300] * 70])
+def test_attention_lengths(lengths, dt, track):
+    pool, q, out, w0, weights, op = _attention_case(lengths, 4, 2, 16, 128, dt, seed=3, track=track)
+    op()
+    _check_attention(pool, q, out, w0, weights, dt)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_many_rows_and_heads(dt):
+    rng = np.random.default_rng(5)
+    pool, q, out, w0, weights, op = _attention_case(list(rng.integers(0, 200, 150)), 1, 32, 16, 128, dt, seed=5)
+    op()
+    _check_attention(pool, q, out, w0, weights, dt)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_scale_and_sharp_scores(dt):
+    """Scores of tens: all the weight on few keys, and a running maximum that grows along the row."""
+    pool, q, out, w0, weights, op = _attention_case([700, 33], 2, 2, 32, 64, dt, seed=8, track=True, scale=0.5,
+                                                    k_scale=4.0)
+    op()
+    _check_attention(pool, q, out, w0, weights, dt, scale=0.5)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_keys_of_minus_infinity_get_no_weight(dt):
+    """A key whose score is -inf (here alone in its first tiles) has probability 0; the row's sum stays finite."""
+    torch = _torch()
+    pool, q, out, w0, weights, op = _attention_case([200], 1, 1, 16, 64, dt, seed=9, track=True)
+    q[:] = 0
+    q[:, :, 0] = 1
+    for slot in list(range(0, 70)) + [120]:
+        pool.k[pool.table_np[0, slot // 16], 0, slot % 16, 0] = -float("inf")
+    op()
+    got = _host(out)
+    k = ref.slots(_host(pool.k), pool.table_np[0], 200)[0]
+    v = ref.slots(_host(pool.v), pool.table_np[0], 200)[0]
+    s = k[:, 0] / 8.0
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    assert (p[:70] == 0).all()
+    want = p @ v
+    rel = 2 * 66 * 2.0**-23 * np.abs(s[np.isfinite(s)]).max() + EXP[dt] + 400 * 2.0**-23
+    assert (np.abs(got[0, 0] - want) <= HALF[dt] * np.abs(want) + rel * (p @ np.abs(v))).all()
+    assert np.array_equal(_host(weights)[0, 0, :70], _host(w0)[0, 0, :70])
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_strided_rows_shared_pages_and_repeats(dt):
+    """q and out as parts of wider rows; two rows read the same pages; a second call gives the same bits."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    pool = Pool([90, 70], heads=2, ps=16, hd=64, dt=dt, seed=11)
+    table = pool.table_np.copy()
+    table[1, :4] = table[0, :4]
+    pool.table_np, pool.table = table, _ints(table)
+    wide = torch.randn(2, 4 + 2, 6, 64, device="cuda").to(_tdt(dt))
+    q = wide[:, 1, :4]
+    hold = torch.full((2, 8, 64), float("nan"), device="cuda", dtype=_tdt(dt))
+    out = hold[:, 2:6]
+    op = PagedAttention(q, pool.k, pool.v, pool.table, pool.lengths, out)
+    op()
+    _check_attention(pool, q, out, None, None, dt)
+    assert bool(torch.isnan(hold[:, :2]).all()) and bool(torch.isnan(hold[:, 6:]).all())
+    first = out.clone()
+    op()
+    assert torch.equal(first, out)
+
+
+def test_attention_bad_pages_and_lengths_raise_the_flag_and_hide_the_slots():
+    """A page id outside the pool hides its slots, a length outside the table is clamped; both are reported."""
+    torch = _torch()
+    pool, q, out, _, _, op = _attention_case([40, 40, 40], 2, 2, 16, 64, "bfloat16", seed=12)
+    table = pool.table_np.copy()
+    table[0, 1], table[1, 0] = pool.k.shape[0], -1
+    pool.table.copy_(_ints(table))
+    pool.lengths.copy_(_ints([40, 16, -5]))
+    op()
+    with pytest.raises(ValueError, match="out of range"):
+        op.check()
+    op.check()  # cleared
+    keep = np.r_[0:16, 32:40]
+    k, v = (np.repeat(ref.slots(_host(p), pool.table_np[0], 40)[:, keep], 2, 0) for p in (pool.k, pool.v))
+    s = np.einsum("hd,hnd->hn", _host(q)[0], k) / 8.0
+    p = np.exp(s - s.max(1, keepdims=True))
+    want = np.einsum("hn,hnd->hd", p / p.sum(1, keepdims=True), v)
+    # (a coarse bound: the values are what is asked, the arithmetic is held to its bound above)
+    assert np.abs(_host(out)[0] - want).max() <= 2 * HALF["bfloat16"] * np.abs(want).max()
+    assert not _host(out)[1].any() and not _host(out)[2].any()
+    pool.lengths.copy_(_ints([0, 0, 10**6]))
+    pool.k.nan_to_num_(), pool.v.nan_to_num_()
+    op()
+    with pytest.raises(ValueError):
+        op.check()
+    assert np.isfinite(_host(out)).all()
+
+
+def test_attention_offsets_beyond_32_bits():
+    """Pages behind the 2^31-th element of the pool."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    heads, ps, hd = 4, 32, 128
+    num = (1 << 31) // (heads * ps * hd) + 40
+    k, v = (torch.empty(num, heads, ps, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = np.array([[num - 1 - 2 * i for i in range(6)]], np.int32)
+    n = 6 * ps - 5
+    for p in (k, v):
+        for i in table[0]:
+            p[int(i)] = torch.randn(heads, ps, hd, device="cuda").to(torch.bfloat16)
+    q = torch.randn(1, heads * 2, hd, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(q)
+    PagedAttention(q, k, v, _ints(table), _ints([n]), out)()
+    small = [_host(p[table[0].tolist()]) for p in (k, v)]
+    (o, _, bound, _), = ref.attention(_host(q), *small, np.arange(6)[None], [n])
+    assert (np.abs(_host(out)[0] - o) <= HALF["bfloat16"] * np.abs(o) + bound).all()
+
+
+# ---- append -----------------------------------------------------------------------------------------------------------------
+
+def _rope(hd, top):
+    torch = _torch()
+    inv = 10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+    ang = torch.arange(top, dtype=torch.float64)[:, None] * inv[None]
+    return ang.cos().float().cuda(), ang.sin().float().cuda()
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("pair_order", [False, True])
+@pytest.mark.parametrize("rotate", [False, True])
+@pytest.mark.parametrize("hq,heads,hd,ps,new,past", [
+    (4, 4, 128, 16, [1], [0]), (4, 2, 64, 8, [5, 0, 17, 1], [3, 9, 0, 40]), (3, 1, 32, 32, [0, 0, 70], [1, 2, 31]),
+    (32, 32, 128, 16, [1] * 9, list(range(9))), (8, 1, 128, 256, [300, 1], [0, 255])])
+def test_append(hq, heads, hd, ps, new, past, rotate, pair_order, dt):
+    from backend.cuda_paged import PagedAppend
+
+    torch = _torch()
+    rows = len(new)
+    pool = Pool([0] * rows, heads=heads, ps=ps, hd=hd, dt=dt, seed=1, room=max(m + n for m, n in zip(past, new)) + 1)
+    before = [p.clone() for p in (pool.k, pool.v)]
+    tokens = sum(new)
+    pad = 3  # tokens behind the last row: left out
+    qkv = torch.randn(tokens + pad, (hq + 2 * heads) * hd, device="cuda").to(_tdt(dt))
+    q, k, v = (x.view(tokens + pad, -1, hd) for x in qkv.split([hq * hd, heads * hd, heads * hd], dim=1))
+    starts = np.r_[0, np.cumsum(new)].astype(np.int32)
+    positions = np.asarray(past) + 7 * (np.arange(rows) % 2)
+    cos, sin = _rope(hd, int(max(positions + new)) + 1) if rotate else (None, None)
+    q_out = torch.full((tokens + pad, hq, hd), 5.0, device="cuda", dtype=_tdt(dt))
+    lengths_out, positions_out = _ints([-1] * rows), _ints([-1] * rows)
+    slot_positions = torch.full((rows, heads, pool.slots), -9, dtype=torch.int32, device="cuda")
+    weights = torch.full((rows, heads, pool.slots), 3.0, device="cuda")
+    op = PagedAppend(k, v, pool.k, pool.v, pool.table, _ints(past), lengths_out, q=q, q_out=q_out, cos=cos, sin=sin,
+                     positions=_ints(positions), positions_out=positions_out, starts=_ints(starts),
+                     slot_positions=slot_positions, weights=weights, pair_order=pair_order)
+    op()
+    op.check()
+    c, s = (None, None) if cos is None else (_host(cos), _host(sin))
+    args = (pool.table_np, past, starts, positions, _host(q), _host(k), _host(v))
+    wk, wv, wq = ref.append(_host(before[0]), _host(before[1]), *args, c, s, pair_order)
+    # |x1 c - x2 s| in fp32: two rounded products and their sum, each off by 2^-24 of at most |x1 c| + |x2 s|
+    mk, mv, mq = (4.0 * 2.0**-24 * 8.0 if rotate else 0.0,) * 3  # |x| < 5.7 here: |x1 c| + |x2 s| <= 5.7 sqrt 2 < 8.1
+    assert float(qkv.float().abs().max()) < 5.65
+    for got, want, m in ((pool.k, wk, mk), (pool.v, wv, mv)):
+        got = _host(got)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        ok = ~np.isnan(want)
+        assert (np.abs(got - want)[ok] <= HALF[dt] * np.abs(want)[ok] + m).all()
+    assert np.array_equal(_host(pool.v)[~np.isnan(wv)], wv[~np.isnan(wv)])  # v is copied
+    got = _host(q_out)
+    assert (np.abs(got - wq)[:tokens] <= HALF[dt] * np.abs(wq)[:tokens] + mq).all() and (got[tokens:] == 5.0).all()
+    assert _host(lengths_out).tolist() == [m + n for m, n in zip(past, new)]
+    assert _host(positions_out).tolist() == (positions + new).tolist()
+    for b in range(rows):
+        at = np.full(pool.slots, -9.0)
+        at[past[b]:past[b] + new[b]] = positions[b] + np.arange(new[b])
+        assert (_host(slot_positions)[b] == at).all()
+        assert (_host(weights)[b] == np.where(at == -9, 3.0, 0.0)).all()
+
+
+def test_append_one_token_a_row_in_place_and_from_a_contiguous_block():
+    """Without starts: a token per row, q rotated in place; then K / V taken from [heads][k|v][seq][dim] blocks."""
+    from backend.cuda_paged import PagedAppend
+
+    torch = _torch()
+    hd, heads, rows = 64, 2, 5
+    past = [0, 7, 8, 15, 16]
+    pool = Pool([0] * rows, heads=heads, ps=8, hd=hd, dt="float32", room=40)
+    q, k, v = (torch.randn(rows, n, hd, device="cuda") for n in (6, heads, heads))
+    cos, sin = _rope(hd, 40)
+    want = ref.append(_host(pool.k), _host(pool.v), pool.table_np, past, np.arange(rows + 1), past, _host(q), _host(k),
+                      _host(v), _host(cos), _host(sin))
+    op = PagedAppend(k, v, pool.k, pool.v, pool.table, _ints(past), q=q, q_out=q, cos=cos, sin=sin)
+    op()
+    op.check()
+    for got, w in zip((pool.k, pool.v, q), want):
+        got, ok = _host(got), ~np.isnan(w)
+        assert np.array_equal(np.isnan(got), np.isnan(w))
+        assert (np.abs(got - w)[ok] <= HALF["float32"] * np.abs(w)[ok] + 4 * 2.0**-24 * 8.0).all()
+    block = torch.randn(heads, 2, 30, hd, device="cuda")
+    pool = Pool([0], heads=heads, ps=8, hd=hd, dt="float32", room=40)
+    PagedAppend(block[:, 0, :21].transpose(0, 1), block[:, 1, :21].transpose(0, 1), pool.k, pool.v, pool.table,
+                _ints([3]), starts=_ints([0, 21]))()
+    for pages, i in ((pool.k, 0), (pool.v, 1)):
+        assert np.array_equal(ref.slots(_host(pages), pool.table_np[0], 24)[:, 3:], _host(block[:, i, :21]))
+
+
+def test_append_leaves_out_what_does_not_fit():
+    """A slot beyond the table, a page id outside the pool and a position outside the rotary table: reported, and
+    neither written nor rotated; the other rows' tokens are."""
+    from backend.cuda_paged import PagedAppend
+
+    torch = _torch()
+    pool = Pool([0] * 4, heads=1, ps=8, hd=32, dt="float32", room=16)
+    table = pool.table_np.copy()
+    table[1, 0] = pool.k.shape[0]
+    pool.table.copy_(_ints(table))
+    k = torch.randn(4, 1, 32, device="cuda")
+    q = torch.randn(4, 1, 32, device="cuda")
+    q_out = torch.zeros_like(q)
+    cos, sin = _rope(32, 10)
+    op = PagedAppend(k, k.clone(), pool.k, pool.v, pool.table, _ints([16, 3, 2, 4]), q=q, q_out=q_out, cos=cos, sin=sin,
+                     positions=_ints([1, 1, 10, 9]))
+    op()
+    with pytest.raises(ValueError, match="out of range"):
+        op.check()
+    written = ~torch.isnan(pool.v).all(dim=-1)
+    assert int(written.sum()) == 1 and bool(written[int(table[3, 0]), 0, 4])
+    assert not _host(q_out)[:3].any() and _host(q_out)[3].any()
+
+
+# ---- eviction -----------------------------------------------------------------------------------------------------------------
+
+def _evict_case(lengths, heads, ps, hd, dt, budget, recent, sink, seed=0, ties=False, in_place=False, weights=None,
+                seen=None):
+    from backend.cuda_paged import PagedEvict
+
+    torch = _torch()
+    rng = np.random.default_rng(seed)
+    pool = Pool(lengths, heads=heads, ps=ps, hd=hd, dt=dt, seed=seed)
+    rows, slots = len(lengths), pool.slots
+    if weights is None:
+        weights = rng.exponential(size=(rows, heads, slots)).astype(np.float32)
+        if ties:
+            weights = np.round(weights).astype(np.float32)
+    seen = [n + 5 for n in lengths] if seen is None else seen
+    pos = np.full((rows, heads, slots), -77, np.int32)
+    for b, n in enumerate(lengths):
+        for h in range(heads):
+            pos[b, h, :n] = np.sort(rng.permutation(seen[b])[:n])[rng.permutation(n)] if n else []
+    w_in, p_in = torch.tensor(weights, device="cuda"), _ints(pos)
+    w_out, p_out = (w_in, p_in) if in_place else (torch.full_like(w_in, -3.0), torch.full_like(p_in, -3))
+    lengths_out = _ints([-1] * rows)
+    before = [p.clone() for p in (pool.k, pool.v)]
+    op = PagedEvict(pool.k, pool.v, pool.table, pool.lengths, w_in, p_in, _ints(seen), w_out, p_out, lengths_out,
+                    budget=budget, recent=recent, sink=sink)
+    op()
+    op.check()
+    got_w, got_p = _host(w_out), _host(p_out)
+    want = [_host(p) for p in before]
+    for b, n in enumerate(lengths):
+        left = min(n, budget)
+        for h in range(heads):
+            src = ref.evict(n, seen[b], weights[b, h], pos[b, h], budget, recent, sink)
+            assert np.array_equal(got_w[b, h, :left], weights[b, h][src], equal_nan=True), (b, h)
+            assert np.array_equal(got_p[b, h, :left], pos[b, h][src])
+            if in_place:
+                assert np.array_equal(got_w[b, h, left:], weights[b, h, left:], equal_nan=True)
+                assert np.array_equal(got_p[b, h, left:], pos[b, h, left:])
+            else:
+                assert (got_w[b, h, left:] == -3).all() and (got_p[b, h, left:] == -3).all()
+            for w, old in zip(want, before):
+                rows_of = ref.slots(_host(old), pool.table_np[b], n)[h][src] if n else []
+                for j in range(left):
+                    w[pool.table_np[b, j // ps], h, j % ps] = rows_of[j]
+    assert _host(lengths_out).tolist() == [min(n, budget) for n in lengths]
+    for pages, w in zip((pool.k, pool.v), want):
+        assert np.array_equal(_host(pages), w, equal_nan=True)
+    return pool, op
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dt,hd", [("float32", 32), ("bfloat16", 64), ("bfloat16", 128), ("float32", 128)])
+@pytest.mark.parametrize("lengths,heads,ps,budget,recent,sink", [
+    ([33], 2, 16, 32, 8, 2), ([0, 1, 2, 5, 17, 64, 65, 200], 2, 8, 17, 5, 1), ([100, 3], 1, 32, 1, 0, 0),
+    ([90, 40], 3, 16, 64, 64, 0), ([90, 40], 1, 16, 20, 0, 20), ([50, 60], 2, 64, 128, 10, 4), ([1500], 1, 16, 700, 100, 4)])
+def test_evict(lengths, heads, ps, budget, recent, sink, dt, hd, in_place):
+    _evict_case(lengths, heads, ps, hd, dt, budget, recent, sink, in_place=in_place)
+
+
+@pytest.mark.parametrize("budget", [1, 13, 64, 255])
+def test_evict_ties_go_to_the_lower_slot(budget):
+    _evict_case([256, 199], 2, 16, 32, "bfloat16", budget, 0, 0, seed=4, ties=True)
+    _evict_case([256], 1, 16, 32, "bfloat16", budget, 0, 0, weights=np.zeros((1, 1, 256), np.float32))
+
+
+def test_evict_ranks_infinities_zeros_of_both_signs_and_nan():
+    rng = np.random.default_rng(6)
+    w = rng.choice(np.array([0.0, -0.0, 1.0, -1.0, np.inf, -np.inf, np.nan, 1e-42, 3e38], np.float32), size=(1, 2, 304))
+    for budget in (5, 100, 250, 303):
+        _evict_case([301], 2, 16, 32, "float32", budget, 2, 1, seed=budget, weights=w.copy())
+
+
+def test_evict_rows_longer_than_shared_memory():
+    _evict_case([70001], 1, 256, 32, "bfloat16", 20000, 300, 4, seed=7)
+    _evict_case([52000, 48000], 1, 64, 32, "bfloat16", 40001, 0, 0, seed=8, ties=True, in_place=True)
+
+
+def test_evict_reports_bad_lengths_and_pages():
+    from backend.cuda_paged import PagedEvict
+
+    torch = _torch()
+    pool, op = _evict_case([40, 40], 1, 8, 32, "float32", 16, 4, 0)
+    op.check()
+    w, p = torch.rand(2, 1, 40, device="cuda"), torch.arange(40, device="cuda", dtype=torch.int32).repeat(2, 1, 1)
+    table = pool.table.clone()
+    table[1, 1:] = 10**6
+    k = pool.k.clone()
+    op = PagedEvict(pool.k, pool.v, table, _ints([99, 40]), w, p, _ints([40, 40]), torch.zeros_like(w),
+                    torch.zeros_like(p), _ints([0, 0]), budget=16, recent=4)
+    op()
+    with pytest.raises(ValueError, match="out of range"):
+        op.check()
+    assert _host(op.lengths_out).tolist() == [16, 16]
+    same = (k == pool.k) | (torch.isnan(k) & torch.isnan(pool.k))
+    for page in pool.table_np[1]:
+        assert bool(same[int(page)].all())
+
+
+# ---- beam search ----------------------------------------------------------------------------------------------------------------
+
+def _select(logits, scores, k, done=None, eos=-1, pad=0):
+    from backend.cuda_paged import BeamSelect
+
+    torch = _torch()
+    b = logits.shape[0]
+    outs = (torch.full((b, k), 9.0, device="cuda"), *(torch.full((b, k), -5, dtype=torch.int32, device="cuda") for _ in range(3)))
+    op = BeamSelect(logits, scores, *outs[:3], done=done, done_out=outs[3], eos=eos, pad=pad)
+    op()
+    return [_host(t) for t in outs]
+
+
+def _check_select(logits, scores, k, done=None, eos=-1, pad=0):
+    got = _select(logits, scores, k, done, eos, pad)
+    lg, sc = _host(logits), _host(scores)
+    for b in range(lg.shape[0]):
+        want = ref.beam_select(lg[b], sc[b], k, None if done is None else _host(done)[b], eos, pad)
+        for name, g, w in zip(("parents", "tokens", "done"), (x[b] for x in got[1:]), want[1:]):
+            assert g.tolist() == w.tolist(), (name, b, g, w, want[0])
+        fine = np.isfinite(want[0])
+        # fp32 exponentials (2 units in the last place) under an fp64 sum: 2^-22 in the sum, so in its logarithm, and
+        # the last rounding
+        assert (np.abs(got[0][b][fine] - want[0][fine]) <= 2.0**-24 * np.abs(want[0])[fine] + 2.0**-22).all()
+        assert (got[0][b][~fine] == -np.inf).all()
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("b,w,vocab,k", [(1, 4, 32000, 4), (1, 1, 1024, 5), (3, 5, 1003, 5), (2, 8, 4096, 16), (2, 3, 7, 4),
+                                         (1, 2, 1, 2), (2, 16, 50001, 16), (1, 64, 5000, 64), (4, 1, 9000, 64),
+                                         (1, 33, 4097, 33)])
+def test_beam_select(b, w, vocab, k, dt):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(b * 1000 + w)
+    logits = (3 * torch.randn(b, w, vocab, device="cuda", generator=g)).to(_tdt(dt))
+    scores = -10 + torch.randn(b, w, device="cuda", generator=g)
+    _check_select(logits, scores, k)
+    done = (torch.rand(b, w, device="cuda", generator=g) < 0.4).to(torch.int32)
+    _check_select(logits, scores, k, done, eos=min(2, vocab - 1), pad=vocab - 1)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_beam_select_ties(dt):
+    """Equal logits, equal beams and constant rows: the lowest beam, then the lowest token."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    few = torch.randint(0, 3, (2, 4, 9001), device="cuda", generator=g).to(_tdt(dt))
+    few[:, 2] = few[:, 0]
+    scores = torch.zeros(2, 4, device="cuda")
+    _check_select(few, scores, 8)
+    _check_select(torch.zeros(1, 3, 20000, device="cuda", dtype=_tdt(dt)), torch.zeros(1, 3, device="cuda"), 64)
+    zeros = torch.zeros(1, 2, 64, device="cuda", dtype=_tdt(dt))
+    zeros[0, 0, ::2] = -0.0
+    _check_select(zeros, torch.zeros(1, 2, device="cuda"), 5)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_beam_select_infinities_and_ended_beams(dt):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randn(3, 3, 5003, device="cuda", generator=g).to(_tdt(dt))
+    inf = float("inf")
+    logits[0, 0] = -inf                      # a beam with nothing left
+    logits[0, 1, 5:] = -inf                  # five tokens left
+    logits[0, 2, :] = -inf
+    logits[0, 2, 7] = 1.0
+    logits[1, :, 100:4000] = torch.finfo(logits.dtype).min  # masked with the type's lowest value: a logit like any other
+    logits[1, 0, 17], logits[1, 1, 18], logits[1, 2, 19] = inf, float("nan"), -inf
+    scores = torch.randn(3, 3, device="cuda", generator=g)
+    scores[2, 0], scores[2, 2] = -inf, float("nan")
+    _check_select(logits, scores, 8)  # entry 0: six candidates for eight places
+    done = torch.tensor([[1, 0, 0], [0, 1, 1], [1, 1, 1]], dtype=torch.int32, device="cuda")
+    _check_select(logits, scores, 8, done, eos=3, pad=4)
+
+
+def test_beam_select_strided_logits():
+    torch = _torch()
+    for dt in ("float32", "bfloat16"):
+        wide = torch.randn(6, 1050, device="cuda").to(_tdt(dt))
+        logits = wide.view(2, 3, 1050)[:, :, 1:1042]
+        _check_select(logits, torch.zeros(2, 3, device="cuda"), 3)
+    stack = torch.randn(2, 3, 1040, device="cuda")
+    _check_select(stack[:, :, :1024], torch.zeros(2, 3, device="cuda"), 3)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("layers,heads,ps,hd,length", [(2, 3, 16, 64, 37), (1, 1, 8, 32, 8), (3, 2, 32, 128, 0),
+                                                       (1, 2, 16, 128, 5), (2, 1, 64, 32, 191), (2, 2, 8, 64, 48)])
+def test_beam_reorder(layers, heads, ps, hd, length, dt):
+    from backend.cuda_paged import BeamReorder
+
+    torch = _torch()
+    rng = np.random.default_rng(length)
+    cases = [[0, 1, 2, 3, 4], [4, 3, 2, 1, 0], [2, 2, 2, 2, 2], [1, 1, 0, 0, 4], [0, 0, 0, 4, 4], [3, 1, 3, 1, 3]]
+    b, w, full = len(cases), 5, length // ps
+    width = full + 2
+    pool = b * full + 2 * b * w + 2
+    order = rng.permutation(pool)
+    table = np.zeros((b, w, width), np.int32)
+    table[:, :, :full] = order[:b * full].reshape(b, 1, full)
+    table[:, :, full:] = order[b * full:b * full + 2 * b * w].reshape(b, w, 2)
+    pages = torch.randn(layers, 2, pool, heads, ps, hd, device="cuda").to(_tdt(dt))
+    before = _host(pages).reshape(layers * 2, pool, heads, ps, hd)
+    parents = _ints(cases)
+    table_out = torch.full((b * w, width), -1, dtype=torch.int32, device="cuda")
+    op = BeamReorder(pages, _ints(table.reshape(b * w, width)), _ints([length] * b), parents, table_out)
+    op()
+    op.check()
+    want = before
+    rows = []
+    for i in range(b):
+        want, t = ref.beam_reorder(want, table[i], length, np.asarray(cases[i]))
+        rows.append(t)
+    assert np.array_equal(_host(table_out), np.concatenate(rows))
+    assert np.array_equal(_host(pages).reshape(want.shape), want)
+    first = pages.clone()
+    op()  # the tables have not changed: a repeat writes the same copies
+    assert torch.equal(first, pages)
+
+
+def test_beam_reorder_reports_bad_parents_and_keeps_the_tables():
+    from backend.cuda_paged import BeamReorder
+
+    torch = _torch()
+    pages = torch.randn(1, 2, 12, 1, 8, 32, device="cuda")
+    table = _ints([[0, 1], [0, 2], [3, 4], [3, 5]])
+    for parents, lengths, bad in (([[0, 2], [1, 1]], [12, 12], 0), ([[0, 0], [-1, 0]], [12, 12], 1),
+                                  ([[1, 0], [1, 1]], [12, 17], 1), ([[1, 0], [0, 0]], [-1, 12], 0)):
+        out = torch.zeros_like(table)
+        op = BeamReorder(pages, table, _ints(lengths), _ints(parents), out)
+        op()
+        with pytest.raises(ValueError, match="out of range"):
+            op.check()
+        assert torch.equal(out[2 * bad:2 * bad + 2], table[2 * bad:2 * bad + 2])
+
+
+# ---- streams and graphs -------------------------------------------------------------------------------------------------------------
+
+def test_calls_on_another_stream_and_captured_replays_follow_the_device_values():
+    """One captured graph of append + attention + eviction is replayed with new lengths, positions and values."""
+    from backend.cuda_paged import PagedAppend, PagedAttention, PagedEvict
+
+    torch = _torch()
+    heads, hd, ps, rows, budget = 2, 64, 8, 3, 24
+    dt = "float32"
+
+    def build(seed):
+        pool = Pool([20, 5, 24], heads=heads, ps=ps, hd=hd, dt=dt, seed=seed, room=10)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        s = dict(pool=pool, q=torch.randn(rows, 4, hd, device="cuda", generator=g),
+                 k=torch.randn(rows, heads, hd, device="cuda", generator=g),
+                 v=torch.randn(rows, heads, hd, device="cuda", generator=g))
+        s["n1"], s["n2"], s["pos2"] = _ints([0] * rows), _ints([0] * rows), _ints([0] * rows)
+        s["pos"] = _ints([20, 5, 24])
+        s["q_out"], s["out"] = torch.zeros_like(s["q"]), torch.zeros_like(s["q"])
+        s["w"] = torch.rand(rows, heads, pool.slots, device="cuda", generator=g)
+        s["sp"] = torch.arange(pool.slots, device="cuda", dtype=torch.int32).expand(rows, heads, -1).contiguous()
+        cos, sin = _rope(hd, 100)
+        ops = [PagedAppend(s["k"], s["v"], pool.k, pool.v, pool.table, pool.lengths, s["n1"], q=s["q"], q_out=s["q_out"],
+                           cos=cos, sin=sin, positions=s["pos"], positions_out=s["pos2"], slot_positions=s["sp"],
+                           weights=s["w"]),
+               PagedAttention(s["q_out"], pool.k, pool.v, pool.table, s["n1"], s["out"], weights=s["w"]),
+               PagedEvict(pool.k, pool.v, pool.table, s["n1"], s["w"], s["sp"], s["pos2"], s["w"], s["sp"], s["n2"],
+                          budget=budget, recent=4)]
+
+        def step():
+            for op in ops:
+                op()
+            pool.lengths.copy_(s["n2"])
+            s["pos"].copy_(s["pos2"])
+
+        return s, ops, step
+
+    one, ops1, step1 = build(3)
+    two, ops2, step2 = build(3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step2()  # a warm-up on another stream, then the capture
+    torch.cuda.current_stream().wait_stream(side)
+    step1()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step2()
+    torch.cuda.synchronize()
+    for i in range(8):
+        for s in (one, two):
+            g = torch.Generator(device="cuda").manual_seed(50 + i)
+            for name in ("q", "k", "v"):
+                s[name].copy_(torch.randn(s[name].shape, device="cuda", generator=g))
+        step1()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in ("out", "w", "sp", "n2", "pos"):
+            assert torch.equal(one[name], two[name]), (i, name)
+        for a, b in ((one["pool"].k, two["pool"].k), (one["pool"].v, two["pool"].v)):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+        assert bool(torch.isfinite(one["out"]).all())
+    assert one["n2"].tolist() == [24, 14, 24]
+    for op in ops1 + ops2:
+        op.check()
