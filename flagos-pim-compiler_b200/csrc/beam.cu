@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
     int4 raw[kBeamVals / V];
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i)
-      if (base + tok(i * V) < a.vocab) raw[i] = ld_stream(reinterpret_cast<const int4*>(x + base + tok(i * V)));
+      if (base + tok(i * V) < a.vocab) raw[i] = ld_once(reinterpret_cast<const int4*>(x + base + tok(i * V)));
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i)
       if (base + tok(i * V) < a.vocab) {

@@ -1,10 +1,38 @@
-// pim_paged_attention: attention of one new token per row over a paged KV cache.
+// pim_paged_attention: attention of one new token per row over a paged KV cache, split over
+// the cache's length and joined.
 //
 //   s_j = scale q . k_j,  p_j = exp(s_j - m) / sum_i exp(s_i - m),  o = sum_j p_j v_j,  j < lengths[row]
 //
-// First form, right for every shape: a CTA per (row, kv head), its warps walk the keys of
-// one query head after another with an online softmax; the keys' probabilities are found
-// again in a second walk when the weights are asked for.
+// Bound by the bytes of K and V, each of which is needed once: a query group shares one kv
+// head, so the unit of work is (row, kv head, head tile of up to 16 query heads).
+//
+// Split.  Lengths are read on the device and differ, so no grid fits them: the units' keys
+// are cut into tiles of 64 and the tiles of all units, in order, are dealt out evenly to as
+// many CTAs as the GPU holds at once (CTA c takes tiles [c T / G, (c + 1) T / G)).  A CTA walks
+// its range unit by unit; units that lie in one CTA are written at once, a unit that spans
+// several leaves a partial (max, sum, o) per CTA, of which a CTA has at most two: its first
+// and its last.  paged_finish_kernel joins them: which CTAs hold a unit follows from the
+// lengths alone, so there are no tickets, no atomics and nothing that must be zero before a
+// call, and the result does not depend on timing.
+//
+// bf16: the products run on warp-level MMA (m16n8k16) straight from registers.  The order of
+// the summed dims is free, so a lane takes the 16 bytes at dim 8 t + 32 i of key g (lane = 4 g +
+// t) for K, which are two k-steps of its B fragment, and the query the same; for V it takes 16
+// bytes at dim 8 g of keys 2t, 2t+1, 2t+8, 2t+9 and pairs two keys' elements with one byte
+// permutation each.  Nothing goes through shared memory, every load is 16 bytes and
+// 64 (K) or 128 (V) contiguous bytes a row.  The next tile's K loads start as soon as this
+// one's scores are formed, its V loads after this one's products.  P enters the second
+// product as two bf16 parts (p = hi + lo, 16 bits of it, so its rounding does not show
+// in the result); with at most 8 heads in a tile the rows 8..15 of the MMA, otherwise idle,
+// carry lo.  tcgen05 would add staging in shared memory and TMEM for a product of 8 rows that
+// the memory system bounds: the warp MMAs are busy for a fifth of the time that K and V take.
+//
+// fp32: a key's dims are spread over head_dim / 4 lanes; the partial dot products of several
+// keys and heads are summed by one butterfly that leaves one score per lane.
+//
+// Weights: a key's probability needs its row's final max and sum, so the first kernel stores
+// the scores and the second adds the probabilities (4 bytes per key and query head, written
+// and read back mostly in L2).
 
 #include <math.h>
 
@@ -18,83 +46,754 @@ struct PagedAttnArgs {
   void* out;
   int64_t q_stride, out_stride;
   const int* lengths;
-  int group;  // query heads per kv head
-  float scale;
+  int hq, group;    // query heads, and per kv head
+  float scale_log2; // scale * log2(e): exponentials are powers of two
   float* weights;
   int64_t w_row_stride, w_head_stride;
   int* err;
+  int head_tiles;   // of a kv head's query group
+  int ctas;
+  float* part_stat; // [ctas][2][NH][2]  max, sum
+  float* part_acc;  // [ctas][2][NH][HD]
+  float* row_stat;  // [rows][hq][2]     of units that one CTA finished (with weights)
+  float* scores;    // [rows][hq][score_stride] (with weights)
+  int64_t score_stride;
 };
 
-constexpr int kPagedWarps = 8;
+constexpr int kTile = 64;          // keys of a tile
+constexpr int kPagedWarps = 4;
+constexpr int kPagedThreads = kPagedWarps * 32;
+// CTAs of the first kernel per SM: what its registers allow without spilling.
+constexpr int paged_ctas_per_sm(bool bf16, int hd) { return bf16 && hd == 128 ? 2 : 3; }
+constexpr int kFinishThreads = 128;
+constexpr int kFinishKeys = 4 * kFinishThreads;  // keys whose weights one CTA adds to
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kPagedWarps * 32) paged_attn_simple_kernel(PagedAttnArgs a) {
-  constexpr int DPL = HD / 32;  // dims of a lane
-  const int h = blockIdx.x, row = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  __shared__ float sm_m[kPagedWarps], sm_l[kPagedWarps], sm_acc[kPagedWarps][HD];
+__device__ __forceinline__ int row_length(const PagedAttnArgs& a, int row) {
+  return min(max(a.lengths[row], 0), a.kv.slots());
+}
+__device__ __forceinline__ int row_tiles(const PagedAttnArgs& a, int row) {
+  return (row_length(a, row) + kTile - 1) / kTile;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Tiles of all rows (per unit of a row), and of those before `row`: sums over the CTA.
+template <int THREADS>
+__device__ __forceinline__ void count_tiles(const PagedAttnArgs& a, int row, int64_t* before, int64_t* total) {
+  __shared__ int64_t sm[2][THREADS / 32];
+  int64_t all = 0, pre = 0;
+  for (int b = threadIdx.x; b < a.kv.rows; b += THREADS) {
+    const int n = row_tiles(a, b);
+    all += n;
+    if (b < row) pre += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    pre += __shfl_xor_sync(0xffffffffu, pre, o);
+  }
+  if (threadIdx.x % 32 == 0) sm[0][threadIdx.x / 32] = all, sm[1][threadIdx.x / 32] = pre;
+  __syncthreads();
+  all = pre = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) all += sm[0][w], pre += sm[1][w];
+  *total = all;
+  *before = pre;
+}
+
+// What one warp carries over a unit's keys: bf16 form (see the head of the file).
+template <int HD, int NH>
+struct MmaCore {
+  using T = __nv_bfloat16;
+  static constexpr bool kBf16 = true;
+  static constexpr int kSub = 16;        // keys of one step of a warp
+  static constexpr int KC = HD / 32;     // 16-byte pieces of a K row per lane
+  static constexpr int VE = HD >= 64 ? 8 : HD / 8;  // dims of a V load
+  static constexpr int VC = HD / (8 * VE);          // V loads of a row per lane
+  static constexpr int NT = VC * VE;     // n-tiles of the output
+  static constexpr int HI = NH / 8;      // head rows of a lane: g (and g + 8)
+  static constexpr int kParts = 1;       // states of a warp
+  uint4 q[HI][KC];
+  uint4 kr[2][KC];
+  uint32_t vr[4][VC][VE / 2];
+  float acc[NT][4];
+  float m[HI], l[HI];
+  int64_t at[2], at_next[2];
+  int lim[2], lim_next[2];
+  int page[2];
+  int g, t;
+
+  __device__ __forceinline__ void init(const PagedAttnArgs& a, int row, int head0, int nh) {
+    const int lane = threadIdx.x % 32;
+    g = lane / 4;
+    t = lane % 4;
+#pragma unroll
+    for (int i = 0; i < HI; ++i) {
+      const bool real = g + 8 * i < nh;
+      const T* qr = static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)(head0 + g + 8 * i) * HD;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        q[i][c] = real ? *reinterpret_cast<const uint4*>(qr + 32 * c + 8 * t) : make_uint4(0, 0, 0, 0);
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+  }
+
+  // Page ids of the 16 keys at key0 (two halves of 8, which never straddle a page).
+  __device__ __forceinline__ void fetch_pages(const PagedAttnArgs& a, const int* trow, int key0, int end) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page[i] = key0 + 8 * i < end ? trow[(key0 + 8 * i) >> a.kv.ps_log2] : 0;
+  }
+  __device__ __forceinline__ void place(const PagedAttnArgs& a, int kvh, int key0, int end) {
+    const int mask = (1 << a.kv.ps_log2) - 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lim_next[i] = min(max(end - key0 - 8 * i, 0), 8);
+      if ((unsigned)page[i] >= (unsigned)a.kv.num_pages) {
+        if (lim_next[i] > 0) raise_flag(a.err);
+        lim_next[i] = 0;
+      }
+      at_next[i] = page[i] * a.kv.page_stride + (((int64_t)kvh << a.kv.ps_log2) + ((key0 + 8 * i) & mask)) * HD;
+    }
+  }
+  __device__ __forceinline__ void load_k(const PagedAttnArgs& a) {
+    const T* kp = static_cast<const T*>(a.kv.k);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        kr[i][c] = make_uint4(0, 0, 0, 0);
+        if (g < lim_next[i]) {
+          const int4 x = ld_once(reinterpret_cast<const int4*>(kp + at_next[i] + g * HD + 32 * c + 8 * t));
+          kr[i][c] = make_uint4(x.x, x.y, x.z, x.w);
+        }
+      }
+  }
+  __device__ __forceinline__ void load_v(const PagedAttnArgs& a) {
+    const T* vp = static_cast<const T*>(a.kv.v);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = r / 2, key = 2 * t + r % 2;
+#pragma unroll
+      for (int c = 0; c < VC; ++c) {
+#pragma unroll
+        for (int w = 0; w < VE / 2; ++w) vr[r][c][w] = 0;
+        if (key < lim[i]) {  // a slot behind the length may hold anything: 0 x NaN must not enter
+          const T* p = vp + at[i] + key * HD + 64 * c + VE * g;
+          if (VE == 8) {
+            const int4 x = ld_once(reinterpret_cast<const int4*>(p));
+            vr[r][c][0] = x.x;
+            vr[r][c][1] = x.y;
+            vr[r][c][VE / 2 - 2] = x.z;
+            vr[r][c][VE / 2 - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            vr[r][c][0] = x.x;
+            vr[r][c][1] = x.y;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void advance() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) at[i] = at_next[i], lim[i] = lim_next[i];
+  }
+
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+  static __device__ __forceinline__ float low(uint32_t p) { return __uint_as_float(p << 16); }
+  static __device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+  // The step's keys key0 .. key0 + 15; the caller loads the next step's K and V in between.
+  template <typename NextK>
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, int row, int head0, int nh, int key0, NextK&& next_k) {
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 q1 = HI > 1 ? q[HI - 1][c] : make_uint4(0, 0, 0, 0);
+        mma(s[i], q[0][c].x, q1.x, q[0][c].y, q1.y, kr[i][c].x, kr[i][c].y);
+        mma(s[i], q[0][c].z, q1.z, q[0][c].w, q1.w, kr[i][c].z, kr[i][c].w);
+      }
+    }
+    next_k();
+    uint32_t hi[2][HI], lo[2][HI];
+    float alpha[HI];
+    bool grew = false;
+#pragma unroll
+    for (int h = 0; h < HI; ++h) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[i][2 * h + e];
+          x = 2 * t + e < lim[i] ? x * a.scale_log2 : -INFINITY;
+          top = fmaxf(top, x);
+        }
+      if (a.scores && g + 8 * h < nh) {
+        float* sp = a.scores + ((int64_t)row * a.hq + head0 + g + 8 * h) * a.score_stride + key0 + 2 * t;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(sp + 8 * i) = make_float2(s[i][2 * h], s[i][2 * h + 1]);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float mn = fmaxf(m[h], top);
+      const float safe = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is 0, not NaN
+      grew |= mn > m[h];
+      alpha[h] = exp2_fast(m[h] - safe);
+      m[h] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float p0 = exp2_fast(s[i][2 * h] - safe), p1 = exp2_fast(s[i][2 * h + 1] - safe);
+        sum += p0 + p1;
+        hi[i][h] = pack2(p0, p1);
+        lo[i][h] = pack2(p0 - low(hi[i][h]), p1 - high(hi[i][h]));
+      }
+      l[h] = l[h] * alpha[h] + sum;
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] *= alpha[e / 2 < HI ? e / 2 : 0];
+    }
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int w = 0; w < VE / 2; ++w)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t b0 = __byte_perm(vr[0][c][w], vr[1][c][w], o ? 0x7632 : 0x5410);
+          const uint32_t b1 = __byte_perm(vr[2][c][w], vr[3][c][w], o ? 0x7632 : 0x5410);
+          float(&d)[4] = acc[c * VE + 2 * w + o];
+          if (HI == 1) {
+            mma(d, hi[0][0], lo[0][0], hi[1][0], lo[1][0], b0, b1);
+          } else {
+            mma(d, hi[0][0], hi[0][HI - 1], hi[1][0], hi[1][HI - 1], b0, b1);
+            mma(d, lo[0][0], lo[0][HI - 1], lo[1][0], lo[1][HI - 1], b0, b1);
+          }
+        }
+  }
+
+  // The state of part `warp` into shared memory: [parts][NH] max and sum, [parts][NH][HD] output.
+  __device__ __forceinline__ void store(float* sm_m, float* sm_l, float* sm_acc, int warp) {
+#pragma unroll
+    for (int h = 0; h < HI; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      const int at = warp * NH + g + 8 * h;
+      if (t == 0) sm_m[at] = m[h], sm_l[at] = l[h];
+      // column n of n-tile (c, j) is dim 8 VE c + VE n + j; this lane has columns 2t and 2t + 1
+#pragma unroll
+      for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < VE; j += 4) {
+            float4 x;
+            float* xs = &x.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float(&d)[4] = acc[c * VE + j + i];
+              xs[i] = HI == 1 ? d[e] + d[2 + e] : d[2 * h + e];
+            }
+            *reinterpret_cast<float4*>(sm_acc + at * HD + 8 * VE * c + (2 * t + e) * VE + j) = x;
+          }
+    }
+  }
+};
+
+// fp32 form.  A group of LPK lanes owns a key, NK keys a step; the NK * NH dot products of a
+// group are summed over its lanes by a butterfly that halves the number of values a lane
+// holds at each step, so one (key, head) is left per lane (or per LPK / N lanes).
+template <int HD, int NH>
+struct FmaCore {
+  using T = float;
+  static constexpr bool kBf16 = false;
+  static constexpr int LPK = HD / 4;
+  static constexpr int KG = 32 / LPK;
+  static constexpr int NK = LPK / NH < 8 ? LPK / NH : 8;
+  static constexpr int N = NK * NH;
+  static constexpr int REP = LPK / N;   // lanes that hold the same score
+  static constexpr int kSub = KG * NK;
+  static constexpr int kParts = KG;
+  float4 q[NH], acc[NH];
+  float m, l;
+  int page[NK];
+  int grp, sl, head, key_of;  // this lane's score: head, and key within the group's NK
+
+  __device__ __forceinline__ void init(const PagedAttnArgs& a, int row, int head0, int nh) {
+    const int lane = threadIdx.x % 32;
+    grp = lane / LPK;
+    sl = lane % LPK;
+    head = sl / REP % NH;
+    key_of = sl / REP / NH;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      q[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (h < nh)
+        q[h] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + row * a.q_stride +
+                                                (int64_t)(head0 + h) * HD + 4 * sl);
+      acc[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ void fetch_pages(const PagedAttnArgs& a, const int* trow, int key0, int end) {
+#pragma unroll
+    for (int u = 0; u < NK; ++u) {
+      const int key = key0 + grp * NK + u;
+      page[u] = key < end ? trow[key >> a.kv.ps_log2] : -1;
+    }
+  }
+  // One step over the keys whose pages were fetched; `end` bounds the keys.
+  template <typename Next>
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, int row, int kvh, int head0, int nh, int key0, int end,
+                                       Next&& next_pages) {
+    float4 k[NK], v[NK];
+    bool ok[NK];
+#pragma unroll
+    for (int u = 0; u < NK; ++u) {
+      const int key = key0 + grp * NK + u;
+      ok[u] = (unsigned)page[u] < (unsigned)a.kv.num_pages;
+      if (!ok[u] && key < end) raise_flag(a.err);
+      k[u] = v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ok[u]) {
+        const int64_t at = page[u] * a.kv.page_stride +
+                           (((int64_t)kvh << a.kv.ps_log2) + (key & ((1 << a.kv.ps_log2) - 1))) * HD + 4 * sl;
+        const int4 x = ld_once(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.k) + at));
+        const int4 y = ld_once(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.v) + at));
+        k[u] = make_float4(__int_as_float(x.x), __int_as_float(x.y), __int_as_float(x.z), __int_as_float(x.w));
+        v[u] = make_float4(__int_as_float(y.x), __int_as_float(y.y), __int_as_float(y.z), __int_as_float(y.w));
+      }
+    }
+    bool mine_ok = false;
+#pragma unroll
+    for (int u = 0; u < NK; ++u) mine_ok |= ok[u] && u == key_of;
+    next_pages();
+    float s[N];
+#pragma unroll
+    for (int u = 0; u < NK; ++u)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+        s[u * NH + h] = fmaf(q[h].x, k[u].x, fmaf(q[h].y, k[u].y, fmaf(q[h].z, k[u].z, q[h].w * k[u].w)));
+    int o = LPK / 2;
+#pragma unroll
+    for (int n = N; n > 1; n /= 2, o /= 2) {
+      const bool up = sl & o;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < n / 2) {
+          const float give = up ? s[i] : s[i + n / 2];
+          const float keep = up ? s[i + n / 2] : s[i];
+          s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+    float x = s[0];
+#pragma unroll
+    for (int r = REP / 2; r > 0; r /= 2) x += __shfl_xor_sync(0xffffffffu, x, r);
+    x = mine_ok ? x * a.scale_log2 : -INFINITY;
+    if (a.scores && sl % REP == 0 && head < nh) {
+      const int key = key0 + grp * NK + key_of;
+      if (key < end) a.scores[((int64_t)row * a.hq + head0 + head) * a.score_stride + key] = x;
+    }
+    float top = x;
+#pragma unroll
+    for (int r = REP * NH; r < LPK; r *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, r));
+    const float mn = fmaxf(m, top);
+    const float safe = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f(m - safe), p = exp2f(x - safe);
+    const bool grew = mn > m;
+    l = l * alpha + p;
+    m = mn;
+    const int base = grp * LPK;
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float f = __shfl_sync(0xffffffffu, alpha, base + h * REP);
+        acc[h].x *= f;
+        acc[h].y *= f;
+        acc[h].z *= f;
+        acc[h].w *= f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NK; ++u)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float f = __shfl_sync(0xffffffffu, p, base + (u * NH + h) * REP);
+        acc[h].x = fmaf(f, v[u].x, acc[h].x);
+        acc[h].y = fmaf(f, v[u].y, acc[h].y);
+        acc[h].z = fmaf(f, v[u].z, acc[h].z);
+        acc[h].w = fmaf(f, v[u].w, acc[h].w);
+      }
+  }
+  __device__ __forceinline__ void store(float* sm_m, float* sm_l, float* sm_acc, int warp) {
+#pragma unroll
+    for (int r = REP * NH; r < LPK; r *= 2) l += __shfl_xor_sync(0xffffffffu, l, r);
+    const int part = warp * KG + grp;
+    if (key_of == 0 && sl % REP == 0) sm_m[part * NH + head] = m, sm_l[part * NH + head] = l;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) *reinterpret_cast<float4*>(sm_acc + (part * NH + h) * HD + 4 * sl) = acc[h];
+  }
+};
+
+// One warp's keys of [begin, end) (begin a multiple of 64), the CTA's warps taking turns.
+template <int HD, int NH>
+__device__ __forceinline__ void walk(MmaCore<HD, NH>& core, const PagedAttnArgs& a, const int* trow, int row, int kvh,
+                                     int head0, int nh, int begin, int end, int warp) {
+  constexpr int S = MmaCore<HD, NH>::kSub, STRIDE = S * kPagedWarps;
+  int key0 = begin + warp * S;
+  if (key0 >= end) return;  // (the whole warp)
+  core.fetch_pages(a, trow, key0, end);
+  core.place(a, kvh, key0, end);
+  core.load_k(a);
+  core.advance();
+  core.load_v(a);
+  core.fetch_pages(a, trow, key0 + STRIDE, end);
+  for (; key0 < end; key0 += STRIDE) {
+    core.step(a, row, head0, nh, key0, [&] {
+      core.place(a, kvh, key0 + STRIDE, end);
+      core.fetch_pages(a, trow, key0 + 2 * STRIDE, end);
+      core.load_k(a);
+    });
+    core.advance();
+    core.load_v(a);
+  }
+}
+
+template <int HD, int NH>
+__device__ __forceinline__ void walk(FmaCore<HD, NH>& core, const PagedAttnArgs& a, const int* trow, int row, int kvh,
+                                     int head0, int nh, int begin, int end, int warp) {
+  constexpr int S = FmaCore<HD, NH>::kSub, STRIDE = S * kPagedWarps;
+  int key0 = begin + warp * S;
+  if (key0 >= end) return;
+  core.fetch_pages(a, trow, key0, end);
+  for (; key0 < end; key0 += STRIDE)
+    core.step(a, row, kvh, head0, nh, key0, end, [&] { core.fetch_pages(a, trow, key0 + STRIDE, end); });
+}
+
+template <typename Core, int HD, int NH>
+__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, HD)) paged_attn_kernel(PagedAttnArgs a) {
+  using T = typename Core::T;
+  constexpr int PARTS = kPagedWarps * Core::kParts;
+  __shared__ float sm_m[PARTS * NH], sm_l[PARTS * NH];
+  __shared__ __align__(16) float sm_acc[PARTS * NH * HD];
+  __shared__ int64_t sm_scan[kPagedWarps];
+  __shared__ int sm_row;
+  __shared__ int64_t sm_rest;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
   pdl_wait();
-  const int want = a.lengths[row];
-  const int len = min(max(want, 0), a.kv.slots());
-  if (len != want && threadIdx.x == 0) raise_flag(a.err);
-  const T* kp = static_cast<const T*>(a.kv.k);
-  const T* vp = static_cast<const T*>(a.kv.v);
-  for (int g = 0; g < a.group; ++g) {
-    const int head = h * a.group + g;
-    const T* qr = static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)head * HD;
-    float q[DPL], acc[DPL], m = -INFINITY, l = 0.f;
+  // where this CTA's range of tiles begins: thread i counts the tiles of rows [i per, (i + 1) per)
+  const int units = a.kv.hkv * a.head_tiles;
+  const int per = (a.kv.rows + kPagedThreads - 1) / kPagedThreads;
+  const int r0 = min(tid * per, a.kv.rows), r1 = min(r0 + per, a.kv.rows);
+  int64_t mine = 0;
+  for (int b = r0; b < r1; ++b) {
+    if (blockIdx.x == 0 && row_length(a, b) != a.lengths[b]) raise_flag(a.err);
+    mine += row_tiles(a, b);
+  }
+  int64_t scan = mine;
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) q[e] = to_f(qr[lane + 32 * e]), acc[e] = 0.f;
-    auto score = [&](int64_t at) {
-      float d = 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += y;
+  }
+  if (lane == 31) sm_scan[warp] = scan;
+  __syncthreads();
+  int64_t total = 0, before = scan - mine;
 #pragma unroll
-      for (int e = 0; e < DPL; ++e) d = fmaf(q[e], to_f(kp[at + lane + 32 * e]), d);
-      return warp_sum(d) * a.scale;
-    };
-    for (int j = warp; j < len; j += kPagedWarps) {
-      const int64_t at = a.kv.at<HD>(row, j, h);
-      if (at < 0) {
-        if (lane == 0) raise_flag(a.err);
-        continue;
-      }
-      const float s = score(at);
-      const float mn = fmaxf(m, s);
-      const float safe = mn == -INFINITY ? 0.f : mn;
-      const float alpha = expf(m - safe), p = expf(s - safe);
-#pragma unroll
-      for (int e = 0; e < DPL; ++e) acc[e] = fmaf(p, to_f(vp[at + lane + 32 * e]), acc[e] * alpha);
-      l = l * alpha + p;
-      m = mn;
+  for (int w = 0; w < kPagedWarps; ++w) {
+    if (w < warp) before += sm_scan[w];
+    total += sm_scan[w];
+  }
+  total *= units;
+  const int64_t ctas = min((int64_t)a.ctas, total);  // each of them has a tile at least
+  if (blockIdx.x >= ctas) return;
+  const int64_t lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1) * total / ctas;
+  if (lo >= before * units && lo < (before + mine) * units) {
+    int64_t at = before * units;
+    int b = r0;
+    for (;; ++b) {
+      const int64_t n = (int64_t)row_tiles(a, b) * units;
+      if (lo < at + n) break;
+      at += n;
+    }
+    sm_row = b;
+    sm_rest = lo - at;
+  }
+  __syncthreads();
+  int row = sm_row;
+  int tiles = row_tiles(a, row);
+  int unit = (int)(sm_rest / tiles), tile = (int)(sm_rest - (int64_t)unit * tiles);
+  for (int64_t left = hi - lo; left > 0;) {
+    const int len = row_length(a, row);
+    const int n = (int)min((int64_t)(tiles - tile), left);
+    const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
+    const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
+    {
+      Core core;
+      core.init(a, row, head0, nh);
+      walk<HD, NH>(core, a, a.kv.table + row * a.kv.table_stride, row, kvh, head0, nh, tile * kTile,
+                   min(len, (tile + n) * kTile), warp);
+      core.store(sm_m, sm_l, sm_acc, warp);
     }
     __syncthreads();
+    const bool whole = n == tiles;
+    // a partial that begins with the CTA's range is its slot 0, one that begins later its slot 1
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (left == hi - lo ? 0 : 1);
+    for (int i = tid; i < nh * HD; i += kPagedThreads) {
+      const int h = i / HD, d = i % HD;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) M = fmaxf(M, sm_m[w * NH + h]);
+      const float safe = M == -INFINITY ? 0.f : M;
+      float L = 0.f, A = 0.f;
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) {
+        const float f = exp2f(sm_m[w * NH + h] - safe);
+        L += sm_l[w * NH + h] * f;
+        A += sm_acc[(w * NH + h) * HD + d] * f;
+      }
+      if (whole) {
+        static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+        if (a.scores && d == 0) {
+          float* st = a.row_stat + ((int64_t)row * a.hq + head0 + h) * 2;
+          st[0] = safe;
+          st[1] = L;
+        }
+      } else {
+        a.part_acc[(slot * NH + h) * HD + d] = A;
+        if (d == 0) {
+          a.part_stat[(slot * NH + h) * 2] = M;
+          a.part_stat[(slot * NH + h) * 2 + 1] = L;
+        }
+      }
+    }
+    __syncthreads();
+    left -= n;
+    tile += n;
+    if (tile == tiles && left > 0) {
+      tile = 0;
+      if (++unit == units) {
+        unit = 0;
+        do ++row;
+        while ((tiles = row_tiles(a, row)) == 0);  // (tiles are left, so a row with some is)
+      }
+    }
+  }
+}
+
+// The CTAs that hold partials of tiles [start, start + n) of `total`: first .. last, and the
+// slot of the first one's.
+struct Holders {
+  int first, last, first_slot;
+};
+__device__ __forceinline__ Holders holders(int64_t start, int64_t n, int64_t total, int64_t ctas) {
+  Holders h;
+  h.first = (int)(((start + 1) * ctas + total - 1) / total) - 1;  // the largest c with c total / ctas <= start
+  h.last = (int)(((start + n) * ctas + total - 1) / total) - 1;
+  h.first_slot = h.first * total / ctas == start ? 0 : 1;
+  return h;
+}
+
+template <typename T, int HD, int NH>
+__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnArgs a, int join_ctas, int key_chunks) {
+  constexpr int WARPS = kFinishThreads / 32;
+  __shared__ float sm_m[WARPS], sm_l[WARPS], sm_acc[WARPS][HD];
+  __shared__ float sm_stat[32][2];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  pdl_trigger();
+  pdl_wait();
+  const bool join = (int)blockIdx.x < join_ctas;
+  int row, head, chunk = 0;
+  if (join) {
+    row = blockIdx.x / a.hq;
+    head = blockIdx.x - row * a.hq;
+  } else {
+    int r = blockIdx.x - join_ctas;
+    chunk = r % key_chunks;
+    r /= key_chunks;
+    row = r / a.kv.hkv;
+    head = (r - row * a.kv.hkv) * a.group;
+    if (chunk * kFinishKeys >= row_length(a, row)) return;
+  }
+  const int tiles = row_tiles(a, row);
+  if (tiles == 0) {  // nothing to attend to
+    for (int d = tid; d < HD; d += kFinishThreads)
+      static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(0.f);
+    return;
+  }
+  int64_t before, total;
+  count_tiles<kFinishThreads>(a, row, &before, &total);
+  const int units = a.kv.hkv * a.head_tiles;
+  total *= units;
+  auto holders_of = [&](int h) {
+    const int unit = h / a.group * a.head_tiles + h % a.group / NH;
+    return holders(before * units + (int64_t)unit * tiles, tiles, total, min((int64_t)a.ctas, total));
+  };
+  auto slot_of = [&](const Holders& p, int c) {
+    return ((int64_t)c * 2 + (c == p.first ? p.first_slot : 0)) * NH;
+  };
+  if (join) {
+    const Holders p = holders_of(head);
+    if (p.first == p.last) return;  // written by its one CTA
+    const int hl = head % a.group % NH;
+    constexpr int DPL = HD / 32;
+    float m = -INFINITY, l = 0.f, acc[DPL];
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
+    for (int c = p.first + warp; c <= p.last; c += WARPS) {
+      const int64_t s = slot_of(p, c) + hl;
+      const float pm = a.part_stat[s * 2], pl = a.part_stat[s * 2 + 1];
+      const float mn = fmaxf(m, pm);
+      const float safe = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2f(m - safe), pf = exp2f(pm - safe);
+      l = l * f + pl * pf;
+#pragma unroll
+      for (int e = 0; e < DPL; ++e) acc[e] = acc[e] * f + a.part_acc[s * HD + lane + 32 * e] * pf;
+      m = mn;
+    }
     if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
 #pragma unroll
     for (int e = 0; e < DPL; ++e) sm_acc[warp][lane + 32 * e] = acc[e];
     __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < kPagedWarps; ++w) M = fmaxf(M, sm_m[w]);
-    const float safe = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < kPagedWarps; ++w) L += sm_l[w] * expf(sm_m[w] - safe);
-    for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-      float A = 0.f;
-      for (int w = 0; w < kPagedWarps; ++w) A += sm_acc[w][d] * expf(sm_m[w] - safe);
+    for (int d = tid; d < HD; d += kFinishThreads) {
+      float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w]);
+      const float safe = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(sm_m[w] - safe);
+        L += sm_l[w] * f;
+        A += sm_acc[w][d] * f;
+      }
       static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
     }
-    if (a.weights)
-      for (int j = warp; j < len; j += kPagedWarps) {
-        const int64_t at = a.kv.at<HD>(row, j, h);
-        if (at < 0) continue;
-        const float s = score(at);
-        if (lane == 0) a.weights[row * a.w_row_stride + h * a.w_head_stride + j] += L > 0.f ? expf(s - safe) / L : 0.f;
+    return;
+  }
+  // the probabilities of this CTA's keys, summed over the group's heads in order
+  const int len = row_length(a, row);
+  float sum[kFinishKeys / kFinishThreads];
+#pragma unroll
+  for (int i = 0; i < kFinishKeys / kFinishThreads; ++i) sum[i] = 0.f;
+  for (int h0 = 0; h0 < a.group; h0 += 32) {
+    const int nh = min(32, a.group - h0);
+    __syncthreads();
+    for (int i = warp; i < nh; i += WARPS) {  // a warp per head: the unit's max and sum
+      const int h = head + h0 + i;
+      const Holders p = holders_of(h);
+      float m = -INFINITY, l = 0.f;
+      if (p.first == p.last) {
+        m = a.row_stat[((int64_t)row * a.hq + h) * 2];
+        l = a.row_stat[((int64_t)row * a.hq + h) * 2 + 1];
+      } else {
+        const int hl = h % a.group % NH;
+        for (int c = p.first + lane; c <= p.last; c += 32) m = fmaxf(m, a.part_stat[(slot_of(p, c) + hl) * 2]);
+        m = warp_max(m);
+        if (m == -INFINITY) m = 0.f;
+        for (int c = p.first + lane; c <= p.last; c += 32) {
+          const float* st = a.part_stat + (slot_of(p, c) + hl) * 2;
+          l += st[1] * exp2f(st[0] - m);
+        }
+        l = warp_sum(l);
       }
+      if (lane == 0) sm_stat[i][0] = m, sm_stat[i][1] = l > 0.f ? 1.f / l : 0.f;
+    }
+    __syncthreads();
+    for (int i = 0; i < nh; ++i) {
+      const float m = sm_stat[i][0], inv = sm_stat[i][1];
+      const float* sp = a.scores + ((int64_t)row * a.hq + head + h0 + i) * a.score_stride;
+#pragma unroll
+      for (int u = 0; u < kFinishKeys / kFinishThreads; ++u) {
+        const int key = chunk * kFinishKeys + u * kFinishThreads + tid;
+        if (key < len) sum[u] += exp2f(sp[key] - m) * inv;
+      }
+    }
+  }
+  float* w = a.weights + row * a.w_row_stride + (int64_t)(head / a.group) * a.w_head_stride;
+#pragma unroll
+  for (int u = 0; u < kFinishKeys / kFinishThreads; ++u) {
+    const int key = chunk * kFinishKeys + u * kFinishThreads + tid;
+    if (key < len) w[key] += sum[u];
   }
 }
 
-static cudaError_t paged_attention(const PagedAttnArgs& a, int hd, int dtype, cudaStream_t st) {
-  return dispatch_type_dim(dtype, hd, [&](auto t, auto d) {
-    return launch_pdl(paged_attn_simple_kernel<decltype(t), decltype(d)::value>, dim3(a.kv.hkv, a.kv.rows),
-                      dim3(kPagedWarps * 32), 0, st, a);
-  });
+
+// Query heads of a tile: the smallest tile that holds the group, up to 16 (bf16) or 8 (fp32) heads.
+static int head_tile(int dtype, int group) {
+  if (dtype == PIM_BF16) return group <= 8 ? 8 : 16;
+  return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
+}
+
+// CTAs of the first kernel: as many as are resident at once on the current device (148 SMs if
+// there is none: the workspace of a call can be asked for anywhere).
+static int paged_ctas(int dtype, int hd) {
+  static int sms[64];
+  const int per_sm = paged_ctas_per_sm(dtype == PIM_BF16, hd);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    (void)cudaGetLastError();
+    return 148 * per_sm;
+  }
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 148;
+    }
+    sms[dev] = n;
+  }
+  return sms[dev] * per_sm;
+}
+
+template <typename Core, int HD, int NH>
+static cudaError_t launch_paged(const PagedAttnArgs& a, cudaStream_t st) {
+  using T = typename Core::T;
+  cudaError_t e = launch_pdl(paged_attn_kernel<Core, HD, NH>, dim3(a.ctas), dim3(kPagedThreads), 0, st, a);
+  if (e != cudaSuccess) return e;
+  const int join = a.kv.rows * a.hq;
+  const int chunks = a.weights ? ceil_div((int64_t)a.kv.max_pages << a.kv.ps_log2, kFinishKeys) : 0;
+  const int64_t grid = join + (int64_t)a.kv.rows * a.kv.hkv * chunks;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  return launch_pdl(paged_finish_kernel<T, HD, NH>, dim3((unsigned)grid), dim3(kFinishThreads), 0, st, a, join,
+                    chunks ? chunks : 1);
+}
+
+template <int HD>
+static cudaError_t paged_attention_hd(const PagedAttnArgs& a, int dtype, int nh, cudaStream_t st) {
+  if (dtype == PIM_BF16)
+    return nh == 8 ? launch_paged<MmaCore<HD, 8>, HD, 8>(a, st)
+                   : launch_paged<MmaCore<HD, 16>, HD, 16>(a, st);
+  if (nh == 1) return launch_paged<FmaCore<HD, 1>, HD, 1>(a, st);
+  if (nh == 2) return launch_paged<FmaCore<HD, 2>, HD, 2>(a, st);
+  if (nh == 4) return launch_paged<FmaCore<HD, 4>, HD, 4>(a, st);
+  return launch_paged<FmaCore<HD, 8>, HD, 8>(a, st);
 }
 
 // nullptr, or what is wrong with the arguments.
@@ -118,11 +817,38 @@ static const char* paged_attention_error(const pim_paged_attention_args* a, int 
   return nullptr;
 }
 
+// The parts of the workspace, as byte offsets.
+struct PagedLayout {
+  int nh, tiles, ctas;
+  int64_t score_stride, acc, row_stat, scores, bytes;
+};
+static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
+  PagedLayout p;
+  const int group = a->q_heads / a->kv.kv_heads;
+  p.nh = head_tile(dtype, group);
+  p.tiles = ceil_div(group, p.nh);
+  p.ctas = paged_ctas(dtype, a->kv.head_dim);
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  const int64_t parts = (int64_t)p.ctas * 2 * p.nh;
+  p.acc = up(parts * 2 * 4);
+  p.row_stat = p.acc + up(parts * a->kv.head_dim * 4);
+  p.score_stride = 0;
+  p.scores = p.bytes = p.row_stat;
+  if (a->weights) {
+    const int64_t heads = (int64_t)a->kv.rows * a->q_heads;
+    p.score_stride = ((int64_t)a->kv.max_pages * a->kv.page_size + 63) / 64 * 64;
+    p.scores = p.row_stat + up(heads * 2 * 4);
+    p.bytes = p.scores + heads * p.score_stride * 4;
+  }
+  return p;
+}
+
 }  // namespace pim
 
 extern "C" int64_t pim_paged_attention_workspace_bytes(const pim_paged_attention_args* a, int32_t dtype) {
-  if (pim::paged_attention_error(a, dtype)) return -1;
-  return 0;
+  using namespace pim;
+  if (paged_attention_error(a, dtype)) return -1;
+  return paged_layout(a, dtype).bytes;
 }
 
 extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dtype, void* workspace,
@@ -133,8 +859,8 @@ extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dt
     snprintf(msg, sizeof(msg), "pim_paged_attention: %s", e);
     return report_status(PIM_EINVAL, msg);
   }
-  const int64_t need = pim_paged_attention_workspace_bytes(a, dtype);
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+  const PagedLayout p = paged_layout(a, dtype);
+  if (!workspace || workspace_bytes < p.bytes || !aligned16(workspace))
     return report_status(PIM_EINVAL, "pim_paged_attention: workspace too small or not 16-byte aligned");
   PagedAttnArgs d{};
   d.kv = to_dev(a->kv);
@@ -143,11 +869,28 @@ extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dt
   d.q_stride = a->q_stride;
   d.out_stride = a->out_stride;
   d.lengths = a->lengths;
+  d.hq = a->q_heads;
   d.group = a->q_heads / a->kv.kv_heads;
-  d.scale = a->scale > 0.f ? a->scale : (float)(1.0 / sqrt((double)a->kv.head_dim));
+  const double scale = a->scale > 0.f ? a->scale : 1.0 / sqrt((double)a->kv.head_dim);
+  d.scale_log2 = (float)(scale * 1.4426950408889634);  // log2(e)
   d.weights = a->weights;
   d.w_row_stride = a->weights_row_stride;
   d.w_head_stride = a->weights_head_stride;
   d.err = a->err_flag;
-  return report_cuda(paged_attention(d, a->kv.head_dim, dtype, (cudaStream_t)stream), "pim_paged_attention");
+  d.head_tiles = p.tiles;
+  d.ctas = p.ctas;
+  char* ws = static_cast<char*>(workspace);
+  d.part_stat = reinterpret_cast<float*>(ws);
+  d.part_acc = reinterpret_cast<float*>(ws + p.acc);
+  if (a->weights) {
+    d.row_stat = reinterpret_cast<float*>(ws + p.row_stat);
+    d.scores = reinterpret_cast<float*>(ws + p.scores);
+    d.score_stride = p.score_stride;
+  }
+  const int hd = a->kv.head_dim;
+  cudaStream_t st = (cudaStream_t)stream;
+  return report_cuda(hd == 128  ? paged_attention_hd<128>(d, dtype, p.nh, st)
+                     : hd == 64 ? paged_attention_hd<64>(d, dtype, p.nh, st)
+                                : paged_attention_hd<32>(d, dtype, p.nh, st),
+                     "pim_paged_attention");
 }

@@ -60,6 +60,16 @@ __device__ __forceinline__ int4 ld_stream(const int4* p) {
   return r;
 }
 
+// 16-byte load of data that is read once and that another grid may have written after this
+// one started (programmatic dependent launch), after pdl_wait(): not the read-only path.
+__device__ __forceinline__ int4 ld_once(const int4* p) {
+  int4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 // Elements of T per 16-byte vector.
 template <typename T>
 struct VecW {
