@@ -7,11 +7,15 @@
 // largest logits: beam_partial_kernel reads every logit once, into registers, and leaves per
 // chunk the sorted K largest (as 64-bit keys: the logit's order-preserving bits above the
 // complement of its token, so keys are unique and equal logits rank by token) and the
-// chunk's maximum and sum of exponentials.  K-th largest of a chunk: it is at least the K-th
-// largest of the threads' maxima, and only K threads can hold values at or above that bound, so
-// at most K * 16 keys are left to rank by counting.  beam_merge_kernel joins the sums to the
-// beams' lse in fp64 (neighbouring candidates decide which tokens come out) and merges the
-// sorted lists: K rounds of a maximum over the lists' heads.
+// chunk's maximum and sum of exponentials.  beam_merge_kernel joins the sums to the beams' lse
+// in fp64 (neighbouring candidates decide which tokens come out), merges each beam's lists
+// with one warp and then the beams.
+//
+// The K largest of a chunk: if every warp's ceil(K / warps)-th largest lane maximum is at least
+// tau, then K values are, so only those >= tau, a few times K of them, are collected and ranked
+// by counting.  Finding tau costs one warp reduction per rank instead of a sort.  Many equal
+// logits can make the collection overflow; then the K-th largest of the threads' (unique)
+// 64-bit maxima is the bound, and only K threads can hold keys at or above it.
 //
 // Reordering.  See pim_beam_reorder in pim_b200.h: the table entries of full pages follow
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
@@ -27,6 +31,7 @@ constexpr int kBeamThreads = 256;
 constexpr int kBeamVals = 16;  // logits of a thread
 constexpr int kBeamChunk = kBeamThreads * kBeamVals;
 constexpr int kMaxBeams = 64;
+constexpr int kMaxSplits = 128;
 
 struct BeamStats {
   float max;
@@ -46,97 +51,128 @@ struct BeamSelectArgs {
   unsigned long long* lists;  // [batch * beams][splits][k]
 };
 
-// A logit's key: larger is better; 0 for a logit that is no candidate.
-__device__ __forceinline__ unsigned long long beam_key(float x, int token) {
+// The bits of a logit in unsigned order; 0 for a logit that is no candidate.
+__device__ __forceinline__ uint32_t logit_order(float x) {
   if (!isfinite(x)) return 0;
-  const uint32_t u = __float_as_uint(x + 0.f);
-  const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
-  return ((unsigned long long)o << 32) | (uint32_t)~token;
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 and +0 are equal
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float key_logit(unsigned long long key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+__device__ __forceinline__ float order_logit(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// A candidate's key: larger is better.
+__device__ __forceinline__ unsigned long long beam_key(uint32_t order, int token) {
+  return ((unsigned long long)order << 32) | (uint32_t)~token;
 }
 __device__ __forceinline__ int key_token(unsigned long long key) { return (int)~(uint32_t)key; }
+
+// The largest of the lanes' 64-bit keys: two 32-bit warp reductions.
+__device__ __forceinline__ unsigned long long warp_best(unsigned long long key) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+  return ((unsigned long long)hi << 32) | lo;
+}
+
+constexpr int kBeamWarps = kBeamThreads / 32;
+constexpr int kBeamCand = kMaxBeams * kBeamVals;
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectArgs a) {
   constexpr int V = VecW<T>::n;
-  __shared__ unsigned long long sm_max[kBeamThreads];
-  __shared__ unsigned long long sm_cand[kMaxBeams * kBeamVals];
+  __shared__ unsigned long long sm_cand[kBeamCand];
+  __shared__ uint32_t sm_top[kBeamWarps], sm_low[kBeamWarps];
+  __shared__ double sm_s[kBeamWarps];
   __shared__ unsigned long long sm_tau;
   __shared__ int sm_n;
-  __shared__ float sm_m[kBeamThreads / 32];
-  __shared__ double sm_s[kBeamThreads / 32];
   const int split = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
   pdl_wait();
   if (a.done && a.done[row]) return;  // offers one candidate, which the merge adds
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   const int base = split * kBeamChunk;
-  float v[kBeamVals];
+  uint32_t o[kBeamVals];
   // value i of this thread is token base + tok(i)
   auto tok = [&](int i) { return ALIGNED ? (i / V) * kBeamThreads * V + tid * V + i % V : i * kBeamThreads + tid; };
-#pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) v[i] = -INFINITY;
   if (ALIGNED) {
     int4 raw[kBeamVals / V];
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i)
-      if (base + tok(i * V) < a.vocab) raw[i] = ld_once(reinterpret_cast<const int4*>(x + base + tok(i * V)));
+      raw[i] = ld_once_if(reinterpret_cast<const int4*>(x + base + tok(i * V)), base + tok(i * V) < a.vocab);
 #pragma unroll
-    for (int i = 0; i < kBeamVals / V; ++i)
-      if (base + tok(i * V) < a.vocab) {
-        float f[V];
-        unpack(raw[i], f, T());
+    for (int i = 0; i < kBeamVals / V; ++i) {
+      float f[V];
+      unpack(raw[i], f, T());
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i * V + e] = f[e];
-      }
+      for (int e = 0; e < V; ++e) o[i * V + e] = base + tok(i * V) < a.vocab ? logit_order(f[e]) : 0;
+    }
   } else {
+    float f[kBeamVals];
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i)
-      if (base + tok(i) < a.vocab) v[i] = to_f(x[base + tok(i)]);
-  }
-  unsigned long long mine = 0;
+    for (int i = 0; i < kBeamVals; ++i) f[i] = base + tok(i) < a.vocab ? to_f(x[base + tok(i)]) : -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) {
-    if (!isfinite(v[i])) v[i] = -INFINITY;
-    const unsigned long long k = beam_key(v[i], base + tok(i));
-    mine = k > mine ? k : mine;
+    for (int i = 0; i < kBeamVals; ++i) o[i] = logit_order(f[i]);
   }
-  sm_max[tid] = mine;
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < kBeamVals; ++i) mine = max(mine, o[i]);
+  const int rounds = (a.k + kBeamWarps - 1) / kBeamWarps;
+  uint32_t cur = mine, low = 0;
+  for (int r = 0; r < rounds; ++r) {
+    low = __reduce_max_sync(0xffffffffu, cur);
+    if (r == 0 && lane == 0) sm_top[warp] = low;
+    const unsigned who = __ballot_sync(0xffffffffu, cur == low);
+    if (lane == __ffs(who) - 1) cur = 0;
+  }
+  if (lane == 0) sm_low[warp] = low;
   if (tid == 0) sm_n = 0, sm_tau = 1;
-  const float wm = warp_max(mine ? key_logit(mine) : -INFINITY);
-  if (lane == 0) sm_m[warp] = wm;
   __syncthreads();
-  float m = sm_m[0];
+  uint32_t top = sm_top[0], tau = sm_low[0];
 #pragma unroll
-  for (int w = 1; w < kBeamThreads / 32; ++w) m = fmaxf(m, sm_m[w]);
-  // fp32 exponentials and a thread's 16 of them; the sum over threads in fp64
-  float part = 0.f;
-  if (m != -INFINITY) {
-#pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) part += expf(v[i] - m);
-  }
-  double s = part;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) sm_s[warp] = s;
-  // the k-th largest of the threads' maxima bounds the chunk's k-th largest from below
-  int above = 0;
-  for (int i = 0; i < kBeamThreads; ++i) above += sm_max[i] > mine;
-  if (mine && above == a.k - 1) sm_tau = mine;
-  __syncthreads();
-  const unsigned long long tau = sm_tau;
+  for (int w = 1; w < kBeamWarps; ++w) top = max(top, sm_top[w]), tau = min(tau, sm_low[w]);
+  tau = max(tau, 1u);  // (0: not a candidate)
   if (mine >= tau) {
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) {
-      const unsigned long long k = beam_key(v[i], base + tok(i));
-      if (k >= tau) sm_cand[atomicAdd(&sm_n, 1)] = k;  // at most k threads come here, with 16 keys each
-    }
+    for (int i = 0; i < kBeamVals; ++i)
+      if (o[i] >= tau) {
+        const int at = atomicAdd(&sm_n, 1);
+        if (at < kBeamCand) sm_cand[at] = beam_key(o[i], base + tok(i));
+      }
   }
+  // fp32 exponentials and a thread's 16 of them; the sum over threads in fp64
+  const float m = top ? order_logit(top) : -INFINITY;
+  float part = 0.f;
+#pragma unroll
+  for (int i = 0; i < kBeamVals; ++i) part += o[i] ? expf(order_logit(o[i]) - m) : 0.f;
+  double s = part;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (lane == 0) sm_s[warp] = s;
   __syncthreads();
-  const int n = sm_n, out = min(n, a.k);
+  int n = sm_n;
+  if (n > kBeamCand) {  // too many equal to the bound: the exact one
+    unsigned long long best = 0;
+#pragma unroll
+    for (int i = 0; i < kBeamVals; ++i) {
+      const unsigned long long k = o[i] ? beam_key(o[i], base + tok(i)) : 0;
+      best = k > best ? k : best;
+    }
+    __syncthreads();
+    sm_cand[tid] = best;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < kBeamThreads; ++i) above += sm_cand[i] > best;
+    if (best && above == a.k - 1) sm_tau = best;
+    if (tid == 0) sm_n = 0;
+    __syncthreads();
+    const unsigned long long bound = sm_tau;
+    if (best >= bound) {
+#pragma unroll
+      for (int i = 0; i < kBeamVals; ++i) {
+        const unsigned long long k = o[i] ? beam_key(o[i], base + tok(i)) : 0;
+        if (k >= bound) sm_cand[atomicAdd(&sm_n, 1)] = k;  // at most k threads come here, with 16 keys each
+      }
+    }
+    __syncthreads();
+    n = sm_n;
+  }
   unsigned long long* list = a.lists + ((int64_t)row * a.splits + split) * a.k;
   for (int i = tid; i < n; i += kBeamThreads) {
     const unsigned long long k = sm_cand[i];
@@ -147,118 +183,126 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   if (tid == 0) {
     BeamStats st;
     st.max = m;
-    st.count = out;
+    st.count = min(n, a.k);
     st.sum = 0;
-    for (int w = 0; w < kBeamThreads / 32; ++w) st.sum += sm_s[w];
+    for (int w = 0; w < kBeamWarps; ++w) st.sum += sm_s[w];
     a.stats[(int64_t)row * a.splits + split] = st;
   }
 }
 
-struct BeamBest {
-  double score;   // -inf: none
-  int64_t flat;   // beam * vocab + token
-};
-__device__ __forceinline__ bool better(const BeamBest& x, const BeamBest& y) {
-  return x.score > y.score || (x.score == y.score && x.flat < y.flat);
+constexpr int kMergeThreads = 512;
+constexpr int kListsPerLane = kMaxSplits / 32;
+
+// Order-preserving bits of a finite double, never 0.
+__device__ __forceinline__ unsigned long long score_order(double s) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(s + 0.0);
+  return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-constexpr int kMergeThreads = 256;
-
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArgs a) {
-  extern __shared__ unsigned char sm_next[];  // [beams * splits] entries of each list that are taken
-  __shared__ double sm_shift[kMaxBeams];      // score_w - lse_w; -inf: the beam offers nothing
+  __shared__ unsigned long long sm_keys[kMaxBeams * kMaxBeams];  // [beams][k], sorted, 0: none
+  __shared__ double sm_shift[kMaxBeams];                         // score_w - lse_w
   __shared__ int sm_done[kMaxBeams];
-  __shared__ BeamBest sm_best[kMergeThreads / 32];
-  __shared__ int sm_list[kMergeThreads / 32];
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
   pdl_wait();
-  const int lists = a.beams * a.splits;
-  for (int i = tid; i < lists; i += kMergeThreads) sm_next[i] = 0;
-  for (int w = warp; w < a.beams; w += kMergeThreads / 32) {
+  for (int w = warp; w < a.beams; w += kMergeThreads / 32) {  // a warp per beam
     const int row = b * a.beams + w;
     const int done = a.done ? a.done[row] : 0;
     const float score = a.scores[row];
-    double shift = score;
-    if (!done) {
-      float m = -INFINITY;
-      for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, a.stats[(int64_t)row * a.splits + i].max);
-      m = warp_max(m);
-      double s = 0;
-      if (m != -INFINITY)
-        for (int i = lane; i < a.splits; i += 32) {
-          const BeamStats st = a.stats[(int64_t)row * a.splits + i];
-          if (st.max != -INFINITY) s += st.sum * exp((double)st.max - (double)m);
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      shift = m == -INFINITY ? -INFINITY : (double)score - ((double)m + log(s));
+    unsigned long long* keys = sm_keys + w * a.k;
+    if (done || !isfinite(score)) {
+      for (int j = lane; j < a.k; j += 32) keys[j] = j == 0 && isfinite(score) ? beam_key(0x80000000u, a.pad) : 0;
+      if (lane == 0) sm_shift[w] = score, sm_done[w] = done;
+      continue;
     }
+    // lane i merges lists i, i + 32, ..: the first two keys of each are at hand
+    unsigned long long head[kListsPerLane], next[kListsPerLane];
+    int taken[kListsPerLane], count[kListsPerLane];
+    float lm[kListsPerLane];
+    double ls[kListsPerLane];
+    const unsigned long long* lists = a.lists + (int64_t)row * a.splits * a.k;
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kListsPerLane; ++q) {
+      const int l = lane + 32 * q;
+      head[q] = next[q] = 0;
+      taken[q] = count[q] = 0;
+      lm[q] = -INFINITY;
+      ls[q] = 0;
+      if (l < a.splits) {
+        const BeamStats st = a.stats[(int64_t)row * a.splits + l];
+        const unsigned long long h = lists[(int64_t)l * a.k], n = a.k > 1 ? lists[(int64_t)l * a.k + 1] : 0;
+        lm[q] = st.max;
+        ls[q] = st.sum;
+        count[q] = st.count;
+        head[q] = st.count > 0 ? h : 0;  // (entries behind the count are not written)
+        next[q] = st.count > 1 ? n : 0;
+      }
+      m = fmaxf(m, lm[q]);
+    }
+    m = warp_max(m);
+    double s = 0;
+#pragma unroll
+    for (int q = 0; q < kListsPerLane; ++q)
+      if (lm[q] != -INFINITY) s += ls[q] * exp((double)lm[q] - (double)m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
-      sm_shift[w] = isfinite(score) ? shift : -INFINITY;
-      sm_done[w] = done;
+      sm_shift[w] = m == -INFINITY ? 0.0 : (double)score - ((double)m + log(s));
+      sm_done[w] = 0;
+    }
+    for (int j = 0; j < a.k; ++j) {
+      unsigned long long mine = head[0];
+#pragma unroll
+      for (int q = 1; q < kListsPerLane; ++q) mine = head[q] > mine ? head[q] : mine;
+      const unsigned long long best = warp_best(mine);
+      if (lane == 0) keys[j] = best;
+      if (best == 0) continue;  // (the warp agrees)
+#pragma unroll
+      for (int q = 0; q < kListsPerLane; ++q)
+        if (head[q] == best) {  // keys are unique: one list of one lane
+          head[q] = next[q];
+          ++taken[q];
+          next[q] = taken[q] + 1 < count[q] ? lists[(int64_t)(lane + 32 * q) * a.k + taken[q] + 1] : 0;
+        }
     }
   }
   __syncthreads();
-  // the head of list l
-  auto head = [&](int l) {
-    BeamBest c{-INFINITY, INT64_MAX};
-    const int w = l / a.splits, split = l - w * a.splits, at = sm_next[l];
-    if (sm_shift[w] == -INFINITY) return c;
-    if (sm_done[w]) {
-      if (split == 0 && at == 0) c.score = sm_shift[w], c.flat = (int64_t)w * a.vocab + a.pad;
-      return c;
-    }
-    const int64_t list = (int64_t)(b * a.beams + w) * a.splits + split;
-    if (at >= a.stats[list].count) return c;
-    const unsigned long long k = a.lists[list * a.k + at];
-    c.score = sm_shift[w] + (double)key_logit(k);
-    c.flat = (int64_t)w * a.vocab + key_token(k);
-    return c;
+  if (warp != 0) return;
+  // lane w merges the lists of beams w and w + 32; of equal scores the lower beam is first
+  int at[2] = {0, 0};
+  unsigned long long score[2];
+  auto look = [&](int i) {
+    const int w = lane + 32 * i;
+    const unsigned long long k = w < a.beams && at[i] < a.k ? sm_keys[w * a.k + at[i]] : 0;
+    score[i] = k ? score_order(sm_shift[w] + (sm_done[w] ? 0.0 : (double)order_logit((uint32_t)(k >> 32)))) : 0;
   };
-  BeamBest mine{-INFINITY, INT64_MAX};
-  int mine_list = -1;
-  auto refresh = [&]() {
-    mine = BeamBest{-INFINITY, INT64_MAX};
-    for (int l = tid; l < lists; l += kMergeThreads) {
-      const BeamBest c = head(l);
-      if (better(c, mine)) mine = c, mine_list = l;
-    }
-  };
-  refresh();
+  look(0);
+  look(1);
   for (int j = 0; j < a.k; ++j) {
-    BeamBest best = mine;
-    int from = mine_list;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      BeamBest other;
-      other.score = __shfl_xor_sync(0xffffffffu, best.score, o);
-      other.flat = __shfl_xor_sync(0xffffffffu, (long long)best.flat, o);
-      const int of = __shfl_xor_sync(0xffffffffu, from, o);
-      if (better(other, best)) best = other, from = of;
-    }
-    __syncthreads();
-    if (lane == 0) sm_best[warp] = best, sm_list[warp] = from;
-    __syncthreads();
-    best = sm_best[0];
-    from = sm_list[0];
-#pragma unroll
-    for (int w = 1; w < kMergeThreads / 32; ++w)
-      if (better(sm_best[w], best)) best = sm_best[w], from = sm_list[w];
-    const bool none = best.score == -INFINITY;
-    const int parent = none ? 0 : (int)(best.flat / a.vocab);
-    const int token = none ? a.pad : (int)(best.flat - (int64_t)parent * a.vocab);
-    if (tid == 0) {
-      const int64_t o = (int64_t)b * a.k + j;
-      a.scores_out[o] = (float)best.score;
-      a.parents[o] = parent;
+    const unsigned long long best = warp_best(score[0] > score[1] ? score[0] : score[1]);
+    const unsigned low = __ballot_sync(0xffffffffu, score[0] == best), high = __ballot_sync(0xffffffffu, score[1] == best);
+    const int i = low ? 0 : 1, from = __ffs(low ? low : high) - 1;
+    const int64_t o = (int64_t)b * a.k + j;
+    if (best == 0) {
+      if (lane == 0) {
+        a.scores_out[o] = -INFINITY;
+        a.parents[o] = 0;
+        a.tokens[o] = a.pad;
+        if (a.done_out) a.done_out[o] = 1;
+      }
+    } else if (lane == from) {
+      const int w = lane + 32 * i, token = key_token(sm_keys[w * a.k + at[i]]);
+      const unsigned long long u = best >> 63 ? best & ~(1ull << 63) : ~best;
+      a.scores_out[o] = (float)__longlong_as_double((long long)u);
+      a.parents[o] = w;
       a.tokens[o] = token;
-      if (a.done_out) a.done_out[o] = none || sm_done[parent] || (a.eos >= 0 && token == a.eos);
+      if (a.done_out) a.done_out[o] = sm_done[w] || (a.eos >= 0 && token == a.eos);
+      ++at[i];
+      look(i);
     }
-    if (!none && from % kMergeThreads == tid) {
-      sm_next[from]++;
-      refresh();
-    }
+    __syncwarp();
   }
 }
 
@@ -273,7 +317,10 @@ struct BeamReorderArgs {
   int* err;
 };
 
-__global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
+constexpr int kReorderThreads = 256;
+constexpr int kCopyPieces = 4 * kReorderThreads;
+
+__global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(BeamReorderArgs a) {
   __shared__ int sm_parent[kMaxBeams], sm_page[kMaxBeams], sm_first[kMaxBeams], sm_childless[kMaxBeams];
   __shared__ int sm_bad, sm_take;
   const int row = blockIdx.x, b = row / a.beams, j = row - b * a.beams, tid = threadIdx.x;
@@ -326,15 +373,25 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(BeamReorderArgs a) {
     }
   }
   if (!copies) return;
+  // 16-byte pieces of the slots in use, kCopyPieces of them per step of a CTA, four in flight per thread
   const int per_head = fill * a.row_bytes / 16, head_pieces = a.row_bytes << a.ps_log2 >> 4;
-  for (int blk = blockIdx.y; blk < a.num_blocks; blk += gridDim.y) {
+  const int pieces = a.hkv * per_head, steps = (pieces + kCopyPieces - 1) / kCopyPieces;
+  for (int64_t item = blockIdx.y; item < (int64_t)a.num_blocks * steps; item += gridDim.y) {
+    const int blk = (int)(item / steps), i0 = (int)(item - (int64_t)blk * steps) * kCopyPieces + tid;
     char* block = a.pages + blk * a.block_bytes;
     const int4* src = reinterpret_cast<const int4*>(block + sm_page[parent] * a.page_bytes);
     int4* dst = reinterpret_cast<int4*>(block + sm_page[take] * a.page_bytes);
-    for (int i = tid; i < a.hkv * per_head; i += blockDim.x) {
-      const int h = i / per_head, r = i - h * per_head;
-      dst[(int64_t)h * head_pieces + r] = src[(int64_t)h * head_pieces + r];
+    int4 v[kCopyPieces / kReorderThreads];
+    int64_t off[kCopyPieces / kReorderThreads];
+#pragma unroll
+    for (int u = 0; u < kCopyPieces / kReorderThreads; ++u) {
+      const int i = i0 + u * kReorderThreads, h = i / per_head;
+      off[u] = (int64_t)h * head_pieces + (i - h * per_head);
+      v[u] = ld_once_if(src + off[u], i < pieces);
     }
+#pragma unroll
+    for (int u = 0; u < kCopyPieces / kReorderThreads; ++u)
+      if (i0 + u * kReorderThreads < pieces) dst[off[u]] = v[u];
   }
 }
 
@@ -344,8 +401,8 @@ static const char* beam_select_error(const pim_beam_select_args* a, int dtype) {
   if (!a->logits || !a->scores || !a->scores_out || !a->parents || !a->tokens) return "null pointer";
   if (a->batch <= 0 || a->beams <= 0 || a->beams > kMaxBeams || a->beams_out <= 0 || a->beams_out > kMaxBeams)
     return "batch must be positive, beams and beams_out 1 to 64";
-  if (a->vocab <= 0 || a->vocab > (1 << 22) || (int64_t)a->batch * a->beams > 65535)
-    return "vocab must be 1 to 2^22, batch * beams at most 65535";
+  if (a->vocab <= 0 || a->vocab > kMaxSplits * kBeamChunk || (int64_t)a->batch * a->beams > 65535)
+    return "vocab must be 1 to 2^19, batch * beams at most 65535";
   if (a->logits_stride < a->vocab) return "logits_stride is less than vocab";
   if ((uintptr_t)a->logits % elem_bytes(dtype)) return "logits are not aligned to their type";
   if (a->eos < -1 || a->eos >= a->vocab || a->pad < 0 || a->pad >= a->vocab) return "eos or pad outside the vocabulary";
@@ -362,15 +419,15 @@ static int64_t beam_stats_bytes(const pim_beam_select_args* a) {
 
 template <typename T>
 static cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t st) {
-  const bool aligned = aligned16(a.logits) && a.stride * sizeof(T) % 16 == 0 && a.vocab % VecW<T>::n == 0;
+  // 16-byte loads where rows allow them; a vocabulary that leaves most warps of such a chunk empty is read by
+  // element, which spreads it over all of them
+  const bool aligned = aligned16(a.logits) && a.stride * sizeof(T) % 16 == 0 && a.vocab % VecW<T>::n == 0 &&
+                       a.vocab >= kBeamThreads * VecW<T>::n;
   const dim3 grid(a.splits, a.batch * a.beams);
   cudaError_t e = aligned ? launch_pdl(beam_partial_kernel<T, true>, grid, dim3(kBeamThreads), 0, st, a)
                           : launch_pdl(beam_partial_kernel<T, false>, grid, dim3(kBeamThreads), 0, st, a);
   if (e != cudaSuccess) return e;
-  static ResidentCache cache;
-  const size_t smem = ((size_t)a.beams * a.splits + 15) / 16 * 16;
-  if (resident_ctas(beam_merge_kernel, kMergeThreads, smem, cache, &e) < 0) return e;
-  return launch_pdl(beam_merge_kernel, dim3(a.batch), dim3(kMergeThreads), smem, st, a);
+  return launch_pdl(beam_merge_kernel, dim3(a.batch), dim3(kMergeThreads), 0, st, a);
 }
 
 }  // namespace pim
@@ -454,7 +511,12 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   d.hkv = a->kv_heads;
   d.row_bytes = a->head_dim * es;
   d.err = a->err_flag;
-  const int by = a->num_blocks < 65535 ? a->num_blocks : 65535;
-  return report_cuda(launch_pdl(beam_reorder_kernel, dim3(a->batch * a->beams, by), dim3(256), 0, (cudaStream_t)stream, d),
+  // About a third of the rows copy: enough CTAs per row that those fill the GPU, and no more than there are steps.
+  const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
+  const int rows = a->batch * a->beams;
+  int64_t by = ceil_div(8 * 148, rows);
+  by = by < steps ? by : steps;
+  return report_cuda(launch_pdl(beam_reorder_kernel, dim3(rows, (unsigned)by), dim3(kReorderThreads), 0,
+                                (cudaStream_t)stream, d),
                      "pim_beam_reorder");
 }

@@ -149,7 +149,8 @@ struct MmaCore {
   // Page ids of the 16 keys at key0 (two halves of 8, which never straddle a page).
   __device__ __forceinline__ void fetch_pages(const PagedAttnArgs& a, const int* trow, int key0, int end) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) page[i] = key0 + 8 * i < end ? trow[(key0 + 8 * i) >> a.kv.ps_log2] : 0;
+    for (int i = 0; i < 2; ++i)
+      page[i] = (int)ld4_if(trow + ((key0 + 8 * i) >> a.kv.ps_log2), key0 + 8 * i < end);
   }
   __device__ __forceinline__ void place(const PagedAttnArgs& a, int kvh, int key0, int end) {
     const int mask = (1 << a.kv.ps_log2) - 1;
@@ -169,11 +170,9 @@ struct MmaCore {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        kr[i][c] = make_uint4(0, 0, 0, 0);
-        if (g < lim_next[i]) {
-          const int4 x = ld_once(reinterpret_cast<const int4*>(kp + at_next[i] + g * HD + 32 * c + 8 * t));
-          kr[i][c] = make_uint4(x.x, x.y, x.z, x.w);
-        }
+        const int4 x = ld_once_if(reinterpret_cast<const int4*>(kp + at_next[i] + g * HD + 32 * c + 8 * t),
+                                  g < lim_next[i]);
+        kr[i][c] = make_uint4(x.x, x.y, x.z, x.w);
       }
   }
   __device__ __forceinline__ void load_v(const PagedAttnArgs& a) {
@@ -183,21 +182,18 @@ struct MmaCore {
       const int i = r / 2, key = 2 * t + r % 2;
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
-#pragma unroll
-        for (int w = 0; w < VE / 2; ++w) vr[r][c][w] = 0;
-        if (key < lim[i]) {  // a slot behind the length may hold anything: 0 x NaN must not enter
-          const T* p = vp + at[i] + key * HD + 64 * c + VE * g;
-          if (VE == 8) {
-            const int4 x = ld_once(reinterpret_cast<const int4*>(p));
-            vr[r][c][0] = x.x;
-            vr[r][c][1] = x.y;
-            vr[r][c][VE / 2 - 2] = x.z;
-            vr[r][c][VE / 2 - 1] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            vr[r][c][0] = x.x;
-            vr[r][c][1] = x.y;
-          }
+        // a slot behind the length may hold anything, and 0 x NaN must not enter: it is not read, but zero
+        const bool ok = key < lim[i];
+        const T* p = vp + at[i] + key * HD + 64 * c + VE * g;
+        if (VE == 8) {
+          const int4 x = ld_once_if(reinterpret_cast<const int4*>(p), ok);
+          vr[r][c][0] = x.x;
+          vr[r][c][1] = x.y;
+          vr[r][c][VE / 2 - 2] = x.z;
+          vr[r][c][VE / 2 - 1] = x.w;
+        } else {
+          vr[r][c][0] = ld4_if(p, ok);
+          vr[r][c][1] = ld4_if(p + 2, ok);
         }
       }
     }
@@ -366,7 +362,8 @@ struct FmaCore {
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
       const int key = key0 + grp * NK + u;
-      page[u] = key < end ? trow[key >> a.kv.ps_log2] : -1;
+      const uint32_t id = ld4_if(trow + (key >> a.kv.ps_log2), key < end);
+      page[u] = key < end ? (int)id : -1;
     }
   }
   // One step over the keys whose pages were fetched; `end` bounds the keys.
@@ -380,15 +377,12 @@ struct FmaCore {
       const int key = key0 + grp * NK + u;
       ok[u] = (unsigned)page[u] < (unsigned)a.kv.num_pages;
       if (!ok[u] && key < end) raise_flag(a.err);
-      k[u] = v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ok[u]) {
-        const int64_t at = page[u] * a.kv.page_stride +
-                           (((int64_t)kvh << a.kv.ps_log2) + (key & ((1 << a.kv.ps_log2) - 1))) * HD + 4 * sl;
-        const int4 x = ld_once(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.k) + at));
-        const int4 y = ld_once(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.v) + at));
-        k[u] = make_float4(__int_as_float(x.x), __int_as_float(x.y), __int_as_float(x.z), __int_as_float(x.w));
-        v[u] = make_float4(__int_as_float(y.x), __int_as_float(y.y), __int_as_float(y.z), __int_as_float(y.w));
-      }
+      const int64_t at = page[u] * a.kv.page_stride +
+                         (((int64_t)kvh << a.kv.ps_log2) + (key & ((1 << a.kv.ps_log2) - 1))) * HD + 4 * sl;
+      const int4 x = ld_once_if(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.k) + at), ok[u]);
+      const int4 y = ld_once_if(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.v) + at), ok[u]);
+      k[u] = make_float4(__int_as_float(x.x), __int_as_float(x.y), __int_as_float(x.z), __int_as_float(x.w));
+      v[u] = make_float4(__int_as_float(y.x), __int_as_float(y.y), __int_as_float(y.z), __int_as_float(y.w));
     }
     bool mine_ok = false;
 #pragma unroll

@@ -33,7 +33,7 @@ struct EvictArgs {
   int smem_keys;  // keys that fit the shared memory of the launch
 };
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512;
 constexpr int kMaxSmemKeys = 48 * 1024;
 constexpr int kMoveThreads = 256;
 
@@ -57,24 +57,20 @@ __device__ __forceinline__ int cta_scan(int v, int* sm, int* total) {
   __syncthreads();
   if (lane == 31) sm[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    int s = sm[lane];
+  int before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    sm[lane] = s;
+  for (int w = 0; w < kSelThreads / 32; ++w) {
+    if (w < warp) before += sm[w];
+    all += sm[w];
   }
-  __syncthreads();
-  *total = sm[31];
-  return x - v + (warp ? sm[warp - 1] : 0);
+  *total = all;
+  return x - v + before;
 }
 
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t keys[];
   __shared__ int hist[2048];
-  __shared__ int sm_scan[32];
+  __shared__ int sm_scan[kSelThreads / 32];
   __shared__ int sm_bin, sm_above;
   const int head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   pdl_trigger();
@@ -89,25 +85,37 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   const int64_t base = row * a.row_stride + head * a.head_stride;
   const float* w = a.weights + base;
   const int* sp = a.slot_positions + base;
-  if (a.weights_out != a.weights)
-    for (int j = tid; j < left; j += kSelThreads) a.weights_out[base + j] = w[j];
-  if (a.slot_positions_out != a.slot_positions)
-    for (int j = tid; j < left; j += kSelThreads) a.slot_positions_out[base + j] = sp[j];
   const int unit = row * a.kv.hkv + head;
-  if (n <= a.budget) {
+  const bool copy_w = a.weights_out != a.weights, copy_p = a.slot_positions_out != a.slot_positions;
+  // (int64: a position near the type's ends less `recent` must not wrap)
+  const int64_t from = (int64_t)a.positions[row] - a.recent;
+  auto make_key = [&](float wt, int p) { return p >= from || p < a.sink ? 0xffffffffu : order_key(wt); };
+  const bool evicts = n > a.budget, in_smem = n <= a.smem_keys;
+  // one pass over the state, kLoads slots of a thread in flight: the kept part's copy and the keys
+  constexpr int kLoads = 8;
+  for (int j = tid; j < n; j += kLoads * kSelThreads) {
+    float wt[kLoads];
+    int p[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      wt[u] = __uint_as_float(ld4_if(w + j + u * kSelThreads, j + u * kSelThreads < n));
+      p[u] = (int)ld4_if(sp + j + u * kSelThreads, j + u * kSelThreads < n);
+    }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int i = j + u * kSelThreads;
+      if (i < left) {
+        if (copy_w) a.weights_out[base + i] = wt[u];
+        if (copy_p) a.slot_positions_out[base + i] = p[u];
+      }
+      if (i < n && evicts && in_smem) keys[i] = make_key(wt[u], p[u]);
+    }
+  }
+  if (!evicts) {
     if (tid == 0 && a.max_moves > 0) a.counts[unit] = 0;
     return;
   }
-  // (int64: a position near the type's ends less `recent` must not wrap)
-  const int64_t from = (int64_t)a.positions[row] - a.recent;
-  auto make_key = [&](int j) {
-    const int p = sp[j];
-    return p >= from || p < a.sink ? 0xffffffffu : order_key(w[j]);
-  };
-  const bool in_smem = n <= a.smem_keys;
-  if (in_smem)
-    for (int j = tid; j < n; j += kSelThreads) keys[j] = make_key(j);
-  auto key = [&](int j) { return in_smem ? keys[j] : make_key(j); };
+  auto key = [&](int j) { return in_smem ? keys[j] : make_key(w[j], sp[j]); };
   // the budget-th largest key
   uint32_t prefix = 0;
   int need = a.budget, shift = 32;
@@ -123,13 +131,17 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
       if ((k & top) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    // thread t owns the two bins 2047 - 2t and 2046 - 2t, so the scan runs from the largest bin down
-    const int b1 = 2047 - 2 * tid, b0 = b1 - 1;
-    const int c1 = hist[b1], c0 = hist[b0];
-    int total;
-    const int above = cta_scan(c1 + c0, sm_scan, &total);
-    if (above < need && need <= above + c1) sm_bin = b1, sm_above = above;
-    if (above + c1 < need && need <= above + c1 + c0) sm_bin = b0, sm_above = above + c1;
+    // thread t owns the bins 2047 - 4t .. 2044 - 4t, so the scan runs from the largest bin down
+    constexpr int OWN = 2048 / kSelThreads;
+    int c[OWN], sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) sum += c[i] = hist[2047 - OWN * tid - i];
+    int above = cta_scan(sum, sm_scan, &total);
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      if (above < need && need <= above + c[i]) sm_bin = 2047 - OWN * tid - i, sm_above = above;
+      above += c[i];
+    }
     __syncthreads();
     prefix |= (uint32_t)sm_bin << shift;
     need -= sm_above;
@@ -169,25 +181,52 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   }
 }
 
+// Up to kWarpMoves moves of a unit's list by one warp.  Each lane finds one row (the freed or the
+// kept slot of a move: one table entry), then all lanes copy 16-byte pieces, eight loads under
+// way at a time, with the rows' places taken from the lanes that know them.
+constexpr int kWarpMoves = 16;
 template <typename T, int HD>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictArgs a, int moves_per_cta) {
-  constexpr int LPR = HD * (int)sizeof(T) / 16;  // 16-byte pieces of a K or V row
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves, int row, int head, int count) {
+  constexpr int LPR = HD * (int)sizeof(T) / 16;        // pieces of a K or V row
+  constexpr int STEPS = kWarpMoves * 2 * LPR / 32, FLY = STEPS < 8 ? STEPS : 8;
+  const int lane = threadIdx.x % 32, mine = lane % kWarpMoves;
+  int64_t at = -1;
+  if (mine < count) {
+    const int2 mv = moves[mine];
+    at = a.kv.at<HD>(row, lane < kWarpMoves ? mv.x : mv.y, head);
+    if (at < 0) raise_flag(a.err);
+  }
+  for (int s0 = 0; s0 < STEPS; s0 += FLY) {
+    int4 v[FLY];
+    int64_t to[FLY];
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      const int flat = (s0 + u) * 32 + lane, m = flat / (2 * LPR), r = flat % (2 * LPR), piece = r % LPR;
+      const int64_t src = __shfl_sync(0xffffffffu, at, kWarpMoves + m);
+      to[u] = __shfl_sync(0xffffffffu, at, m);
+      T* p = static_cast<T*>(r < LPR ? a.kv.k : a.kv.v);
+      if (src < 0) to[u] = -1;
+      v[u] = ld_once_if(reinterpret_cast<const int4*>(p + src) + piece, to[u] >= 0);
+    }
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      const int r = ((s0 + u) * 32 + lane) % (2 * LPR), piece = r % LPR;
+      T* p = static_cast<T*>(r < LPR ? a.kv.k : a.kv.v);
+      if (to[u] >= 0) reinterpret_cast<int4*>(p + to[u])[piece] = v[u];
+    }
+  }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictArgs a) {
+  constexpr int WARPS = kMoveThreads / 32;
   const int unit = blockIdx.x, row = unit / a.kv.hkv, head = unit - row * a.kv.hkv;
   pdl_trigger();
   pdl_wait();
   const int count = a.counts[unit];
-  const int m0 = blockIdx.y * moves_per_cta, m1 = min(count, m0 + moves_per_cta);
-  for (int i = m0 * 2 * LPR + threadIdx.x; i < m1 * 2 * LPR; i += kMoveThreads) {
-    const int m = i / (2 * LPR), r = i % (2 * LPR), piece = r % LPR;
-    const int2 mv = a.moves[(int64_t)unit * a.max_moves + m];
-    const int64_t to = a.kv.at<HD>(row, mv.x, head), from = a.kv.at<HD>(row, mv.y, head);
-    if (to < 0 || from < 0) {
-      raise_flag(a.err);
-      continue;
-    }
-    T* p = static_cast<T*>(r < LPR ? a.kv.k : a.kv.v);
-    reinterpret_cast<int4*>(p + to)[piece] = reinterpret_cast<const int4*>(p + from)[piece];
-  }
+  for (int64_t m = (int64_t)(blockIdx.y * WARPS + threadIdx.x / 32) * kWarpMoves; m < count;
+       m += (int64_t)gridDim.y * WARPS * kWarpMoves)
+    move_rows<T, HD>(a, a.moves + (int64_t)unit * a.max_moves + m, row, head, count - (int)m);
 }
 
 static int64_t evict_max_moves(const pim_paged_evict_args* a) {
@@ -225,10 +264,9 @@ static cudaError_t evict(EvictArgs& a, int hd, int dtype, cudaStream_t st) {
   e = launch_pdl(evict_select_kernel, dim3(a.kv.hkv, a.kv.rows), dim3(kSelThreads), (size_t)a.smem_keys * 4, st, a);
   if (e != cudaSuccess || a.max_moves == 0) return e;
   return dispatch_type_dim(dtype, hd, [&](auto t, auto d) {
-    // at least 32 moves a CTA; gridDim.y stays within its limit at the longest rows
-    const int per = (int)(a.max_moves / 32 > 65535 ? (a.max_moves + 65534) / 65535 : 32);
+    const int by = ceil_div(a.max_moves, kWarpMoves * kMoveThreads / 32);
     return launch_pdl(evict_move_kernel<decltype(t), decltype(d)::value>,
-                      dim3(a.kv.rows * a.kv.hkv, ceil_div(a.max_moves, per)), dim3(kMoveThreads), 0, st, a, per);
+                      dim3(a.kv.rows * a.kv.hkv, by < 65535 ? by : 65535), dim3(kMoveThreads), 0, st, a);
   });
 }
 

@@ -481,7 +481,7 @@ typedef struct pim_beam_select_args {
   int32_t* done_out;        /* [batch, beams_out] the parent had ended or the token is `eos`; may be NULL */
   int32_t batch, beams;     /* beams <= 64 */
   int32_t beams_out;        /* <= 64 */
-  int32_t vocab;
+  int32_t vocab;            /* <= 2^19 */
   int32_t eos;              /* -1: no such token */
   int32_t pad;              /* the token a beam that has ended continues with, 0 <= pad < vocab */
 } pim_beam_select_args;
@@ -492,7 +492,8 @@ typedef struct pim_beam_select_args {
  * logit that is not finite is no candidate and no part of the sum; a beam whose score is
  * not finite offers none.  Where fewer than beams_out candidates are left, the rest get
  * score -inf, parent 0, token `pad`, done 1.  Candidates of one beam are compared by their
- * logits, those of different beams by their scores in fp64; scores_out is rounded once.
+ * logits, those of different beams by their scores in fp64 (of equal ones the lower beam is
+ * first); scores_out is rounded once.
  * Stands beside pim_argmax (greedy sampling, docs/spec.md:1552-1556). */
 int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
                     void* stream);

@@ -130,7 +130,7 @@ def _beam(**kw):
 @pytest.mark.parametrize("kw,message", [
     (dict(logits=None), "null"), (dict(tokens=None), "null"), (dict(beams=65), "beams"), (dict(beams_out=0), "beams"),
     (dict(beams_out=65), "beams"), (dict(batch=0), "batch"), (dict(batch=20000), "batch"), (dict(vocab=0), "vocab"),
-    (dict(vocab=1 << 23, logits_stride=1 << 23), "vocab"), (dict(logits_stride=999), "logits_stride"),
+    (dict(vocab=(1 << 19) + 1, logits_stride=1 << 20), "vocab"), (dict(logits_stride=999), "logits_stride"),
     (dict(logits=P + 1), "aligned"), (dict(eos=1000), "eos"), (dict(pad=-1), "pad"), (dict(pad=1000), "pad"),
     (dict(scores_out=P), "of their own"), (dict(done=P, done_out=P), "of their own")])
 def test_beam_select_refusals(kw, message):
