@@ -4,10 +4,10 @@
 // above every weight; the budget largest stay, of equal ones the lower slot.  The selection
 // is a radix select: weights map to unsigned keys of the same order, three passes over
 // 11 + 11 + 10 bits find the key of the budget-th largest and how many equal to it stay.
-// A scan in slot order then lists the freed slots below the budget and the kept ones above
-// it; there are equally many, and moving the i-th kept one into the i-th freed slot moves the
-// fewest rows that any compaction can.  Sources lie at or above the budget and destinations
-// below it, so the moves need no order.
+// The kept slots as bit words, scanned in slot order, then list the freed slots below the
+// budget and the kept ones above it; there are equally many, and moving the i-th kept one into
+// the i-th freed slot moves the fewest rows that any compaction can.  Sources lie at or above
+// the budget and destinations below it, so the moves need no order.
 //
 // evict_select_kernel: one CTA per (row, head), keys in shared memory where they fit; it
 // reads 8 bytes a slot and writes the state and the list of moves.  evict_move_kernel: moves
@@ -30,12 +30,14 @@ struct EvictArgs {
   int* counts;   // [rows * hkv] moves
   int2* moves;   // [rows * hkv][max_moves] (freed slot, kept slot)
   int max_moves;
-  int smem_keys;  // keys that fit the shared memory of the launch
+  int64_t page_pieces;  // 16-byte pieces between pages
 };
 
 constexpr int kSelThreads = 512;
 constexpr int kMaxSmemKeys = 48 * 1024;
+constexpr int kChunkWords = kMaxSmemKeys / 32;
 constexpr int kMoveThreads = 256;
+constexpr int kFusedMoves = 256;  // see evict()
 
 // Unsigned key of the same order as the weight; NaN lowest.  -0 and +0 are equal.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -46,18 +48,18 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 // Exclusive prefix sum over the CTA (kSelThreads threads); *total: the sum.
-__device__ __forceinline__ int cta_scan(int v, int* sm, int* total) {
+__device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* sm, uint32_t* total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int x = v;
+  uint32_t x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 31) sm[warp] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  uint32_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kSelThreads / 32; ++w) {
     if (w < warp) before += sm[w];
@@ -67,15 +69,59 @@ __device__ __forceinline__ int cta_scan(int v, int* sm, int* total) {
   return x - v + before;
 }
 
+// Up to kWarpMoves moves of a unit's list by one warp.  Each lane finds one row (the freed or the
+// kept slot of a move: one table entry), then all lanes copy 16-byte pieces (LPR of them are a K or
+// V row), eight loads under way at a time, with the rows' places taken from the lanes that know them.
+constexpr int kWarpMoves = 16;
+template <int LPR>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves, int row, int head, int count) {
+  constexpr int STEPS = kWarpMoves * 2 * LPR / 32, FLY = STEPS < 8 ? STEPS : 8;
+  const int lane = threadIdx.x % 32, mine = lane % kWarpMoves;
+  int64_t at = -1;  // in pieces
+  if (mine < count) {
+    const int2 mv = moves[mine];
+    const int slot = lane < kWarpMoves ? mv.x : mv.y;
+    const int page = a.kv.table[row * a.kv.table_stride + (slot >> a.kv.ps_log2)];
+    if ((unsigned)page < (unsigned)a.kv.num_pages)
+      at = page * a.page_pieces + (((int64_t)head << a.kv.ps_log2) + (slot & ((1 << a.kv.ps_log2) - 1))) * LPR;
+    else
+      raise_flag(a.err);
+  }
+  for (int s0 = 0; s0 < STEPS; s0 += FLY) {
+    int4 v[FLY];
+    int64_t to[FLY];
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      const int flat = (s0 + u) * 32 + lane, m = flat / (2 * LPR), r = flat % (2 * LPR), piece = r % LPR;
+      const int64_t src = __shfl_sync(0xffffffffu, at, kWarpMoves + m);
+      to[u] = __shfl_sync(0xffffffffu, at, m);
+      const int4* p = static_cast<const int4*>(r < LPR ? a.kv.k : a.kv.v);
+      if (src < 0) to[u] = -1;
+      v[u] = ld_once_if(p + src + piece, to[u] >= 0);
+    }
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      const int r = ((s0 + u) * 32 + lane) % (2 * LPR), piece = r % LPR;
+      int4* p = static_cast<int4*>(r < LPR ? a.kv.k : a.kv.v);
+      if (to[u] >= 0) p[to[u] + piece] = v[u];
+    }
+  }
+}
+
+// SMEM: the keys of a row fit the shared memory.  LPR: 0, or the CTA moves its rows itself.
+template <bool SMEM, int LPR>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[2048];
-  __shared__ int sm_scan[kSelThreads / 32];
-  __shared__ int sm_bin, sm_above;
-  const int head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t sm_more[kChunkWords], sm_equal[kChunkWords];
+  __shared__ uint32_t sm_scan[kSelThreads / 32];
+  __shared__ uint32_t sm_bin, sm_above, sm_count;
+  const int head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
   pdl_trigger();
   pdl_wait();
   const int want = a.lengths[row];
+  const int64_t next = a.positions[row];
   const int n = min(max(want, 0), a.kv.slots());
   const int left = min(n, a.budget);
   if (head == 0 && tid == 0) {
@@ -88,10 +134,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   const int unit = row * a.kv.hkv + head;
   const bool copy_w = a.weights_out != a.weights, copy_p = a.slot_positions_out != a.slot_positions;
   // (int64: a position near the type's ends less `recent` must not wrap)
-  const int64_t from = (int64_t)a.positions[row] - a.recent;
+  const int64_t from = next - a.recent;
   auto make_key = [&](float wt, int p) { return p >= from || p < a.sink ? 0xffffffffu : order_key(wt); };
-  const bool evicts = n > a.budget, in_smem = n <= a.smem_keys;
-  // one pass over the state, kLoads slots of a thread in flight: the kept part's copy and the keys
+  const bool evicts = n > a.budget;
+  __syncthreads();
+  // one pass over the state, kLoads slots of a thread in flight: the kept part's copy, the keys and the first
+  // histogram
   constexpr int kLoads = 8;
   for (int j = tid; j < n; j += kLoads * kSelThreads) {
     float wt[kLoads];
@@ -108,116 +156,117 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
         if (copy_w) a.weights_out[base + i] = wt[u];
         if (copy_p) a.slot_positions_out[base + i] = p[u];
       }
-      if (i < n && evicts && in_smem) keys[i] = make_key(wt[u], p[u]);
+      if (i < n && evicts) {
+        const uint32_t k = make_key(wt[u], p[u]);
+        if (SMEM) keys[i] = k;
+        atomicAdd(&hist[k >> 21], 1);
+      }
     }
   }
   if (!evicts) {
-    if (tid == 0 && a.max_moves > 0) a.counts[unit] = 0;
+    if (LPR == 0 && tid == 0) a.counts[unit] = 0;
     return;
   }
-  auto key = [&](int j) { return in_smem ? keys[j] : make_key(w[j], sp[j]); };
+  auto key = [&](int j) { return SMEM ? keys[j] : make_key(w[j], sp[j]); };
   // the budget-th largest key
-  uint32_t prefix = 0;
-  int need = a.budget, shift = 32;
+  uint32_t prefix = 0, need = a.budget;
+  int shift = 32;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int bits = pass < 2 ? 11 : 10, bins = 1 << bits;
-    const uint32_t top = pass ? ~0u << shift : 0;  // bits fixed so far
-    shift -= bits;
-    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += kSelThreads) {
-      const uint32_t k = key(j);
-      if ((k & top) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+    if (pass) {
+      const uint32_t top = ~0u << shift;  // bits fixed so far
+      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      for (int j = tid; j < n; j += kSelThreads) {
+        const uint32_t k = key(j);
+        if ((k & top) == prefix) atomicAdd(&hist[(k >> (shift - bits)) & (bins - 1)], 1);
+      }
     }
+    shift -= bits;
     __syncthreads();
     // thread t owns the bins 2047 - 4t .. 2044 - 4t, so the scan runs from the largest bin down
     constexpr int OWN = 2048 / kSelThreads;
-    int c[OWN], sum = 0, total;
+    uint32_t c[OWN], sum = 0, total;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) sum += c[i] = hist[2047 - OWN * tid - i];
-    int above = cta_scan(sum, sm_scan, &total);
+    uint32_t above = cta_scan(sum, sm_scan, &total);
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      if (above < need && need <= above + c[i]) sm_bin = 2047 - OWN * tid - i, sm_above = above;
+      if (above < need && need <= above + c[i]) sm_bin = 2047 - OWN * tid - i, sm_above = above, sm_count = c[i];
       above += c[i];
     }
     __syncthreads();
-    prefix |= (uint32_t)sm_bin << shift;
+    prefix |= sm_bin << shift;
     need -= sm_above;
   }
-  // prefix: the smallest key kept; `need` of those equal to it stay, the lowest slots first.
-  // A thread owns consecutive slots (an odd number of them: no shared-memory bank conflicts).
-  const int per = ((n + kSelThreads - 1) / kSelThreads) | 1;
-  const int j0 = min((int64_t)tid * per, (int64_t)n), j1 = min(j0 + per, n);
-  int total, eq = 0;
-  for (int j = j0; j < j1; ++j) eq += key(j) == prefix;
-  const int eq0 = cta_scan(eq, sm_scan, &total);
-  int holes = 0, sources = 0, e = eq0;
-  for (int j = j0; j < j1; ++j) {
-    const uint32_t k = key(j);
-    const bool keep = k > prefix || (k == prefix && e++ < need);
-    holes += !keep && j < a.budget;
-    sources += keep && j >= a.budget;
-  }
-  const int h0 = cta_scan(holes, sm_scan, &total);
-  int moved;
-  const int s0 = cta_scan(sources, sm_scan, &moved);
+  // prefix: the smallest key kept; `need` of the sm_count equal to it stay, the lowest slots first
+  const bool ties = need < sm_count;
   int2* mv = a.moves + (int64_t)unit * a.max_moves;
-  int hi = h0, si = s0;
-  e = eq0;
-  for (int j = j0; j < j1; ++j) {
-    const uint32_t k = key(j);
-    const bool keep = k > prefix || (k == prefix && e++ < need);
-    if (!keep && j < a.budget) mv[hi++].x = j;
-    if (keep && j >= a.budget) mv[si++].y = j;
+  uint32_t moved_to = 0, moved_from = 0;
+  for (int c0 = 0; c0 < n; c0 += kMaxSmemKeys) {  // (one round where SMEM)
+    const int m = min(n - c0, kMaxSmemKeys), words = (m + 31) / 32;
+    for (int i = warp; i < words; i += kSelThreads / 32) {
+      const int j = c0 + 32 * i + lane;
+      const uint32_t k = j < n ? key(j) : 0;
+      const uint32_t more = __ballot_sync(0xffffffffu, j < n && k > prefix);
+      const uint32_t equal = __ballot_sync(0xffffffffu, j < n && k == prefix);
+      if (lane == 0) sm_more[i] = more, sm_equal[i] = equal;
+    }
+    __syncthreads();
+    const int per = (words + kSelThreads - 1) / kSelThreads;
+    const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    uint32_t total;
+    if (ties) {
+      uint32_t count = 0;
+      for (int i = w0; i < w1; ++i) count += __popc(sm_equal[i]);
+      uint32_t before = cta_scan(count, sm_scan, &total);
+      for (int i = w0; i < w1; ++i) {
+        uint32_t rest = sm_equal[i], keep = 0;
+        for (; rest && before < need; ++before) {
+          keep |= rest & (0u - rest);
+          rest &= rest - 1;
+        }
+        before += __popc(rest);
+        sm_equal[i] = keep;
+      }
+      need -= min(need, total);
+    }
+    // the slots of word i that a move frees (below the budget) or takes its row from (above it)
+    auto freed = [&](int i) {
+      const int b = a.budget - c0 - 32 * i;
+      return b <= 0 ? 0u : ~(sm_more[i] | sm_equal[i]) & (b >= 32 ? ~0u : (1u << b) - 1);
+    };
+    auto taken = [&](int i) {
+      const int b = a.budget - c0 - 32 * i;
+      return b >= 32 ? 0u : (sm_more[i] | sm_equal[i]) & (b <= 0 ? ~0u : ~((1u << b) - 1));
+    };
+    uint32_t counts = 0;  // freed in the low, taken in the high half: at most kMaxSmemKeys < 2^16 of each
+    for (int i = w0; i < w1; ++i) counts += __popc(freed(i)) + (__popc(taken(i)) << 16);
+    const uint32_t before = cta_scan(counts, sm_scan, &total);
+    uint32_t to = moved_to + (before & 0xffff), src = moved_from + (before >> 16);
+    for (int i = w0; i < w1; ++i) {
+      for (uint32_t x = freed(i); x; x &= x - 1) mv[to++].x = c0 + 32 * i + __ffs(x) - 1;
+      for (uint32_t x = taken(i); x; x &= x - 1) mv[src++].y = c0 + 32 * i + __ffs(x) - 1;
+    }
+    moved_to += total & 0xffff;
+    moved_from += total >> 16;
+    __syncthreads();
   }
-  if (tid == 0) a.counts[unit] = moved;
-  __syncthreads();
+  const int moved = (int)moved_from;  // as many as were freed: budget slots are kept in all
+  if (LPR == 0 && tid == 0) a.counts[unit] = moved;
   for (int i = tid; i < moved; i += kSelThreads) {
     const int2 m = mv[i];
     a.weights_out[base + m.x] = w[m.y];
     a.slot_positions_out[base + m.x] = sp[m.y];
   }
-}
-
-// Up to kWarpMoves moves of a unit's list by one warp.  Each lane finds one row (the freed or the
-// kept slot of a move: one table entry), then all lanes copy 16-byte pieces, eight loads under
-// way at a time, with the rows' places taken from the lanes that know them.
-constexpr int kWarpMoves = 16;
-template <typename T, int HD>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves, int row, int head, int count) {
-  constexpr int LPR = HD * (int)sizeof(T) / 16;        // pieces of a K or V row
-  constexpr int STEPS = kWarpMoves * 2 * LPR / 32, FLY = STEPS < 8 ? STEPS : 8;
-  const int lane = threadIdx.x % 32, mine = lane % kWarpMoves;
-  int64_t at = -1;
-  if (mine < count) {
-    const int2 mv = moves[mine];
-    at = a.kv.at<HD>(row, lane < kWarpMoves ? mv.x : mv.y, head);
-    if (at < 0) raise_flag(a.err);
-  }
-  for (int s0 = 0; s0 < STEPS; s0 += FLY) {
-    int4 v[FLY];
-    int64_t to[FLY];
-#pragma unroll
-    for (int u = 0; u < FLY; ++u) {
-      const int flat = (s0 + u) * 32 + lane, m = flat / (2 * LPR), r = flat % (2 * LPR), piece = r % LPR;
-      const int64_t src = __shfl_sync(0xffffffffu, at, kWarpMoves + m);
-      to[u] = __shfl_sync(0xffffffffu, at, m);
-      T* p = static_cast<T*>(r < LPR ? a.kv.k : a.kv.v);
-      if (src < 0) to[u] = -1;
-      v[u] = ld_once_if(reinterpret_cast<const int4*>(p + src) + piece, to[u] >= 0);
-    }
-#pragma unroll
-    for (int u = 0; u < FLY; ++u) {
-      const int r = ((s0 + u) * 32 + lane) % (2 * LPR), piece = r % LPR;
-      T* p = static_cast<T*>(r < LPR ? a.kv.k : a.kv.v);
-      if (to[u] >= 0) reinterpret_cast<int4*>(p + to[u])[piece] = v[u];
-    }
+  if constexpr (LPR > 0) {
+    for (int m = warp * kWarpMoves; m < moved; m += kSelThreads / 32 * kWarpMoves)
+      move_rows<LPR>(a, mv + m, row, head, moved - m);
   }
 }
 
-template <typename T, int HD>
+template <int LPR>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictArgs a) {
   constexpr int WARPS = kMoveThreads / 32;
   const int unit = blockIdx.x, row = unit / a.kv.hkv, head = unit - row * a.kv.hkv;
@@ -226,7 +275,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictArgs a) {
   const int count = a.counts[unit];
   for (int64_t m = (int64_t)(blockIdx.y * WARPS + threadIdx.x / 32) * kWarpMoves; m < count;
        m += (int64_t)gridDim.y * WARPS * kWarpMoves)
-    move_rows<T, HD>(a, a.moves + (int64_t)unit * a.max_moves + m, row, head, count - (int)m);
+    move_rows<LPR>(a, a.moves + (int64_t)unit * a.max_moves + m, row, head, count - (int)m);
 }
 
 static int64_t evict_max_moves(const pim_paged_evict_args* a) {
@@ -256,18 +305,36 @@ static int64_t evict_counts_bytes(const pim_paged_evict_args* a) {
   return ((int64_t)a->kv.rows * a->kv.kv_heads * 4 + 255) / 256 * 256;
 }
 
-static cudaError_t evict(EvictArgs& a, int hd, int dtype, cudaStream_t st) {
+template <bool SMEM, int LPR>
+static cudaError_t launch_select(const EvictArgs& a, size_t smem, cudaStream_t st) {
   static ResidentCache cache;
-  a.smem_keys = (int)min((int64_t)kMaxSmemKeys, (int64_t)a.kv.max_pages << a.kv.ps_log2);
   cudaError_t e;
-  if (resident_ctas(evict_select_kernel, kSelThreads, (size_t)a.smem_keys * 4, cache, &e) < 0) return e;
-  e = launch_pdl(evict_select_kernel, dim3(a.kv.hkv, a.kv.rows), dim3(kSelThreads), (size_t)a.smem_keys * 4, st, a);
-  if (e != cudaSuccess || a.max_moves == 0) return e;
-  return dispatch_type_dim(dtype, hd, [&](auto t, auto d) {
-    const int by = ceil_div(a.max_moves, kWarpMoves * kMoveThreads / 32);
-    return launch_pdl(evict_move_kernel<decltype(t), decltype(d)::value>,
-                      dim3(a.kv.rows * a.kv.hkv, by < 65535 ? by : 65535), dim3(kMoveThreads), 0, st, a);
-  });
+  if (resident_ctas(evict_select_kernel<SMEM, LPR>, kSelThreads, smem, cache, &e) < 0) return e;
+  return launch_pdl(evict_select_kernel<SMEM, LPR>, dim3(a.kv.hkv, a.kv.rows), dim3(kSelThreads), smem, st, a);
+}
+
+template <int LPR>
+static cudaError_t evict_rows(const EvictArgs& a, cudaStream_t st) {
+  const int64_t slots = (int64_t)a.kv.max_pages << a.kv.ps_log2;
+  const bool smem = slots <= kMaxSmemKeys;
+  const size_t bytes = smem ? (size_t)slots * 4 : 0;
+  // Where a unit cannot have more moves than the selecting CTA's warps do in one go, that CTA does them: a launch less.
+  if (a.max_moves <= kFusedMoves)
+    return smem ? launch_select<true, LPR>(a, bytes, st) : launch_select<false, LPR>(a, bytes, st);
+  const cudaError_t e = smem ? launch_select<true, 0>(a, bytes, st) : launch_select<false, 0>(a, bytes, st);
+  if (e != cudaSuccess) return e;
+  const int by = ceil_div(a.max_moves, kWarpMoves * kMoveThreads / 32);
+  return launch_pdl(evict_move_kernel<LPR>, dim3(a.kv.rows * a.kv.hkv, by < 65535 ? by : 65535), dim3(kMoveThreads), 0,
+                    st, a);
+}
+
+static cudaError_t evict(const EvictArgs& a, int row_bytes, cudaStream_t st) {
+  switch (row_bytes) {
+    case 64: return evict_rows<4>(a, st);
+    case 128: return evict_rows<8>(a, st);
+    case 256: return evict_rows<16>(a, st);
+    default: return evict_rows<32>(a, st);
+  }
 }
 
 }  // namespace pim
@@ -306,5 +373,6 @@ extern "C" int pim_paged_evict(const pim_paged_evict_args* a, int32_t dtype, voi
   d.counts = static_cast<int*>(workspace);
   d.moves = reinterpret_cast<int2*>(static_cast<char*>(workspace) + evict_counts_bytes(a));
   d.max_moves = (int)evict_max_moves(a);
-  return report_cuda(evict(d, a->kv.head_dim, dtype, (cudaStream_t)stream), "pim_paged_evict");
+  d.page_pieces = a->kv.page_stride * elem_bytes(dtype) / 16;
+  return report_cuda(evict(d, a->kv.head_dim * elem_bytes(dtype), (cudaStream_t)stream), "pim_paged_evict");
 }
