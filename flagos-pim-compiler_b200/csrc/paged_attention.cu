@@ -61,6 +61,7 @@ struct PagedAttnArgs {
 };
 
 constexpr int kTile = 64;          // keys of a tile
+constexpr int kUnitCost = 2;       // what a unit costs beside its tiles, in tiles: see the head of the file
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 // CTAs of the first kernel per SM: what its registers allow without spilling.
@@ -74,19 +75,24 @@ __device__ __forceinline__ int row_length(const PagedAttnArgs& a, int row) {
 __device__ __forceinline__ int row_tiles(const PagedAttnArgs& a, int row) {
   return (row_length(a, row) + kTile - 1) / kTile;
 }
+// What a row's unit counts for when the work is dealt out; its tiles are the last of it.
+__device__ __forceinline__ int row_cost(const PagedAttnArgs& a, int row) {
+  const int n = row_tiles(a, row);
+  return n ? n + kUnitCost : 0;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Tiles of all rows (per unit of a row), and of those before `row`: sums over the CTA.
+// Cost of all rows (per unit of a row), and of those before `row`: sums over the CTA.
 template <int THREADS>
-__device__ __forceinline__ void count_tiles(const PagedAttnArgs& a, int row, int64_t* before, int64_t* total) {
+__device__ __forceinline__ void count_cost(const PagedAttnArgs& a, int row, int64_t* before, int64_t* total) {
   __shared__ int64_t sm[2][THREADS / 32];
   int64_t all = 0, pre = 0;
   for (int b = threadIdx.x; b < a.kv.rows; b += THREADS) {
-    const int n = row_tiles(a, b);
+    const int n = row_cost(a, b);
     all += n;
     if (b < row) pre += n;
   }
@@ -502,14 +508,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
   pdl_wait();
-  // where this CTA's range of tiles begins: thread i counts the tiles of rows [i per, (i + 1) per)
+  // where this CTA's range begins: thread i counts the cost of rows [i per, (i + 1) per)
   const int units = a.kv.hkv * a.head_tiles;
   const int per = (a.kv.rows + kPagedThreads - 1) / kPagedThreads;
   const int r0 = min(tid * per, a.kv.rows), r1 = min(r0 + per, a.kv.rows);
   int64_t mine = 0;
   for (int b = r0; b < r1; ++b) {
     if (blockIdx.x == 0 && row_length(a, b) != a.lengths[b]) raise_flag(a.err);
-    mine += row_tiles(a, b);
+    mine += row_cost(a, b);
   }
   int64_t scan = mine;
 #pragma unroll
@@ -526,14 +532,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
     total += sm_scan[w];
   }
   total *= units;
-  const int64_t ctas = min((int64_t)a.ctas, total);  // each of them has a tile at least
+  const int64_t ctas = min((int64_t)a.ctas, total);  // none of them has an empty range
   if (blockIdx.x >= ctas) return;
   const int64_t lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1) * total / ctas;
   if (lo >= before * units && lo < (before + mine) * units) {
     int64_t at = before * units;
     int b = r0;
     for (;; ++b) {
-      const int64_t n = (int64_t)row_tiles(a, b) * units;
+      const int64_t n = (int64_t)row_cost(a, b) * units;
       if (lo < at + n) break;
       at += n;
     }
@@ -542,11 +548,17 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
   }
   __syncthreads();
   int row = sm_row;
-  int tiles = row_tiles(a, row);
-  int unit = (int)(sm_rest / tiles), tile = (int)(sm_rest - (int64_t)unit * tiles);
+  int cost = row_cost(a, row);
+  int unit = (int)(sm_rest / cost);
+  int64_t at = sm_rest - (int64_t)unit * cost;  // within the unit
+  bool first = true;
   for (int64_t left = hi - lo; left > 0;) {
-    const int len = row_length(a, row);
-    const int n = (int)min((int64_t)(tiles - tile), left);
+    const int len = row_length(a, row), tiles = cost - kUnitCost;
+    // the part of [at, at + left) that is tiles of this unit
+    const int64_t stop = min(at + left, (int64_t)cost);
+    const int tile = (int)max(at - kUnitCost, (int64_t)0), n = (int)(stop - kUnitCost) - tile;
+    left -= stop - at;
+    if (n > 0) {
     const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
     const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
     {
@@ -559,7 +571,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
     __syncthreads();
     const bool whole = n == tiles;
     // a partial that begins with the CTA's range is its slot 0, one that begins later its slot 1
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (left == hi - lo ? 0 : 1);
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (first ? 0 : 1);
+    first = false;
     for (int i = tid; i < nh * HD; i += kPagedThreads) {
       const int h = i / HD, d = i % HD;
       float M = -INFINITY;
@@ -589,29 +602,30 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
       }
     }
     __syncthreads();
-    left -= n;
-    tile += n;
-    if (tile == tiles && left > 0) {
-      tile = 0;
+    }
+    at = stop;
+    if (at == cost && left > 0) {
+      at = 0;
       if (++unit == units) {
         unit = 0;
         do ++row;
-        while ((tiles = row_tiles(a, row)) == 0);  // (tiles are left, so a row with some is)
+        while ((cost = row_cost(a, row)) == 0);  // (some of the range is left, so a row with some is)
       }
     }
   }
 }
 
-// The CTAs that hold partials of tiles [start, start + n) of `total`: first .. last, and the
-// slot of the first one's.
+// The CTAs that hold a unit's tiles, the unit's cost being [start, start + kUnitCost + tiles) of `total`: first ..
+// last, and the slot of the first one's part.
 struct Holders {
   int first, last, first_slot;
 };
-__device__ __forceinline__ Holders holders(int64_t start, int64_t n, int64_t total, int64_t ctas) {
+__device__ __forceinline__ Holders holders(int64_t start, int tiles, int64_t total, int64_t ctas) {
   Holders h;
-  h.first = (int)(((start + 1) * ctas + total - 1) / total) - 1;  // the largest c with c total / ctas <= start
-  h.last = (int)(((start + n) * ctas + total - 1) / total) - 1;
-  h.first_slot = h.first * total / ctas == start ? 0 : 1;
+  const int64_t begin = start + kUnitCost, end = begin + tiles;
+  h.first = (int)(((begin + 1) * ctas + total - 1) / total) - 1;  // the largest c with c total / ctas <= begin
+  h.last = (int)((end * ctas + total - 1) / total) - 1;
+  h.first_slot = h.first * total / ctas >= start ? 0 : 1;
   return h;
 }
 
@@ -643,12 +657,12 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
     return;
   }
   int64_t before, total;
-  count_tiles<kFinishThreads>(a, row, &before, &total);
+  count_cost<kFinishThreads>(a, row, &before, &total);
   const int units = a.kv.hkv * a.head_tiles;
   total *= units;
   auto holders_of = [&](int h) {
     const int unit = h / a.group * a.head_tiles + h % a.group / NH;
-    return holders(before * units + (int64_t)unit * tiles, tiles, total, min((int64_t)a.ctas, total));
+    return holders(before * units + (int64_t)unit * (tiles + kUnitCost), tiles, total, min((int64_t)a.ctas, total));
   };
   auto slot_of = [&](const Holders& p, int c) {
     return ((int64_t)c * 2 + (c == p.first ? p.first_slot : 0)) * NH;
