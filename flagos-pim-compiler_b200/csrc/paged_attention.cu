@@ -52,19 +52,20 @@ struct PagedAttnArgs {
   int64_t w_row_stride, w_head_stride;
   int* err;
   int head_tiles;   // of a kv head's query group
+  int whole_warps;  // a CTA of so many warps per unit (paged_whole_kernel); 0: split
   int ctas;
+  int64_t* cost;    // [rows + 1] cost of the units of the rows before, and of all
   float* part_stat; // [ctas][2][NH][2]  max, sum
   float* part_acc;  // [ctas][2][NH][HD]
   float* row_stat;  // [rows][hq][2]     of units that one CTA finished (with weights)
   float* scores;    // [rows][hq][score_stride] (with weights)
-  int64_t score_stride;
+  int64_t score_stride; // slots of a row in `scores` (paged_whole_kernel: in shared memory)
 };
 
 constexpr int kTile = 64;          // keys of a tile
 constexpr int kUnitCost = 2;       // what a unit costs beside its tiles, in tiles: see the head of the file
-constexpr int kPagedWarps = 4;
-constexpr int kPagedThreads = kPagedWarps * 32;
-// CTAs of the first kernel per SM: what its registers allow without spilling.
+constexpr int kSplitWarps = 4;     // of a CTA that walks a range of tiles
+// CTAs of the splitting kernel per SM: what its registers allow without spilling.
 constexpr int paged_ctas_per_sm(bool bf16, int hd) { return bf16 && hd == 128 ? 2 : 3; }
 constexpr int kFinishThreads = 128;
 constexpr int kFinishKeys = 4 * kFinishThreads;  // keys whose weights one CTA adds to
@@ -84,30 +85,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Cost of all rows (per unit of a row), and of those before `row`: sums over the CTA.
-template <int THREADS>
-__device__ __forceinline__ void count_cost(const PagedAttnArgs& a, int row, int64_t* before, int64_t* total) {
-  __shared__ int64_t sm[2][THREADS / 32];
-  int64_t all = 0, pre = 0;
-  for (int b = threadIdx.x; b < a.kv.rows; b += THREADS) {
-    const int n = row_cost(a, b);
-    all += n;
-    if (b < row) pre += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    pre += __shfl_xor_sync(0xffffffffu, pre, o);
-  }
-  if (threadIdx.x % 32 == 0) sm[0][threadIdx.x / 32] = all, sm[1][threadIdx.x / 32] = pre;
-  __syncthreads();
-  all = pre = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) all += sm[0][w], pre += sm[1][w];
-  *total = all;
-  *before = pre;
 }
 
 // What one warp carries over a unit's keys: bf16 form (see the head of the file).
@@ -225,8 +202,9 @@ struct MmaCore {
   static __device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
   // The step's keys key0 .. key0 + 15; the caller loads the next step's K and V in between.
+  // `scores`: where the unit's first head has its scores, or nullptr.
   template <typename NextK>
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, int row, int head0, int nh, int key0, NextK&& next_k) {
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k) {
     float s[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -254,8 +232,8 @@ struct MmaCore {
           x = 2 * t + e < lim[i] ? x * a.scale_log2 : -INFINITY;
           top = fmaxf(top, x);
         }
-      if (a.scores && g + 8 * h < nh) {
-        float* sp = a.scores + ((int64_t)row * a.hq + head0 + g + 8 * h) * a.score_stride + key0 + 2 * t;
+      if (scores && g + 8 * h < nh) {
+        float* sp = scores + (g + 8 * h) * a.score_stride + key0 + 2 * t;
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(sp + 8 * i) = make_float2(s[i][2 * h], s[i][2 * h + 1]);
       }
@@ -342,10 +320,11 @@ struct FmaCore {
   static constexpr int REP = LPK / N;   // lanes that hold the same score
   static constexpr int kSub = KG * NK;
   static constexpr int kParts = KG;
-  float4 q[NH], acc[NH];
+  float4 q[NH], acc[NH], k[NK], v[NK];
   float m, l;
   int page[NK];
-  int grp, sl, head, key_of;  // this lane's score: head, and key within the group's NK
+  int64_t at[NK], at_next[NK];  // this lane's 16 bytes of each key; -1: no such key
+  int grp, sl, head, key_of;    // this lane's score: head, and key within the group's NK
 
   __device__ __forceinline__ void init(const PagedAttnArgs& a, int row, int head0, int nh) {
     const int lane = threadIdx.x % 32;
@@ -368,38 +347,51 @@ struct FmaCore {
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
       const int key = key0 + grp * NK + u;
-      const uint32_t id = ld4_if(trow + (key >> a.kv.ps_log2), key < end);
-      page[u] = key < end ? (int)id : -1;
+      page[u] = (int)ld4_if(trow + (key >> a.kv.ps_log2), key < end);
     }
   }
-  // One step over the keys whose pages were fetched; `end` bounds the keys.
-  template <typename Next>
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, int row, int kvh, int head0, int nh, int key0, int end,
-                                       Next&& next_pages) {
-    float4 k[NK], v[NK];
-    bool ok[NK];
+  __device__ __forceinline__ void place(const PagedAttnArgs& a, int kvh, int key0, int end) {
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
       const int key = key0 + grp * NK + u;
-      ok[u] = (unsigned)page[u] < (unsigned)a.kv.num_pages;
-      if (!ok[u] && key < end) raise_flag(a.err);
-      const int64_t at = page[u] * a.kv.page_stride +
-                         (((int64_t)kvh << a.kv.ps_log2) + (key & ((1 << a.kv.ps_log2) - 1))) * HD + 4 * sl;
-      const int4 x = ld_once_if(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.k) + at), ok[u]);
-      const int4 y = ld_once_if(reinterpret_cast<const int4*>(static_cast<const float*>(a.kv.v) + at), ok[u]);
-      k[u] = make_float4(__int_as_float(x.x), __int_as_float(x.y), __int_as_float(x.z), __int_as_float(x.w));
-      v[u] = make_float4(__int_as_float(y.x), __int_as_float(y.y), __int_as_float(y.z), __int_as_float(y.w));
+      at_next[u] = -1;
+      if (key < end) {
+        if ((unsigned)page[u] < (unsigned)a.kv.num_pages)
+          at_next[u] = page[u] * a.kv.page_stride +
+                       (((int64_t)kvh << a.kv.ps_log2) + (key & ((1 << a.kv.ps_log2) - 1))) * HD + 4 * sl;
+        else
+          raise_flag(a.err);
+      }
     }
+  }
+  static __device__ __forceinline__ float4 load(const void* pages, int64_t at) {
+    const int4 x = ld_once_if(reinterpret_cast<const int4*>(static_cast<const float*>(pages) + at), at >= 0);
+    return make_float4(__int_as_float(x.x), __int_as_float(x.y), __int_as_float(x.z), __int_as_float(x.w));
+  }
+  __device__ __forceinline__ void load_k(const PagedAttnArgs& a) {
+#pragma unroll
+    for (int u = 0; u < NK; ++u) k[u] = load(a.kv.k, at_next[u]);
+  }
+  __device__ __forceinline__ void load_v(const PagedAttnArgs& a) {
+#pragma unroll
+    for (int u = 0; u < NK; ++u) v[u] = load(a.kv.v, at[u]);
+  }
+  __device__ __forceinline__ void advance() {
+#pragma unroll
+    for (int u = 0; u < NK; ++u) at[u] = at_next[u];
+  }
+  template <typename NextK>
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k) {
     bool mine_ok = false;
 #pragma unroll
-    for (int u = 0; u < NK; ++u) mine_ok |= ok[u] && u == key_of;
-    next_pages();
+    for (int u = 0; u < NK; ++u) mine_ok |= at[u] >= 0 && u == key_of;
     float s[N];
 #pragma unroll
     for (int u = 0; u < NK; ++u)
 #pragma unroll
       for (int h = 0; h < NH; ++h)
         s[u * NH + h] = fmaf(q[h].x, k[u].x, fmaf(q[h].y, k[u].y, fmaf(q[h].z, k[u].z, q[h].w * k[u].w)));
+    next_k();
     int o = LPK / 2;
 #pragma unroll
     for (int n = N; n > 1; n /= 2, o /= 2) {
@@ -416,10 +408,8 @@ struct FmaCore {
 #pragma unroll
     for (int r = REP / 2; r > 0; r /= 2) x += __shfl_xor_sync(0xffffffffu, x, r);
     x = mine_ok ? x * a.scale_log2 : -INFINITY;
-    if (a.scores && sl % REP == 0 && head < nh) {
-      const int key = key0 + grp * NK + key_of;
-      if (key < end) a.scores[((int64_t)row * a.hq + head0 + head) * a.score_stride + key] = x;
-    }
+    // (a key behind the end writes -inf behind the row's scores, within score_stride)
+    if (scores && sl % REP == 0 && head < nh) scores[head * a.score_stride + key0 + grp * NK + key_of] = x;
     float top = x;
 #pragma unroll
     for (int r = REP * NH; r < LPK; r *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, r));
@@ -461,12 +451,13 @@ struct FmaCore {
   }
 };
 
-// One warp's keys of [begin, end) (begin a multiple of 64), the CTA's warps taking turns.
-template <int HD, int NH>
-__device__ __forceinline__ void walk(MmaCore<HD, NH>& core, const PagedAttnArgs& a, const int* trow, int row, int kvh,
-                                     int head0, int nh, int begin, int end, int warp) {
-  constexpr int S = MmaCore<HD, NH>::kSub, STRIDE = S * kPagedWarps;
-  int key0 = begin + warp * S;
+// One warp's keys of [begin, end) (begin a multiple of 64), the CTA's WARPS warps taking turns: page ids two steps
+// ahead, the next step's K loads once this one's scores are formed, its V loads after this one's products.
+template <int WARPS, typename Core>
+__device__ __forceinline__ void walk(Core& core, const PagedAttnArgs& a, const int* trow, float* scores, int kvh, int nh,
+                                     int begin, int end) {
+  constexpr int STRIDE = Core::kSub * WARPS;
+  int key0 = begin + (int)threadIdx.x / 32 * Core::kSub;
   if (key0 >= end) return;  // (the whole warp)
   core.fetch_pages(a, trow, key0, end);
   core.place(a, kvh, key0, end);
@@ -475,7 +466,7 @@ __device__ __forceinline__ void walk(MmaCore<HD, NH>& core, const PagedAttnArgs&
   core.load_v(a);
   core.fetch_pages(a, trow, key0 + STRIDE, end);
   for (; key0 < end; key0 += STRIDE) {
-    core.step(a, row, head0, nh, key0, [&] {
+    core.step(a, scores, nh, key0, [&] {
       core.place(a, kvh, key0 + STRIDE, end);
       core.fetch_pages(a, trow, key0 + 2 * STRIDE, end);
       core.load_k(a);
@@ -485,24 +476,85 @@ __device__ __forceinline__ void walk(MmaCore<HD, NH>& core, const PagedAttnArgs&
   }
 }
 
-template <int HD, int NH>
-__device__ __forceinline__ void walk(FmaCore<HD, NH>& core, const PagedAttnArgs& a, const int* trow, int row, int kvh,
-                                     int head0, int nh, int begin, int end, int warp) {
-  constexpr int S = FmaCore<HD, NH>::kSub, STRIDE = S * kPagedWarps;
-  int key0 = begin + warp * S;
-  if (key0 >= end) return;
-  core.fetch_pages(a, trow, key0, end);
-  for (; key0 < end; key0 += STRIDE)
-    core.step(a, row, kvh, head0, nh, key0, end, [&] { core.fetch_pages(a, trow, key0 + STRIDE, end); });
+// The parts of a unit that a CTA's warps hold, brought together.
+template <typename Core, int HD, int NH, int WARPS>
+struct Joint {
+  static constexpr int PARTS = WARPS * Core::kParts;
+  float m[PARTS * NH], l[PARTS * NH];
+  float top[NH], sum[NH];  // the unit's max (0 where there is none) and sum
+  float none[NH];          // 1 where no key had a score above -inf
+  alignas(16) float acc[PARTS * NH * HD];
+
+  // Keys [begin, end) of the unit by the whole CTA; out(h, d, value before the division) for its heads.
+  template <typename Out>
+  __device__ __forceinline__ void run(const PagedAttnArgs& a, int row, int kvh, int head0, int nh, int begin, int end,
+                                      float* scores, Out&& out) {
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    {
+      Core core;
+      core.init(a, row, head0, nh);
+      walk<WARPS>(core, a, a.kv.table + row * a.kv.table_stride, scores, kvh, nh, begin, end);
+      core.store(m, l, acc, warp);
+    }
+    __syncthreads();
+    for (int h = warp; h < nh; h += WARPS) {  // a lane per part
+      const float pm = lane < PARTS ? m[lane * NH + h] : -INFINITY;
+      const float M = warp_max(pm);
+      const float safe = M == -INFINITY ? 0.f : M;
+      const float f = exp2f(pm - safe);
+      const float L = warp_sum(lane < PARTS ? l[lane * NH + h] * f : 0.f);
+      if (lane < PARTS) m[lane * NH + h] = f;
+      if (lane == 0) top[h] = safe, sum[h] = L, none[h] = M == -INFINITY;
+    }
+    __syncthreads();
+    for (int i = tid; i < nh * HD; i += WARPS * 32) {
+      const int h = i / HD, d = i % HD;
+      float A = 0.f;
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) A += acc[(w * NH + h) * HD + d] * m[w * NH + h];
+      out(h, d, A);
+    }
+  }
+};
+
+// A CTA per unit: rows short enough for one to walk, with their scores in shared memory where the weights are asked
+// for.  One launch and no workspace.
+template <typename Core, int HD, int NH, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) paged_whole_kernel(PagedAttnArgs a) {
+  using T = typename Core::T;
+  extern __shared__ float sm_scores[];  // [NH][score_stride]
+  __shared__ Joint<Core, HD, NH, WARPS> joint;
+  const int tid = threadIdx.x;
+  pdl_trigger();
+  pdl_wait();
+  const int units = a.kv.hkv * a.head_tiles;
+  const int row = blockIdx.x / units, unit = blockIdx.x - row * units;
+  const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
+  const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
+  const int len = row_length(a, row);
+  if (tid == 0 && len != a.lengths[row]) raise_flag(a.err);
+  joint.run(a, row, kvh, head0, nh, 0, len, a.weights ? sm_scores : nullptr, [&](int h, int d, float A) {
+    const float L = joint.sum[h];
+    static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+  });
+  if (!a.weights) return;
+  float* w = a.weights + row * a.w_row_stride + (int64_t)kvh * a.w_head_stride;
+  for (int key = tid; key < len; key += WARPS * 32) {
+    float p = 0.f;
+    for (int h = 0; h < nh; ++h) {
+      const float L = joint.sum[h];
+      p += L > 0.f ? exp2f(sm_scores[h * a.score_stride + key] - joint.top[h]) * (1.f / L) : 0.f;
+    }
+    w[key] += p;
+  }
 }
 
 template <typename Core, int HD, int NH>
-__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, HD)) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kSplitWarps * 32, paged_ctas_per_sm(Core::kBf16, HD)) paged_attn_kernel(PagedAttnArgs a) {
   using T = typename Core::T;
-  constexpr int PARTS = kPagedWarps * Core::kParts;
-  __shared__ float sm_m[PARTS * NH], sm_l[PARTS * NH];
-  __shared__ __align__(16) float sm_acc[PARTS * NH * HD];
-  __shared__ int64_t sm_scan[kPagedWarps];
+  constexpr int THREADS = kSplitWarps * 32;
+  __shared__ Joint<Core, HD, NH, kSplitWarps> joint;
+  __shared__ int64_t sm_scan[kSplitWarps];
   __shared__ int sm_row;
   __shared__ int64_t sm_rest;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -510,7 +562,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
   pdl_wait();
   // where this CTA's range begins: thread i counts the cost of rows [i per, (i + 1) per)
   const int units = a.kv.hkv * a.head_tiles;
-  const int per = (a.kv.rows + kPagedThreads - 1) / kPagedThreads;
+  const int per = (a.kv.rows + THREADS - 1) / THREADS;
   const int r0 = min(tid * per, a.kv.rows), r1 = min(r0 + per, a.kv.rows);
   int64_t mine = 0;
   for (int b = r0; b < r1; ++b) {
@@ -527,9 +579,17 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
   __syncthreads();
   int64_t total = 0, before = scan - mine;
 #pragma unroll
-  for (int w = 0; w < kPagedWarps; ++w) {
+  for (int w = 0; w < kSplitWarps; ++w) {
     if (w < warp) before += sm_scan[w];
     total += sm_scan[w];
+  }
+  if (blockIdx.x == 0) {  // for the second kernel
+    int64_t at = before * units;
+    for (int b = r0; b < r1; ++b) {
+      a.cost[b] = at;
+      at += (int64_t)row_cost(a, b) * units;
+    }
+    if (tid == 0) a.cost[a.kv.rows] = total * units;
   }
   total *= units;
   const int64_t ctas = min((int64_t)a.ctas, total);  // none of them has an empty range
@@ -559,49 +619,29 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(Core::kBf16, 
     const int tile = (int)max(at - kUnitCost, (int64_t)0), n = (int)(stop - kUnitCost) - tile;
     left -= stop - at;
     if (n > 0) {
-    const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
-    const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
-    {
-      Core core;
-      core.init(a, row, head0, nh);
-      walk<HD, NH>(core, a, a.kv.table + row * a.kv.table_stride, row, kvh, head0, nh, tile * kTile,
-                   min(len, (tile + n) * kTile), warp);
-      core.store(sm_m, sm_l, sm_acc, warp);
-    }
-    __syncthreads();
-    const bool whole = n == tiles;
-    // a partial that begins with the CTA's range is its slot 0, one that begins later its slot 1
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (first ? 0 : 1);
-    first = false;
-    for (int i = tid; i < nh * HD; i += kPagedThreads) {
-      const int h = i / HD, d = i % HD;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < PARTS; ++w) M = fmaxf(M, sm_m[w * NH + h]);
-      const float safe = M == -INFINITY ? 0.f : M;
-      float L = 0.f, A = 0.f;
-#pragma unroll
-      for (int w = 0; w < PARTS; ++w) {
-        const float f = exp2f(sm_m[w * NH + h] - safe);
-        L += sm_l[w * NH + h] * f;
-        A += sm_acc[(w * NH + h) * HD + d] * f;
-      }
-      if (whole) {
-        static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
-        if (a.scores && d == 0) {
-          float* st = a.row_stat + ((int64_t)row * a.hq + head0 + h) * 2;
-          st[0] = safe;
-          st[1] = L;
-        }
-      } else {
-        a.part_acc[(slot * NH + h) * HD + d] = A;
-        if (d == 0) {
-          a.part_stat[(slot * NH + h) * 2] = M;
-          a.part_stat[(slot * NH + h) * 2 + 1] = L;
-        }
-      }
-    }
-    __syncthreads();
+      const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
+      const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
+      const bool whole = n == tiles;
+      // a partial that begins with the CTA's range is its slot 0, one that begins later its slot 1
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * NH;
+      first = false;
+      const int64_t head_at = (int64_t)row * a.hq + head0;
+      joint.run(a, row, kvh, head0, nh, tile * kTile, min(len, (tile + n) * kTile),
+                a.scores ? a.scores + head_at * a.score_stride : nullptr, [&](int h, int d, float A) {
+                  const float L = joint.sum[h];
+                  if (whole) {
+                    static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] =
+                        from_f<T>(L > 0.f ? A / L : 0.f);
+                  } else {
+                    a.part_acc[(slot + h) * HD + d] = A;
+                  }
+                  if (d == 0 && (!whole || a.scores)) {
+                    float* st = whole ? a.row_stat + (head_at + h) * 2 : a.part_stat + (slot + h) * 2;
+                    st[0] = !whole && joint.none[h] ? -INFINITY : joint.top[h];
+                    st[1] = L;
+                  }
+                });
+      __syncthreads();
     }
     at = stop;
     if (at == cost && left > 0) {
@@ -656,13 +696,10 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
       static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(0.f);
     return;
   }
-  int64_t before, total;
-  count_cost<kFinishThreads>(a, row, &before, &total);
-  const int units = a.kv.hkv * a.head_tiles;
-  total *= units;
+  const int64_t before = a.cost[row], total = a.cost[a.kv.rows];
   auto holders_of = [&](int h) {
     const int unit = h / a.group * a.head_tiles + h % a.group / NH;
-    return holders(before * units + (int64_t)unit * (tiles + kUnitCost), tiles, total, min((int64_t)a.ctas, total));
+    return holders(before + (int64_t)unit * (tiles + kUnitCost), tiles, total, min((int64_t)a.ctas, total));
   };
   auto slot_of = [&](const Holders& p, int c) {
     return ((int64_t)c * 2 + (c == p.first ? p.first_slot : 0)) * NH;
@@ -705,11 +742,22 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
     }
     return;
   }
-  // the probabilities of this CTA's keys, summed over the group's heads in order
-  const int len = row_length(a, row);
-  float sum[kFinishKeys / kFinishThreads];
+  // the probabilities of this CTA's keys, summed over the group's heads in order; the scores of the first heads and
+  // the weights are under way while the units' statistics are found
+  constexpr int KEYS = kFinishKeys / kFinishThreads, AHEAD = 4;
+  const int len = row_length(a, row), key0 = chunk * kFinishKeys + tid;
+  float* w = a.weights + row * a.w_row_stride + (int64_t)(head / a.group) * a.w_head_stride;
+  const float* sp = a.scores + ((int64_t)row * a.hq + head) * a.score_stride;
+  float sum[KEYS], old[KEYS], x[AHEAD][KEYS];
 #pragma unroll
-  for (int i = 0; i < kFinishKeys / kFinishThreads; ++i) sum[i] = 0.f;
+  for (int u = 0; u < KEYS; ++u) {
+    const int key = key0 + u * kFinishThreads;
+    sum[u] = 0.f;
+    old[u] = __uint_as_float(ld4_if(w + key, key < len));
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      x[i][u] = __uint_as_float(ld4_if(sp + i * a.score_stride + key, key < len && i < a.group));
+  }
   for (int h0 = 0; h0 < a.group; h0 += 32) {
     const int nh = min(32, a.group - h0);
     __syncthreads();
@@ -722,36 +770,40 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
         l = a.row_stat[((int64_t)row * a.hq + h) * 2 + 1];
       } else {
         const int hl = h % a.group % NH;
-        for (int c = p.first + lane; c <= p.last; c += 32) m = fmaxf(m, a.part_stat[(slot_of(p, c) + hl) * 2]);
-        m = warp_max(m);
-        if (m == -INFINITY) m = 0.f;
         for (int c = p.first + lane; c <= p.last; c += 32) {
-          const float* st = a.part_stat + (slot_of(p, c) + hl) * 2;
-          l += st[1] * exp2f(st[0] - m);
+          const float2 st = *reinterpret_cast<const float2*>(a.part_stat + (slot_of(p, c) + hl) * 2);
+          const float mn = fmaxf(m, st.x), safe = mn == -INFINITY ? 0.f : mn;
+          l = l * exp2f(m - safe) + st.y * exp2f(st.x - safe);
+          m = mn;
         }
-        l = warp_sum(l);
+        const float M = warp_max(m), safe = M == -INFINITY ? 0.f : M;
+        l = warp_sum(l * exp2f(m - safe));
+        m = safe;
       }
       if (lane == 0) sm_stat[i][0] = m, sm_stat[i][1] = l > 0.f ? 1.f / l : 0.f;
     }
     __syncthreads();
-    for (int i = 0; i < nh; ++i) {
-      const float m = sm_stat[i][0], inv = sm_stat[i][1];
-      const float* sp = a.scores + ((int64_t)row * a.hq + head + h0 + i) * a.score_stride;
+    for (int i0 = 0; i0 < nh; i0 += AHEAD) {
+      if (h0 + i0 > 0) {
 #pragma unroll
-      for (int u = 0; u < kFinishKeys / kFinishThreads; ++u) {
-        const int key = chunk * kFinishKeys + u * kFinishThreads + tid;
-        if (key < len) sum[u] += exp2f(sp[key] - m) * inv;
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+          for (int u = 0; u < KEYS; ++u)
+            x[i][u] = __uint_as_float(ld4_if(sp + (h0 + i0 + i) * a.score_stride + key0 + u * kFinishThreads,
+                                             key0 + u * kFinishThreads < len && i0 + i < nh));
       }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (i0 + i < nh) {
+#pragma unroll
+          for (int u = 0; u < KEYS; ++u) sum[u] += exp2f(x[i][u] - sm_stat[i0 + i][0]) * sm_stat[i0 + i][1];
+        }
     }
   }
-  float* w = a.weights + row * a.w_row_stride + (int64_t)(head / a.group) * a.w_head_stride;
 #pragma unroll
-  for (int u = 0; u < kFinishKeys / kFinishThreads; ++u) {
-    const int key = chunk * kFinishKeys + u * kFinishThreads + tid;
-    if (key < len) w[key] += sum[u];
-  }
+  for (int u = 0; u < KEYS; ++u)
+    if (key0 + u * kFinishThreads < len) w[key0 + u * kFinishThreads] = old[u] + sum[u];
 }
-
 
 // Query heads of a tile: the smallest tile that holds the group, up to 16 (bf16) or 8 (fp32) heads.
 static int head_tile(int dtype, int group) {
@@ -780,10 +832,27 @@ static int paged_ctas(int dtype, int hd) {
   return sms[dev] * per_sm;
 }
 
+template <typename Core, int HD, int NH, int WARPS>
+static cudaError_t launch_whole(const PagedAttnArgs& a, cudaStream_t st) {
+  static ResidentCache cache;
+  const size_t smem = a.weights ? (size_t)NH * a.score_stride * 4 : 0;
+  cudaError_t e;
+  if (resident_ctas(paged_whole_kernel<Core, HD, NH, WARPS>, WARPS * 32, smem, cache, &e) < 0) return e;
+  return launch_pdl(paged_whole_kernel<Core, HD, NH, WARPS>, dim3(a.kv.rows * a.kv.hkv * a.head_tiles),
+                    dim3(WARPS * 32), smem, st, a);
+}
+
 template <typename Core, int HD, int NH>
 static cudaError_t launch_paged(const PagedAttnArgs& a, cudaStream_t st) {
   using T = typename Core::T;
-  cudaError_t e = launch_pdl(paged_attn_kernel<Core, HD, NH>, dim3(a.ctas), dim3(kPagedThreads), 0, st, a);
+  if (a.whole_warps == 8) {
+    // (the parts of 16 heads by 8 warps would not fit the static shared memory: see paged_layout())
+    if constexpr (NH <= 8) return launch_whole<Core, HD, NH, 8>(a, st);
+    return cudaErrorNotSupported;
+  }
+  if (a.whole_warps == 4) return launch_whole<Core, HD, NH, 4>(a, st);
+  if (a.whole_warps == 2) return launch_whole<Core, HD, NH, 2>(a, st);
+  cudaError_t e = launch_pdl(paged_attn_kernel<Core, HD, NH>, dim3(a.ctas), dim3(kSplitWarps * 32), 0, st, a);
   if (e != cudaSuccess) return e;
   const int join = a.kv.rows * a.hq;
   const int chunks = a.weights ? ceil_div((int64_t)a.kv.max_pages << a.kv.ps_log2, kFinishKeys) : 0;
@@ -828,7 +897,9 @@ static const char* paged_attention_error(const pim_paged_attention_args* a, int 
 // The parts of the workspace, as byte offsets.
 struct PagedLayout {
   int nh, tiles, ctas;
-  int64_t score_stride, acc, row_stat, scores, bytes;
+  bool whole;
+  int whole_warps;
+  int64_t score_stride, stat, acc, row_stat, scores, bytes;
 };
 static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
   PagedLayout p;
@@ -836,15 +907,29 @@ static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
   p.nh = head_tile(dtype, group);
   p.tiles = ceil_div(group, p.nh);
   p.ctas = paged_ctas(dtype, a->kv.head_dim);
+  const int64_t slots = (int64_t)a->kv.max_pages * a->kv.page_size, units = (int64_t)a->kv.rows * a->kv.kv_heads * p.tiles;
+  // A CTA per unit saves the second launch and the join, and loses where rows are long: with few units 8 warps a CTA win
+  // up to 512 slots (1 row x 32 heads bf16: 4.4, 5.5, 7.3, 11.2 us at 128, 256, 512, 1024 slots against 8.3, 9.0, 9.6, 9.9
+  // split; 16 x 4 fp32: 3.4, 5.0, 7.8, 16.5 against 8.4, 8.8, 10.1, 12.5).  With more units than SMs fewer warps a CTA are
+  // better, bf16 2 up to 256 slots (128 rows x 8 heads x 8: 22.6, 35.6, 60.8 us at 128, 256, 512 against 38.6, 46.7,
+  // 61.7), fp32 4 up to 512 (64 x 8 x 4: 8.6, 16.6, 30.5, 56.7 at 128 .. 1024 against 17.3, 24.7, 34.7, 55.8).  A query
+  // group of several tiles would add to the same weights from several CTAs: it is split.
+  const bool many = units > 2 * 148;
+  p.whole_warps = many ? (dtype == PIM_BF16 ? 2 : 4) : p.nh > 8 ? 4 : 8;
+  p.whole = slots <= (many && dtype == PIM_BF16 ? 256 : 512) && (!a->weights || p.tiles == 1);
+  p.score_stride = (slots + 63) / 64 * 64;
+  if (p.whole) {
+    p.stat = p.acc = p.row_stat = p.scores = p.bytes = 0;
+    return p;
+  }
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   const int64_t parts = (int64_t)p.ctas * 2 * p.nh;
-  p.acc = up(parts * 2 * 4);
+  p.stat = up(((int64_t)a->kv.rows + 1) * 8);
+  p.acc = p.stat + up(parts * 2 * 4);
   p.row_stat = p.acc + up(parts * a->kv.head_dim * 4);
-  p.score_stride = 0;
   p.scores = p.bytes = p.row_stat;
   if (a->weights) {
     const int64_t heads = (int64_t)a->kv.rows * a->q_heads;
-    p.score_stride = ((int64_t)a->kv.max_pages * a->kv.page_size + 63) / 64 * 64;
     p.scores = p.row_stat + up(heads * 2 * 4);
     p.bytes = p.scores + heads * p.score_stride * 4;
   }
@@ -868,7 +953,7 @@ extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dt
     return report_status(PIM_EINVAL, msg);
   }
   const PagedLayout p = paged_layout(a, dtype);
-  if (!workspace || workspace_bytes < p.bytes || !aligned16(workspace))
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)))
     return report_status(PIM_EINVAL, "pim_paged_attention: workspace too small or not 16-byte aligned");
   PagedAttnArgs d{};
   d.kv = to_dev(a->kv);
@@ -887,13 +972,17 @@ extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dt
   d.err = a->err_flag;
   d.head_tiles = p.tiles;
   d.ctas = p.ctas;
-  char* ws = static_cast<char*>(workspace);
-  d.part_stat = reinterpret_cast<float*>(ws);
-  d.part_acc = reinterpret_cast<float*>(ws + p.acc);
-  if (a->weights) {
-    d.row_stat = reinterpret_cast<float*>(ws + p.row_stat);
-    d.scores = reinterpret_cast<float*>(ws + p.scores);
-    d.score_stride = p.score_stride;
+  d.whole_warps = p.whole ? p.whole_warps : 0;
+  d.score_stride = p.score_stride;
+  if (!p.whole) {
+    char* ws = static_cast<char*>(workspace);
+    d.cost = reinterpret_cast<int64_t*>(ws);
+    d.part_stat = reinterpret_cast<float*>(ws + p.stat);
+    d.part_acc = reinterpret_cast<float*>(ws + p.acc);
+    if (a->weights) {
+      d.row_stat = reinterpret_cast<float*>(ws + p.row_stat);
+      d.scores = reinterpret_cast<float*>(ws + p.scores);
+    }
   }
   const int hd = a->kv.head_dim;
   cudaStream_t st = (cudaStream_t)stream;
