@@ -28,15 +28,14 @@
 namespace pim {
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamVals = 16;  // logits of a thread
-constexpr int kBeamChunk = kBeamThreads * kBeamVals;
+constexpr int kBeamChunk = kBeamThreads * 16;  // tokens of the smallest chunk (a thread holds 16 or 32 logits)
 constexpr int kMaxBeams = 64;
 constexpr int kMaxSplits = 128;
 
 struct BeamStats {
-  float max;
+  float max;   // as a power of two: sum counts 2^max; -inf where there is no finite logit
   int count;   // entries of the chunk's list
-  double sum;  // of exp(x - max) over the chunk's finite logits
+  double sum;  // of exp(x) / 2^max over the chunk's finite logits
 };
 
 struct BeamSelectArgs {
@@ -64,6 +63,15 @@ __device__ __forceinline__ unsigned long long beam_key(uint32_t order, int token
 }
 __device__ __forceinline__ int key_token(unsigned long long key) { return (int)~(uint32_t)key; }
 
+// log2(e) in two parts, and 2^x.
+constexpr float kLog2eHi = 1.4426950408889634f;
+constexpr float kLog2eLo = (float)(1.4426950408889634 - (double)kLog2eHi);
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The largest of the lanes' 64-bit keys: two 32-bit warp reductions.
 __device__ __forceinline__ unsigned long long warp_best(unsigned long long key) {
   const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
@@ -72,11 +80,9 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long key) 
 }
 
 constexpr int kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamCand = kMaxBeams * kBeamVals;
-
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, int kBeamVals>
 __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectArgs a) {
-  constexpr int V = VecW<T>::n;
+  constexpr int V = VecW<T>::n, kBeamCand = kMaxBeams * kBeamVals;
   __shared__ unsigned long long sm_cand[kBeamCand];
   __shared__ uint32_t sm_top[kBeamWarps], sm_low[kBeamWarps];
   __shared__ double sm_s[kBeamWarps];
@@ -87,7 +93,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   pdl_wait();
   if (a.done && a.done[row]) return;  // offers one candidate, which the merge adds
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-  const int base = split * kBeamChunk;
+  const int base = split * (kBeamThreads * kBeamVals);
   uint32_t o[kBeamVals];
   // value i of this thread is token base + tok(i)
   auto tok = [&](int i) { return ALIGNED ? (i / V) * kBeamThreads * V + tid * V + i % V : i * kBeamThreads + tid; };
@@ -136,11 +142,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
         if (at < kBeamCand) sm_cand[at] = beam_key(o[i], base + tok(i));
       }
   }
-  // fp32 exponentials and a thread's 16 of them; the sum over threads in fp64
+  // exp(x - m) = 2^(x log2(e) - m2), m2 the rounded m log2(e), with log2(e) in two parts so that the argument carries one
+  // rounding; a thread's 16 or 32 of them in fp32, the sum over threads in fp64.
   const float m = top ? order_logit(top) : -INFINITY;
+  const float m2 = top ? m * kLog2eHi : 0.f;
   float part = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) part += o[i] ? expf(order_logit(o[i]) - m) : 0.f;
+  for (int i = 0; i < kBeamVals; ++i) {
+    const float x = order_logit(o[i]);
+    const float e = exp2_approx(fmaf(x, kLog2eLo, fmaf(x, kLog2eHi, -m2)));
+    part += o[i] ? e : 0.f;
+  }
   double s = part;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -182,7 +194,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   }
   if (tid == 0) {
     BeamStats st;
-    st.max = m;
+    st.max = top ? m2 : -INFINITY;
     st.count = min(n, a.k);
     st.sum = 0;
     for (int w = 0; w < kBeamWarps; ++w) st.sum += sm_s[w];
@@ -191,7 +203,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
 }
 
 constexpr int kMergeThreads = 512;
-constexpr int kListsPerLane = kMaxSplits / 32;
+constexpr int kDeep = 4;  // keys of a list at hand
 
 // Order-preserving bits of a finite double, never 0.
 __device__ __forceinline__ unsigned long long score_order(double s) {
@@ -199,6 +211,8 @@ __device__ __forceinline__ unsigned long long score_order(double s) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
+// Q: lists of a lane (splits <= 32 Q).
+template <int Q>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArgs a) {
   __shared__ unsigned long long sm_keys[kMaxBeams * kMaxBeams];  // [beams][k], sorted, 0: none
   __shared__ double sm_shift[kMaxBeams];                         // score_w - lse_w
@@ -216,55 +230,60 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
       if (lane == 0) sm_shift[w] = score, sm_done[w] = done;
       continue;
     }
-    // lane i merges lists i, i + 32, ..: the first two keys of each are at hand
-    unsigned long long head[kListsPerLane], next[kListsPerLane];
-    int taken[kListsPerLane], count[kListsPerLane];
-    float lm[kListsPerLane];
-    double ls[kListsPerLane];
+    // lane i merges lists i, i + 32, ..: the first kDeep keys of each are at hand
+    unsigned long long key[Q][kDeep];
+    int taken[Q], count[Q];
+    float lm[Q];
+    double ls[Q];
     const unsigned long long* lists = a.lists + (int64_t)row * a.splits * a.k;
     float m = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < kListsPerLane; ++q) {
+    for (int q = 0; q < Q; ++q) {
       const int l = lane + 32 * q;
-      head[q] = next[q] = 0;
       taken[q] = count[q] = 0;
       lm[q] = -INFINITY;
       ls[q] = 0;
       if (l < a.splits) {
         const BeamStats st = a.stats[(int64_t)row * a.splits + l];
-        const unsigned long long h = lists[(int64_t)l * a.k], n = a.k > 1 ? lists[(int64_t)l * a.k + 1] : 0;
         lm[q] = st.max;
         ls[q] = st.sum;
         count[q] = st.count;
-        head[q] = st.count > 0 ? h : 0;  // (entries behind the count are not written)
-        next[q] = st.count > 1 ? n : 0;
       }
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        const unsigned long long* p = lists + (int64_t)l * a.k + d;
+        const bool there = l < a.splits && d < a.k;  // (a key behind the list's count is not written: dropped below)
+        key[q][d] = ld4_if(p, there) | (unsigned long long)ld4_if(reinterpret_cast<const uint32_t*>(p) + 1, there) << 32;
+      }
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) key[q][d] = d < count[q] ? key[q][d] : 0;
       m = fmaxf(m, lm[q]);
     }
     m = warp_max(m);
     double s = 0;
 #pragma unroll
-    for (int q = 0; q < kListsPerLane; ++q)
-      if (lm[q] != -INFINITY) s += ls[q] * exp((double)lm[q] - (double)m);
+    for (int q = 0; q < Q; ++q)
+      if (lm[q] != -INFINITY) s += ls[q] * exp2((double)lm[q] - (double)m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
-      sm_shift[w] = m == -INFINITY ? 0.0 : (double)score - ((double)m + log(s));
+      sm_shift[w] = m == -INFINITY ? 0.0 : (double)score - ((double)m + log2(s)) * 0.69314718055994530942;
       sm_done[w] = 0;
     }
     for (int j = 0; j < a.k; ++j) {
-      unsigned long long mine = head[0];
+      unsigned long long mine = key[0][0];
 #pragma unroll
-      for (int q = 1; q < kListsPerLane; ++q) mine = head[q] > mine ? head[q] : mine;
+      for (int q = 1; q < Q; ++q) mine = key[q][0] > mine ? key[q][0] : mine;
       const unsigned long long best = warp_best(mine);
       if (lane == 0) keys[j] = best;
       if (best == 0) continue;  // (the warp agrees)
 #pragma unroll
-      for (int q = 0; q < kListsPerLane; ++q)
-        if (head[q] == best) {  // keys are unique: one list of one lane
-          head[q] = next[q];
-          ++taken[q];
-          next[q] = taken[q] + 1 < count[q] ? lists[(int64_t)(lane + 32 * q) * a.k + taken[q] + 1] : 0;
+      for (int q = 0; q < Q; ++q)
+        if (key[q][0] == best) {  // keys are unique: one list of one lane
+#pragma unroll
+          for (int d = 0; d + 1 < kDeep; ++d) key[q][d] = key[q][d + 1];
+          const int next = ++taken[q] + kDeep - 1;
+          key[q][kDeep - 1] = next < count[q] ? lists[(int64_t)(lane + 32 * q) * a.k + next] : 0;
         }
     }
   }
@@ -326,20 +345,22 @@ __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(BeamReord
   const int row = blockIdx.x, b = row / a.beams, j = row - b * a.beams, tid = threadIdx.x;
   pdl_trigger();
   pdl_wait();
+  // (the length and the parents come together; only the partly filled pages wait for them)
   const int n = a.lengths[b], ps = 1 << a.ps_log2;
+  const int p = tid < a.beams ? a.parents[b * a.beams + tid] : 0;
   const int full = n >> a.ps_log2, fill = n & (ps - 1);
-  if (tid == 0) sm_bad = n < 0 || n > (int64_t)a.max_pages << a.ps_log2, sm_take = 0;
+  bool mine_bad = n < 0 || n > (int64_t)a.max_pages << a.ps_log2 || p < 0 || p >= a.beams;
+  if (tid == 0) sm_bad = 0, sm_take = 0;
   __syncthreads();
   if (tid < a.beams) {
-    const int p = a.parents[b * a.beams + tid];
     sm_parent[tid] = p;
-    if (p < 0 || p >= a.beams) sm_bad = 1;
-    if (!sm_bad && fill) {  // (a length out of range was seen before the barrier: `full` is an entry of the table)
+    if (!mine_bad && fill) {
       const int page = a.table[(int64_t)(b * a.beams + tid) * a.table_stride + full];
       sm_page[tid] = page;
-      if (page < 0 || page >= a.num_pages) sm_bad = 1;
+      mine_bad = page < 0 || page >= a.num_pages;
     }
   }
+  if (mine_bad) sm_bad = 1;
   __syncthreads();
   const bool bad = sm_bad;
   if (bad && tid == 0 && blockIdx.y == 0) raise_flag(a.err);
@@ -411,23 +432,30 @@ static const char* beam_select_error(const pim_beam_select_args* a, int dtype) {
   return nullptr;
 }
 
-static int beam_splits(int vocab) { return ceil_div(vocab, kBeamChunk); }
+// Logits of a thread: 32 where that leaves two chunks for every SM, which halves the lists and the work beside the
+// logits (8 x 16 beams of 131072 fp32 logits with the reordering: 64.2 us against 69.4; 32 x 8 of 32000 bf16: 85.5 against
+// 86.5); else 16, for more CTAs.
+static int beam_vals(const pim_beam_select_args* a) {
+  return (int64_t)a->batch * a->beams * ceil_div(a->vocab, 2 * kBeamChunk) >= 2 * 148 ? 32 : 16;
+}
+static int beam_splits(const pim_beam_select_args* a) { return ceil_div(a->vocab, kBeamThreads * beam_vals(a)); }
 
 static int64_t beam_stats_bytes(const pim_beam_select_args* a) {
-  return (int64_t)a->batch * a->beams * beam_splits(a->vocab) * (int64_t)sizeof(BeamStats);
+  return (int64_t)a->batch * a->beams * beam_splits(a) * (int64_t)sizeof(BeamStats);
 }
 
-template <typename T>
+template <typename T, int VALS>
 static cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t st) {
   // 16-byte loads where rows allow them; a vocabulary that leaves most warps of such a chunk empty is read by
   // element, which spreads it over all of them
   const bool aligned = aligned16(a.logits) && a.stride * sizeof(T) % 16 == 0 && a.vocab % VecW<T>::n == 0 &&
                        a.vocab >= kBeamThreads * VecW<T>::n;
   const dim3 grid(a.splits, a.batch * a.beams);
-  cudaError_t e = aligned ? launch_pdl(beam_partial_kernel<T, true>, grid, dim3(kBeamThreads), 0, st, a)
-                          : launch_pdl(beam_partial_kernel<T, false>, grid, dim3(kBeamThreads), 0, st, a);
+  const cudaError_t e = aligned ? launch_pdl(beam_partial_kernel<T, true, VALS>, grid, dim3(kBeamThreads), 0, st, a)
+                                : launch_pdl(beam_partial_kernel<T, false, VALS>, grid, dim3(kBeamThreads), 0, st, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(beam_merge_kernel, dim3(a.batch), dim3(kMergeThreads), 0, st, a);
+  return a.splits <= 32 ? launch_pdl(beam_merge_kernel<1>, dim3(a.batch), dim3(kMergeThreads), 0, st, a)
+                        : launch_pdl(beam_merge_kernel<kMaxSplits / 32>, dim3(a.batch), dim3(kMergeThreads), 0, st, a);
 }
 
 }  // namespace pim
@@ -435,7 +463,7 @@ static cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t st) {
 extern "C" int64_t pim_beam_select_workspace_bytes(const pim_beam_select_args* a, int32_t dtype) {
   using namespace pim;
   if (beam_select_error(a, dtype)) return -1;
-  return beam_stats_bytes(a) + (int64_t)a->batch * a->beams * beam_splits(a->vocab) * a->beams_out * 8;
+  return beam_stats_bytes(a) + (int64_t)a->batch * a->beams * beam_splits(a) * a->beams_out * 8;
 }
 
 extern "C" int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
@@ -463,11 +491,14 @@ extern "C" int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, voi
   d.vocab = a->vocab;
   d.eos = a->eos;
   d.pad = a->pad;
-  d.splits = beam_splits(a->vocab);
+  d.splits = beam_splits(a);
   d.stats = static_cast<BeamStats*>(workspace);
   d.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + beam_stats_bytes(a));
-  return report_cuda(dtype == PIM_BF16 ? beam_select<__nv_bfloat16>(d, (cudaStream_t)stream)
-                                       : beam_select<float>(d, (cudaStream_t)stream),
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool wide = beam_vals(a) == 32;
+  return report_cuda(dtype == PIM_BF16 ? wide ? beam_select<__nv_bfloat16, 32>(d, st) : beam_select<__nv_bfloat16, 16>(d, st)
+                     : wide            ? beam_select<float, 32>(d, st)
+                                       : beam_select<float, 16>(d, st),
                      "pim_beam_select");
 }
 
@@ -511,6 +542,7 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   d.hkv = a->kv_heads;
   d.row_bytes = a->head_dim * es;
   d.err = a->err_flag;
+  if (page * es / 16 > (1 << 30)) return bad("a page of more than 16 GiB");
   // About a third of the rows copy: enough CTAs per row that those fill the GPU, and no more than there are steps.
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
   const int rows = a->batch * a->beams;
