@@ -21,6 +21,7 @@
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
 // copies read pages of beams with children and write pages of beams without.
 
+#include <float.h>
 #include <math.h>
 
 #include "paged.cuh"
@@ -66,6 +67,7 @@ __device__ __forceinline__ int key_token(unsigned long long key) { return (int)~
 // log2(e) in two parts, and 2^x.
 constexpr float kLog2eHi = 1.4426950408889634f;
 constexpr float kLog2eLo = (float)(1.4426950408889634 - (double)kLog2eHi);
+static_assert(kLog2eLo > 0, "-inf x kLog2eLo must stay -inf");
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -92,33 +94,39 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   pdl_trigger();
   pdl_wait();
   if (a.done && a.done[row]) return;  // offers one candidate, which the merge adds
-  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  const T* row_x = static_cast<const T*>(a.logits) + row * a.stride;
   const int base = split * (kBeamThreads * kBeamVals);
-  uint32_t o[kBeamVals];
+  float x[kBeamVals];  // -inf: no candidate
   // value i of this thread is token base + tok(i)
   auto tok = [&](int i) { return ALIGNED ? (i / V) * kBeamThreads * V + tid * V + i % V : i * kBeamThreads + tid; };
   if (ALIGNED) {
     int4 raw[kBeamVals / V];
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i)
-      raw[i] = ld_once_if(reinterpret_cast<const int4*>(x + base + tok(i * V)), base + tok(i * V) < a.vocab);
+      raw[i] = ld_once_if(reinterpret_cast<const int4*>(row_x + base + tok(i * V)), base + tok(i * V) < a.vocab);
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i) {
       float f[V];
       unpack(raw[i], f, T());
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[i * V + e] = base + tok(i * V) < a.vocab ? logit_order(f[e]) : 0;
+      for (int e = 0; e < V; ++e) x[i * V + e] = f[e];
     }
   } else {
-    float f[kBeamVals];
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) f[i] = base + tok(i) < a.vocab ? to_f(x[base + tok(i)]) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) o[i] = logit_order(f[i]);
+    for (int i = 0; i < kBeamVals; ++i) x[i] = base + tok(i) < a.vocab ? to_f(row_x[base + tok(i)]) : -INFINITY;
   }
-  uint32_t mine = 0;
+  if (ALIGNED && base + kBeamThreads * kBeamVals > a.vocab) {  // the last chunk
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) mine = max(mine, o[i]);
+    for (int i = 0; i < kBeamVals; ++i)
+      if (base + tok(i) >= a.vocab) x[i] = -INFINITY;
+  }
+  float mine_x = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kBeamVals; ++i) {
+    x[i] = fabsf(x[i]) < INFINITY ? x[i] : -INFINITY;
+    mine_x = fmaxf(mine_x, x[i]);
+  }
+  const uint32_t mine = logit_order(mine_x);
   const int rounds = (a.k + kBeamWarps - 1) / kBeamWarps;
   uint32_t cur = mine, low = 0;
   for (int r = 0; r < rounds; ++r) {
@@ -135,11 +143,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   for (int w = 1; w < kBeamWarps; ++w) top = max(top, sm_top[w]), tau = min(tau, sm_low[w]);
   tau = max(tau, 1u);  // (0: not a candidate)
   if (mine >= tau) {
+    const float least = order_logit(tau == 1 ? logit_order(-FLT_MAX) : tau);
 #pragma unroll
     for (int i = 0; i < kBeamVals; ++i)
-      if (o[i] >= tau) {
+      if (x[i] >= least) {
         const int at = atomicAdd(&sm_n, 1);
-        if (at < kBeamCand) sm_cand[at] = beam_key(o[i], base + tok(i));
+        if (at < kBeamCand) sm_cand[at] = beam_key(logit_order(x[i]), base + tok(i));
       }
   }
   // exp(x - m) = 2^(x log2(e) - m2), m2 the rounded m log2(e), with log2(e) in two parts so that the argument carries one
@@ -148,11 +157,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   const float m2 = top ? m * kLog2eHi : 0.f;
   float part = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) {
-    const float x = order_logit(o[i]);
-    const float e = exp2_approx(fmaf(x, kLog2eLo, fmaf(x, kLog2eHi, -m2)));
-    part += o[i] ? e : 0.f;
-  }
+  for (int i = 0; i < kBeamVals; ++i)  // (-inf gives 0: kLog2eLo is positive)
+    part += exp2_approx(fmaf(x[i], kLog2eLo, fmaf(x[i], kLog2eHi, -m2)));
   double s = part;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
     unsigned long long best = 0;
 #pragma unroll
     for (int i = 0; i < kBeamVals; ++i) {
-      const unsigned long long k = o[i] ? beam_key(o[i], base + tok(i)) : 0;
+      const unsigned long long k = x[i] != -INFINITY ? beam_key(logit_order(x[i]), base + tok(i)) : 0;
       best = k > best ? k : best;
     }
     __syncthreads();
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
     if (best >= bound) {
 #pragma unroll
       for (int i = 0; i < kBeamVals; ++i) {
-        const unsigned long long k = o[i] ? beam_key(o[i], base + tok(i)) : 0;
+        const unsigned long long k = x[i] != -INFINITY ? beam_key(logit_order(x[i]), base + tok(i)) : 0;
         if (k >= bound) sm_cand[atomicAdd(&sm_n, 1)] = k;  // at most k threads come here, with 16 keys each
       }
     }
