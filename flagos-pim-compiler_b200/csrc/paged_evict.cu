@@ -37,7 +37,8 @@ constexpr int kSelThreads = 512;
 constexpr int kMaxSmemKeys = 48 * 1024;
 constexpr int kChunkWords = kMaxSmemKeys / 32;
 constexpr int kMoveThreads = 256;
-constexpr int kFusedMoves = 256;  // see evict()
+constexpr int kFusedMoves = 256;  // see evict_rows()
+constexpr int kFewEvicted = 8;
 
 // Unsigned key of the same order as the weight; NaN lowest.  -0 and +0 are equal.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -108,6 +109,21 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves,
   }
 }
 
+// The state of the slots that are refilled and, with LPR, their K and V, by the selecting CTA.
+template <int LPR>
+__device__ __forceinline__ void finish_moves(const EvictArgs& a, const int2* mv, int moved, int row, int head,
+                                             int64_t base, const float* w, const int* sp) {
+  for (int i = threadIdx.x; i < moved; i += kSelThreads) {
+    const int2 m = mv[i];
+    a.weights_out[base + m.x] = w[m.y];
+    a.slot_positions_out[base + m.x] = sp[m.y];
+  }
+  if constexpr (LPR > 0) {
+    for (int m = threadIdx.x / 32 * kWarpMoves; m < moved; m += kSelThreads / 32 * kWarpMoves)
+      move_rows<LPR>(a, mv + m, row, head, moved - m);
+  }
+}
+
 // SMEM: the keys of a row fit the shared memory.  LPR: 0, or the CTA moves its rows itself.
 template <bool SMEM, int LPR>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
@@ -136,7 +152,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   // (int64: a position near the type's ends less `recent` must not wrap)
   const int64_t from = next - a.recent;
   auto make_key = [&](float wt, int p) { return p >= from || p < a.sink ? 0xffffffffu : order_key(wt); };
-  const bool evicts = n > a.budget;
+  const bool evicts = n > a.budget, few = SMEM && LPR > 0 && n - a.budget <= kFewEvicted;
   __syncthreads();
   // one pass over the state, kLoads slots of a thread in flight: the kept part's copy, the keys and the first
   // histogram
@@ -159,12 +175,56 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
       if (i < n && evicts) {
         const uint32_t k = make_key(wt[u], p[u]);
         if (SMEM) keys[i] = k;
-        atomicAdd(&hist[k >> 21], 1);
+        if (!few) atomicAdd(&hist[k >> 21], 1);
       }
     }
   }
   if (!evicts) {
     if (LPR == 0 && tid == 0) a.counts[unit] = 0;
+    return;
+  }
+  if (few) {
+    // A step's one or few tokens over the budget: that many rounds of a minimum, in place of the histograms and scans.
+    // Of equal keys the higher slot goes.
+    __shared__ uint2 sm_least[kSelThreads / 32];
+    __shared__ int sm_gone[kFewEvicted];
+    const int gone = n - a.budget;
+    unsigned long long last = 0;  // (every packed key is above it: a slot's complement is not 0)
+    __syncthreads();
+    for (int r = 0; r < gone; ++r) {
+      unsigned long long best = ~0ull;
+      for (int j = tid; j < n; j += kSelThreads) {
+        const unsigned long long x = (unsigned long long)keys[j] << 32 | (uint32_t)~j;
+        if (x > last && x < best) best = x;
+      }
+      uint32_t hi = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32));
+      uint32_t lo = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : ~0u);
+      if (lane == 0) sm_least[warp] = make_uint2(lo, hi);
+      __syncthreads();
+      const uint2 x = lane < kSelThreads / 32 ? sm_least[lane] : make_uint2(~0u, ~0u);
+      hi = __reduce_min_sync(0xffffffffu, x.y);
+      lo = __reduce_min_sync(0xffffffffu, x.y == hi ? x.x : ~0u);
+      last = (unsigned long long)hi << 32 | lo;
+      if (tid == 0) sm_gone[r] = (int)~lo;
+      __syncthreads();
+    }
+    // the freed slots below the budget in order, and the kept ones above it
+    int2* mv = a.moves + (int64_t)unit * a.max_moves;
+    if (warp == 0) {
+      const int mine = lane < gone ? sm_gone[lane] : n;
+      int rank = 0;
+      bool stays = lane < gone;  // slot budget + lane
+      for (int i = 0; i < gone; ++i) {
+        rank += sm_gone[i] < mine;
+        if (sm_gone[i] == a.budget + lane) stays = false;
+      }
+      if (lane < gone && mine < a.budget) mv[rank].x = mine;
+      const unsigned who = __ballot_sync(0xffffffffu, stays);
+      if (stays) mv[__popc(who & ((1u << lane) - 1))].y = a.budget + lane;
+      if (lane == 0) sm_count = __popc(who);
+    }
+    __syncthreads();
+    finish_moves<LPR>(a, mv, (int)sm_count, row, head, base, w, sp);
     return;
   }
   auto key = [&](int j) { return SMEM ? keys[j] : make_key(w[j], sp[j]); };
@@ -255,15 +315,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   }
   const int moved = (int)moved_from;  // as many as were freed: budget slots are kept in all
   if (LPR == 0 && tid == 0) a.counts[unit] = moved;
-  for (int i = tid; i < moved; i += kSelThreads) {
-    const int2 m = mv[i];
-    a.weights_out[base + m.x] = w[m.y];
-    a.slot_positions_out[base + m.x] = sp[m.y];
-  }
-  if constexpr (LPR > 0) {
-    for (int m = warp * kWarpMoves; m < moved; m += kSelThreads / 32 * kWarpMoves)
-      move_rows<LPR>(a, mv + m, row, head, moved - m);
-  }
+  finish_moves<LPR>(a, mv, moved, row, head, base, w, sp);
 }
 
 template <int LPR>

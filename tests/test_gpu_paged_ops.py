@@ -417,6 +417,17 @@ def test_evict(lengths, heads, ps, budget, recent, sink, dt, hd, in_place):
     _evict_case(lengths, heads, ps, hd, dt, budget, recent, sink, in_place=in_place)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("over", [1, 2, 3, 8, 9, 30])
+def test_evict_a_few_tokens_over_the_budget(over, in_place):
+    """The steps of a bounded cache: rows one or a few tokens over, with ties and protected tokens among the lightest."""
+    for budget in (1, 16, 40, 200):
+        lengths = [budget + over, budget, budget + 1, max(budget - 3, 0)]
+        _evict_case(lengths, 2, 8, 64, "bfloat16", budget, min(3, budget - 1), min(1, budget - 1), seed=over, ties=True,
+                    in_place=in_place)
+        _evict_case(lengths, 1, 8, 32, "float32", budget, 0, 0, seed=over + 1)
+
+
 @pytest.mark.parametrize("budget", [1, 13, 64, 255])
 def test_evict_ties_go_to_the_lower_slot(budget):
     _evict_case([256, 199], 2, 16, 32, "bfloat16", budget, 0, 0, seed=4, ties=True)
