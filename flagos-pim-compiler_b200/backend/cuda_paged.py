@@ -52,14 +52,21 @@ def _dt(t) -> str:
     return str(t.dtype).removeprefix("torch.")
 
 
+def _span(t) -> tuple[int, int]:
+    """First byte of a tensor's memory and the one behind its last."""
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.numel() * t.element_size()
+    return at, at + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else at
+
+
+def _meet(a, b) -> bool:
+    return a[0] < b[1] and b[0] < a[1]
+
+
 def _overlap(a, b) -> bool:
     """Whether two tensors' memory ranges meet."""
-    def span(t):
-        last = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    return _meet(_span(a), _span(b))
 
 
 def _rows_apart(a, b) -> bool:
@@ -80,10 +87,11 @@ def _rows_apart(a, b) -> bool:
 
 def _apart(outputs: dict, others: dict) -> None:
     """No output shares memory with another output or with an input."""
-    outs = [(n, t) for n, t in outputs.items() if t is not None]
-    for i, (n, t) in enumerate(outs):
-        for m, u in outs[i + 1:] + [(m, u) for m, u in others.items() if u is not None]:
-            if _overlap(t, u):
+    outs = [(n, _span(t)) for n, t in outputs.items() if t is not None]
+    ins = [(n, _span(t)) for n, t in others.items() if t is not None]
+    for i, (n, span) in enumerate(outs):
+        for m, other in outs[i + 1:] + ins:
+            if _meet(span, other):
                 raise ValueError(f"{n} shares memory with {m}")
 
 
@@ -128,6 +136,12 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
+def _raw_stream(torch, index: int) -> int:
+    """The device's current stream as the C ABI takes it (torch.cuda.current_stream builds an object: 2 us a call)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+
+
 class _Op:
     """One bound entry point: argument struct, workspace, error flag."""
 
@@ -159,19 +173,19 @@ class _Op:
             self._ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
             extra = (self._ws.data_ptr(), self._ws.numel())
         self._extra = extra
-        self._home = torch.cuda.current_stream(dev).cuda_stream
-        self._seen = {self._home}
+        self._index = dev.index
+        self._seen = {_raw_stream(torch, dev.index)}
 
     def _run(self) -> None:
-        torch = self._torch
-        stream = torch.cuda.current_stream(self._dev)
-        st = stream.cuda_stream
+        torch, index = self._torch, self._index
+        st = _raw_stream(torch, index)
         if st not in self._seen and not torch.cuda.is_current_stream_capturing():
             self._seen.add(st)  # its memory is given back only after this stream's work, too
+            stream = torch.cuda.current_stream(self._dev)
             for t in (*self._keep, self._ws, self._err):
                 if t is not None:
                     t.record_stream(stream)
-        if torch.cuda.current_device() == self._dev.index:
+        if torch.cuda.current_device() == index:
             rc = self._fn(self._ref, self._code, *self._extra, st)
         else:
             with torch.cuda.device(self._dev):
@@ -246,8 +260,8 @@ class PagedAppend(_Op):
             a.state_row_stride, a.state_head_stride = _state_strides(weights)
         _apart(dict(lengths_out=lengths_out, positions_out=positions_out),
                dict(lengths=lengths, positions=positions, starts=starts, table=table))
-        _apart(dict(k_pages=k_pages), dict(k=k, v=v, q=q, q_out=q_out))
-        _apart(dict(v_pages=v_pages), dict(k=k, v=v, q=q, q_out=q_out))
+        for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _apart({name: pages}, dict(k=k, v=v, q=q, q_out=q_out))
         if q is not None:
             for name, t in (("q", q), ("k", k), ("v", v)):
                 if not (t is q and q_out.data_ptr() == q.data_ptr()) and not _rows_apart(q_out, t):
