@@ -2,12 +2,14 @@
 //
 // Per (row, kv head), over the n slots in use: a token that must stay (recent or sink) ranks
 // above every weight; the budget largest stay, of equal ones the lower slot.  The selection
-// is a radix select: weights map to unsigned keys of the same order, three passes over
-// 11 + 11 + 10 bits find the key of the budget-th largest and how many equal to it stay.
-// The kept slots as bit words, scanned in slot order, then list the freed slots below the
-// budget and the kept ones above it; there are equally many, and moving the i-th kept one into
-// the i-th freed slot moves the fewest rows that any compaction can.  Sources lie at or above
-// the budget and destinations below it, so the moves need no order.
+// is a radix select over 64-bit keys, the weight's bits in unsigned order above the complement
+// of the slot: they are unique, so equal weights need no case of their own, and the bound of
+// what stays is one key.  Passes of 11 + 11 + 10 bits (of the slot's too, where weights are
+// equal) narrow it down until at most 256 keys share the bits fixed so far; those are ranked
+// by counting.  The kept slots as bit words, scanned in slot order, then list the freed slots
+// below the budget and the kept ones above it; there are equally many, and moving the i-th kept
+// one into the i-th freed slot moves the fewest rows that any compaction can.  Sources lie at or
+// above the budget and destinations below it, so the moves need no order.
 //
 // evict_select_kernel: one CTA per (row, head), keys in shared memory where they fit; it
 // reads 8 bytes a slot and writes the state and the list of moves.  evict_move_kernel: moves
@@ -39,6 +41,7 @@ constexpr int kChunkWords = kMaxSmemKeys / 32;
 constexpr int kMoveThreads = 256;
 constexpr int kFusedMoves = 256;  // see evict_rows()
 constexpr int kFewEvicted = 8;
+constexpr int kRankMost = 256;
 
 // Unsigned key of the same order as the weight; NaN lowest.  -0 and +0 are equal.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -113,10 +116,27 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves,
 template <int LPR>
 __device__ __forceinline__ void finish_moves(const EvictArgs& a, const int2* mv, int moved, int row, int head,
                                              int64_t base, const float* w, const int* sp) {
-  for (int i = threadIdx.x; i < moved; i += kSelThreads) {
-    const int2 m = mv[i];
-    a.weights_out[base + m.x] = w[m.y];
-    a.slot_positions_out[base + m.x] = sp[m.y];
+  constexpr int FLY = 4;
+  for (int i0 = threadIdx.x; i0 < moved; i0 += FLY * kSelThreads) {
+    int2 m[FLY];
+    uint32_t x[FLY], p[FLY];
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      const int i = i0 + u * kSelThreads;
+      m[u].x = (int)ld4_if(&mv[i].x, i < moved);
+      m[u].y = (int)ld4_if(&mv[i].y, i < moved);
+    }
+#pragma unroll
+    for (int u = 0; u < FLY; ++u) {
+      x[u] = ld4_if(w + m[u].y, i0 + u * kSelThreads < moved);
+      p[u] = ld4_if(sp + m[u].y, i0 + u * kSelThreads < moved);
+    }
+#pragma unroll
+    for (int u = 0; u < FLY; ++u)
+      if (i0 + u * kSelThreads < moved) {
+        a.weights_out[base + m[u].x] = __uint_as_float(x[u]);
+        a.slot_positions_out[base + m[u].x] = (int)p[u];
+      }
   }
   if constexpr (LPR > 0) {
     for (int m = threadIdx.x / 32 * kWarpMoves; m < moved; m += kSelThreads / 32 * kWarpMoves)
@@ -129,7 +149,9 @@ template <bool SMEM, int LPR>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t keys[];
   __shared__ uint32_t hist[2048];
-  __shared__ uint32_t sm_more[kChunkWords], sm_equal[kChunkWords];
+  __shared__ uint32_t sm_keep[kChunkWords], sm_at[kChunkWords];
+  __shared__ unsigned long long sm_near[kRankMost];
+  __shared__ unsigned long long sm_bound;
   __shared__ uint32_t sm_scan[kSelThreads / 32];
   __shared__ uint32_t sm_bin, sm_above, sm_count;
   const int head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -228,19 +250,18 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
     return;
   }
   auto key = [&](int j) { return SMEM ? keys[j] : make_key(w[j], sp[j]); };
-  // the budget-th largest key
-  uint32_t prefix = 0, need = a.budget;
-  int shift = 32;
-#pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bits = pass < 2 ? 11 : 10, bins = 1 << bits;
+  auto packed = [&](int j) { return (unsigned long long)key(j) << 32 | (uint32_t)~j; };
+  // the budget-th largest packed key
+  unsigned long long bound = 0;
+  uint32_t need = a.budget;
+  int shift = 64;
+  for (int pass = 0;; ++pass) {
+    const int bits = pass % 3 < 2 ? 11 : 10;
     if (pass) {
-      const uint32_t top = ~0u << shift;  // bits fixed so far
-      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
+#pragma unroll 4
       for (int j = tid; j < n; j += kSelThreads) {
-        const uint32_t k = key(j);
-        if ((k & top) == prefix) atomicAdd(&hist[(k >> (shift - bits)) & (bins - 1)], 1);
+        const unsigned long long k = packed(j);
+        if (k >> shift == bound >> shift) atomicAdd(&hist[(uint32_t)(k >> (shift - bits)) & ((1u << bits) - 1)], 1);
       }
     }
     shift -= bits;
@@ -249,7 +270,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
     constexpr int OWN = 2048 / kSelThreads;
     uint32_t c[OWN], sum = 0, total;
 #pragma unroll
-    for (int i = 0; i < OWN; ++i) sum += c[i] = hist[2047 - OWN * tid - i];
+    for (int i = 0; i < OWN; ++i) {
+      sum += c[i] = hist[2047 - OWN * tid - i];
+      hist[2047 - OWN * tid - i] = 0;
+    }
     uint32_t above = cta_scan(sum, sm_scan, &total);
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
@@ -257,57 +281,75 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
       above += c[i];
     }
     __syncthreads();
-    prefix |= sm_bin << shift;
+    bound |= (unsigned long long)sm_bin << shift;
     need -= sm_above;
+    if (sm_count <= kRankMost || shift == 0) break;
   }
-  // prefix: the smallest key kept; `need` of the sm_count equal to it stay, the lowest slots first
-  const bool ties = need < sm_count;
+  if (shift > 0) {  // rank those that share the bits fixed so far; with all fixed there is one
+    __syncthreads();
+    if (tid == 0) sm_count = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = tid; j < n; j += kSelThreads) {
+      const unsigned long long k = packed(j);
+      if (k >> shift == bound >> shift) sm_near[atomicAdd(&sm_count, 1)] = k;
+    }
+    __syncthreads();
+    const int near = (int)sm_count;
+    if (tid < near) {
+      const unsigned long long mine = sm_near[tid];
+      uint32_t rank = 0;
+      for (int i = 0; i < near; ++i) rank += sm_near[i] > mine;
+      if (rank == need - 1) sm_bound = mine;
+    }
+    __syncthreads();
+    bound = sm_bound;
+  }
   int2* mv = a.moves + (int64_t)unit * a.max_moves;
+  const int half = (n + 1) / 2;  // (at most half of the slots move: two lists fit the place of the keys)
   uint32_t moved_to = 0, moved_from = 0;
   for (int c0 = 0; c0 < n; c0 += kMaxSmemKeys) {  // (one round where SMEM)
     const int m = min(n - c0, kMaxSmemKeys), words = (m + 31) / 32;
+#pragma unroll 4
     for (int i = warp; i < words; i += kSelThreads / 32) {
       const int j = c0 + 32 * i + lane;
-      const uint32_t k = j < n ? key(j) : 0;
-      const uint32_t more = __ballot_sync(0xffffffffu, j < n && k > prefix);
-      const uint32_t equal = __ballot_sync(0xffffffffu, j < n && k == prefix);
-      if (lane == 0) sm_more[i] = more, sm_equal[i] = equal;
+      const uint32_t keep = __ballot_sync(0xffffffffu, j < n && packed(j < n ? j : 0) >= bound);
+      if (lane == 0) sm_keep[i] = keep;
     }
     __syncthreads();
-    const int per = (words + kSelThreads - 1) / kSelThreads;
-    const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
-    uint32_t total;
-    if (ties) {
-      uint32_t count = 0;
-      for (int i = w0; i < w1; ++i) count += __popc(sm_equal[i]);
-      uint32_t before = cta_scan(count, sm_scan, &total);
-      for (int i = w0; i < w1; ++i) {
-        uint32_t rest = sm_equal[i], keep = 0;
-        for (; rest && before < need; ++before) {
-          keep |= rest & (0u - rest);
-          rest &= rest - 1;
-        }
-        before += __popc(rest);
-        sm_equal[i] = keep;
-      }
-      need -= min(need, total);
-    }
     // the slots of word i that a move frees (below the budget) or takes its row from (above it)
     auto freed = [&](int i) {
       const int b = a.budget - c0 - 32 * i;
-      return b <= 0 ? 0u : ~(sm_more[i] | sm_equal[i]) & (b >= 32 ? ~0u : (1u << b) - 1);
+      return b <= 0 ? 0u : ~sm_keep[i] & (b >= 32 ? ~0u : (1u << b) - 1);
     };
     auto taken = [&](int i) {
       const int b = a.budget - c0 - 32 * i;
-      return b >= 32 ? 0u : (sm_more[i] | sm_equal[i]) & (b <= 0 ? ~0u : ~((1u << b) - 1));
+      return b >= 32 ? 0u : sm_keep[i] & (b <= 0 ? ~0u : ~((1u << b) - 1));
     };
-    uint32_t counts = 0;  // freed in the low, taken in the high half: at most kMaxSmemKeys < 2^16 of each
+    const int per = (words + kSelThreads - 1) / kSelThreads;
+    const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    uint32_t total, counts = 0;  // freed in the low, taken in the high half: at most kMaxSmemKeys < 2^16 of each
     for (int i = w0; i < w1; ++i) counts += __popc(freed(i)) + (__popc(taken(i)) << 16);
-    const uint32_t before = cta_scan(counts, sm_scan, &total);
-    uint32_t to = moved_to + (before & 0xffff), src = moved_from + (before >> 16);
+    uint32_t before = cta_scan(counts, sm_scan, &total);
     for (int i = w0; i < w1; ++i) {
-      for (uint32_t x = freed(i); x; x &= x - 1) mv[to++].x = c0 + 32 * i + __ffs(x) - 1;
-      for (uint32_t x = taken(i); x; x &= x - 1) mv[src++].y = c0 + 32 * i + __ffs(x) - 1;
+      sm_at[i] = before;
+      before += __popc(freed(i)) + (__popc(taken(i)) << 16);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = warp; i < words; i += kSelThreads / 32) {  // a lane per slot
+      const uint32_t f = freed(i), t = taken(i), lower = (1u << lane) - 1, at = sm_at[i];
+      const int j = c0 + 32 * i + lane;
+      if (f >> lane & 1) {
+        const uint32_t to = moved_to + (at & 0xffff) + __popc(f & lower);
+        if (SMEM) keys[to] = j;
+        else mv[to].x = j;
+      }
+      if (t >> lane & 1) {
+        const uint32_t src = moved_from + (at >> 16) + __popc(t & lower);
+        if (SMEM) keys[half + src] = j;
+        else mv[src].y = j;
+      }
     }
     moved_to += total & 0xffff;
     moved_from += total >> 16;
@@ -315,6 +357,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   }
   const int moved = (int)moved_from;  // as many as were freed: budget slots are kept in all
   if (LPR == 0 && tid == 0) a.counts[unit] = moved;
+  if (SMEM) {
+#pragma unroll 4
+    for (int i = tid; i < moved; i += kSelThreads) mv[i] = make_int2((int)keys[i], (int)keys[half + i]);
+  }
+  __syncthreads();
   finish_moves<LPR>(a, mv, moved, row, head, base, w, sp);
 }
 
