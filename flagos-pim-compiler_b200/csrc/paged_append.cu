@@ -10,13 +10,19 @@
 // 16 bytes at dim d and the 16 bytes at d + head_dim / 2, which the rotation mixes, so
 // nothing is exchanged between threads.  A token's row, slot and page are found once per
 // CTA (one thread per token) and shared.
+//
+// Many tokens: a CTA takes whole tokens, a round of its threads after another (8 prompts of up to 2048
+// tokens x 96 heads, 392 MB: 67.6 us, 5.8 TB/s, with 128 threads; 71 with 256; loads issued ahead of the
+// rows and pages, or several rounds at once, cost registers and with them CTAs: 76 to 82 us).  Few: a CTA
+// takes one round's pieces, so that a token is spread over several, and loads them before it knows where
+// they go (one token x 96 heads: 2.8 us against 4.1).
 
 #include "paged.cuh"
 
 namespace pim {
 
-constexpr int kAppendThreads = 256;
-constexpr int kAppendTokens = 64;  // most tokens of a CTA
+constexpr int kAppendThreads = 128;
+constexpr int kAppendTokens = 72;  // most tokens of a CTA (a token has at least 4 items)
 
 struct AppendArgs {
   PagedKV kv;
@@ -35,11 +41,70 @@ struct AppendArgs {
   int* err;
 };
 
+// Item (16-byte pair) r of a token: head r / CH (q's, then k's, then v's), dims (r % CH) V .. and half a head further.
 template <typename T, int HD>
+struct AppendItem {
+  static constexpr int V = VecW<T>::n, HALF = HD / 2, CH = HALF / V;
+  int head, c, h;
+  bool is_q, is_v;
+  __device__ __forceinline__ AppendItem(const AppendArgs& a, int r) {
+    head = r / CH;
+    c = r - head * CH;
+    is_q = head < a.hq;
+    is_v = head >= a.hq + a.kv.hkv;
+    h = is_q ? head : is_v ? head - a.hq - a.kv.hkv : head - a.hq;
+  }
+  __device__ __forceinline__ const T* source(const AppendArgs& a, int64_t t) const {
+    return is_q   ? static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)h * HD
+           : is_v ? static_cast<const T*>(a.v) + t * a.v_stride + h * a.v_head_stride
+                  : static_cast<const T*>(a.k) + t * a.k_stride + h * a.k_head_stride;
+  }
+  __device__ __forceinline__ int first(const AppendArgs& a) const { return a.pair_order ? 2 * c * V : c * V; }
+  __device__ __forceinline__ int second(const AppendArgs& a) const { return a.pair_order ? 2 * c * V + V : HALF + c * V; }
+  // Rotates the pair and writes it to its q_out row or slot (page offset `at`).
+  __device__ __forceinline__ void put(const AppendArgs& a, int64_t t, int row, int slot, int pos, int64_t at,
+                                      const int4& r1, const int4& r2) const {
+    T* dst = is_q ? static_cast<T*>(a.q_out) + t * a.q_out_stride + (int64_t)h * HD
+                  : static_cast<T*>(is_v ? a.kv.v : a.kv.k) + at + ((int64_t)h << a.kv.ps_log2) * HD;
+    float x1[V], x2[V];
+    unpack(r1, x1, T());
+    unpack(r2, x2, T());
+    if (a.pair_order) {  // (1st, 2nd) of each pair were adjacent
+      float y[2 * V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = x1[e], y[V + e] = x2[e];
+#pragma unroll
+      for (int e = 0; e < V; ++e) x1[e] = y[2 * e], x2[e] = y[2 * e + 1];
+    }
+    if (!is_v && a.cos) {
+      const float* cp = a.cos + (int64_t)pos * HALF + c * V;
+      const float* sp = a.sin + (int64_t)pos * HALF + c * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float cs = cp[e], sn = sp[e];
+        const float o1 = x1[e] * cs - x2[e] * sn, o2 = x2[e] * cs + x1[e] * sn;
+        x1[e] = o1;
+        x2[e] = o2;
+      }
+    }
+    *reinterpret_cast<int4*>(dst + c * V) = pack(x1, T());
+    *reinterpret_cast<int4*>(dst + HALF + c * V) = pack(x2, T());
+    if (is_v && c == 0 && a.weights) {
+      const int64_t o = row * a.state_row_stride + h * a.state_head_stride + slot;
+      a.slot_positions[o] = pos;
+      a.weights[o] = 0.f;
+    }
+  }
+};
+
+// FEW: a CTA has one item per thread of the run [128 blockIdx.x, ..) of all tokens' items; else whole tokens.
+template <typename T, int HD, bool FEW>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a, int tokens_per_cta, int work_ctas) {
-  constexpr int V = VecW<T>::n, HALF = HD / 2, CH = HALF / V;  // CH 16-byte pairs a head
+  using Item = AppendItem<T, HD>;
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0 && a.starts && (a.starts[0] < 0 || a.starts[a.kv.rows] > a.tokens))
+    raise_flag(a.err);
   if ((int)blockIdx.x >= work_ctas) {  // the lengths after the call
     const int b = (blockIdx.x - work_ctas) * kAppendThreads + threadIdx.x;
     if (b < a.kv.rows) {
@@ -50,12 +115,23 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a, in
     }
     return;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0 && a.starts && (a.starts[0] < 0 || a.starts[a.kv.rows] > a.tokens))
-    raise_flag(a.err);
   __shared__ int s_row[kAppendTokens], s_slot[kAppendTokens], s_pos[kAppendTokens];
   __shared__ int64_t s_at[kAppendTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * tokens_per_cta;
-  const int nt = (int)min((int64_t)tokens_per_cta, a.tokens - t0);
+  const int per = (a.hq + 2 * a.kv.hkv) * Item::CH;  // items of a token
+  const int64_t begin = FEW ? (int64_t)blockIdx.x * kAppendThreads : 0;
+  const int64_t t0 = FEW ? begin / per : (int64_t)blockIdx.x * tokens_per_cta;
+  const int skip = FEW ? (int)(begin - t0 * per) : 0;  // items of token t0 that the CTA before has
+  const int count = FEW ? (int)min((int64_t)kAppendThreads, a.tokens * per - begin)
+                        : (int)min((int64_t)tokens_per_cta, a.tokens - t0) * per;
+  const int nt = (skip + count + per - 1) / per;
+  int4 r1, r2;
+  if (FEW) {
+    const int i = skip + threadIdx.x, ti = i / per;
+    const Item item(a, i - ti * per);
+    const T* src = item.source(a, t0 + ti);
+    r1 = ld_once_if(reinterpret_cast<const int4*>(src + item.first(a)), (int)threadIdx.x < count);
+    r2 = ld_once_if(reinterpret_cast<const int4*>(src + item.second(a)), (int)threadIdx.x < count);
+  }
   if ((int)threadIdx.x < nt) {
     const int64_t t = t0 + threadIdx.x;
     int row = -1;
@@ -86,61 +162,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a, in
     s_at[threadIdx.x] = at;
   }
   __syncthreads();
-  const int heads = a.hq + 2 * a.kv.hkv, per = heads * CH;
-  for (int i = threadIdx.x; i < nt * per; i += kAppendThreads) {
-    const int ti = i / per, r = i - ti * per;
-    const int head = r / CH, c = r - head * CH;
-    const int64_t at = s_at[ti];
+  for (int n = threadIdx.x; n < count; n += kAppendThreads) {
+    const int i = skip + n, ti = i / per;
+    const int64_t at = s_at[ti], t = t0 + ti;
     if (at < 0) continue;
-    const int64_t t = t0 + ti;
-    const bool is_q = head < a.hq, is_v = head >= a.hq + a.kv.hkv;
-    const int h = is_q ? head : is_v ? head - a.hq - a.kv.hkv : head - a.hq;
-    const T* src;
-    T* dst;
-    if (is_q) {
-      src = static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)h * HD;
-      dst = static_cast<T*>(a.q_out) + t * a.q_out_stride + (int64_t)h * HD;
-    } else {
-      src = is_v ? static_cast<const T*>(a.v) + t * a.v_stride + h * a.v_head_stride
-                 : static_cast<const T*>(a.k) + t * a.k_stride + h * a.k_head_stride;
-      dst = static_cast<T*>(is_v ? a.kv.v : a.kv.k) + at + (((int64_t)h << a.kv.ps_log2)) * HD;
+    const Item item(a, i - ti * per);
+    if (!FEW) {
+      const T* src = item.source(a, t);
+      r1 = *reinterpret_cast<const int4*>(src + item.first(a));
+      r2 = *reinterpret_cast<const int4*>(src + item.second(a));
     }
-    int4 r1, r2;
-    if (a.pair_order) {
-      r1 = *reinterpret_cast<const int4*>(src + 2 * c * V);
-      r2 = *reinterpret_cast<const int4*>(src + 2 * c * V + V);
-    } else {
-      r1 = *reinterpret_cast<const int4*>(src + c * V);
-      r2 = *reinterpret_cast<const int4*>(src + HALF + c * V);
-    }
-    float x1[V], x2[V];
-    unpack(r1, x1, T());
-    unpack(r2, x2, T());
-    if (a.pair_order) {  // (1st, 2nd) of each pair were adjacent
-      float y[2 * V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = x1[e], y[V + e] = x2[e];
-#pragma unroll
-      for (int e = 0; e < V; ++e) x1[e] = y[2 * e], x2[e] = y[2 * e + 1];
-    }
-    if (!is_v && a.cos) {
-      const float* cp = a.cos + (int64_t)s_pos[ti] * HALF + c * V;
-      const float* sp = a.sin + (int64_t)s_pos[ti] * HALF + c * V;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float cs = cp[e], sn = sp[e];
-        const float o1 = x1[e] * cs - x2[e] * sn, o2 = x2[e] * cs + x1[e] * sn;
-        x1[e] = o1;
-        x2[e] = o2;
-      }
-    }
-    *reinterpret_cast<int4*>(dst + c * V) = pack(x1, T());
-    *reinterpret_cast<int4*>(dst + HALF + c * V) = pack(x2, T());
-    if (is_v && c == 0 && a.weights) {
-      const int64_t o = s_row[ti] * a.state_row_stride + h * a.state_head_stride + s_slot[ti];
-      a.slot_positions[o] = s_pos[ti];
-      a.weights[o] = 0.f;
-    }
+    item.put(a, t, s_row[ti], s_slot[ti], s_pos[ti], at, r1, r2);
   }
 }
 
@@ -149,12 +181,18 @@ static cudaError_t append(const AppendArgs& a, int hd, int dtype, cudaStream_t s
     using T = decltype(t);
     constexpr int HD = decltype(d)::value;
     const int per = (a.hq + 2 * a.kv.hkv) * (HD / 2 / VecW<T>::n);
-    int tpc = 2 * kAppendThreads / per;  // tokens of a CTA: two rounds of its threads
-    tpc = tpc < 1 ? 1 : tpc > kAppendTokens ? kAppendTokens : tpc;
-    const int work = ceil_div(a.tokens, tpc);
+    const int64_t items = a.tokens * per;
     const int tail = a.lengths_out || a.positions_out ? ceil_div(a.kv.rows, kAppendThreads) : 0;
-    if (work + tail == 0) return cudaSuccess;
-    return launch_pdl(append_kernel<T, HD>, dim3(work + tail), dim3(kAppendThreads), 0, st, a, tpc, work);
+    // few: the items do not fill the GPU's threads
+    if (items <= 2048 * 148) {
+      const int work = ceil_div(items, kAppendThreads);
+      if (work + tail == 0) return cudaSuccess;
+      return launch_pdl(append_kernel<T, HD, true>, dim3(work + tail), dim3(kAppendThreads), 0, st, a, 0, work);
+    }
+    int tpc = 2 * kAppendThreads / per;  // tokens of a CTA: two rounds of its threads
+    tpc = tpc < 1 ? 1 : tpc > 64 ? 64 : tpc;
+    const int work = ceil_div(a.tokens, tpc);
+    return launch_pdl(append_kernel<T, HD, false>, dim3(work + tail), dim3(kAppendThreads), 0, st, a, tpc, work);
   });
 }
 

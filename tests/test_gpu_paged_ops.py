@@ -270,6 +270,7 @@ def test_append(hq, heads, hd, ps, new, past, rotate, pair_order, dt):
     before = [p.clone() for p in (pool.k, pool.v)]
     tokens = sum(new)
     pad = 3  # tokens behind the last row: left out
+    torch.manual_seed(hq + hd + tokens)
     qkv = torch.randn(tokens + pad, (hq + 2 * heads) * hd, device="cuda").to(_tdt(dt))
     q, k, v = (x.view(tokens + pad, -1, hd) for x in qkv.split([hq * hd, heads * hd, heads * hd], dim=1))
     starts = np.r_[0, np.cumsum(new)].astype(np.int32)
@@ -288,8 +289,8 @@ def test_append(hq, heads, hd, ps, new, past, rotate, pair_order, dt):
     args = (pool.table_np, past, starts, positions, _host(q), _host(k), _host(v))
     wk, wv, wq = ref.append(_host(before[0]), _host(before[1]), *args, c, s, pair_order)
     # |x1 c - x2 s| in fp32: two rounded products and their sum, each off by 2^-24 of at most |x1 c| + |x2 s|
-    mk, mv, mq = (4.0 * 2.0**-24 * 8.0 if rotate else 0.0,) * 3  # |x| < 5.7 here: |x1 c| + |x2 s| <= 5.7 sqrt 2 < 8.1
-    assert float(qkv.float().abs().max()) < 5.65
+    # (and c, s are of one angle: |x1 c| + |x2 s| <= sqrt 2 max |x|)
+    mk, mv, mq = (4.0 * 2.0**-24 * 2.0**0.5 * float(qkv.float().abs().max()) if rotate else 0.0,) * 3
     for got, want, m in ((pool.k, wk, mk), (pool.v, wv, mv)):
         got = _host(got)
         assert np.array_equal(np.isnan(got), np.isnan(want))
