@@ -342,7 +342,7 @@ struct BeamReorderArgs {
   int* err;
 };
 
-constexpr int kReorderThreads = 256;
+constexpr int kReorderThreads = 64;  // (at least kMaxBeams)
 constexpr int kCopyPieces = 8 * kReorderThreads;
 
 __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(BeamReorderArgs a) {
@@ -552,7 +552,7 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   // About a third of the rows copy: enough CTAs per row that those fill the GPU, and no more than there are steps.
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
   const int rows = a->batch * a->beams;
-  int64_t by = ceil_div(24 * 148, rows);
+  int64_t by = ceil_div(96 * 148, rows);
   by = by < steps ? by : steps;
   return report_cuda(launch_pdl(beam_reorder_kernel, dim3(rows, (unsigned)by), dim3(kReorderThreads), 0,
                                 (cudaStream_t)stream, d),

@@ -38,8 +38,8 @@ struct EvictArgs {
 constexpr int kSelThreads = 512;
 constexpr int kMaxSmemKeys = 48 * 1024;
 constexpr int kChunkWords = kMaxSmemKeys / 32;
-constexpr int kMoveThreads = 256;
-constexpr int kFusedMoves = 256;  // see evict_rows()
+constexpr int kMoveThreads = 128;
+constexpr int kFusedMoves = 128;  // see evict_rows()
 constexpr int kFewEvicted = 8;
 constexpr int kRankMost = 256;
 
@@ -76,7 +76,9 @@ __device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* sm, uint32_t*
 // Up to kWarpMoves moves of a unit's list by one warp.  Each lane finds one row (the freed or the
 // kept slot of a move: one table entry), then all lanes copy 16-byte pieces (LPR of them are a K or
 // V row), eight loads under way at a time, with the rows' places taken from the lanes that know them.
-constexpr int kWarpMoves = 16;
+// (8 prompts cut from up to 8190 to 2048 slots x 32 heads, 232 MB of rows: 8 moves a warp and 128 threads a CTA
+// 67.5 us with the selection, 16 and 256 72.7, 4 and 128 72.1.)
+constexpr int kWarpMoves = 8;
 template <int LPR>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves, int row, int head, int count) {
   constexpr int STEPS = kWarpMoves * 2 * LPR / 32, FLY = STEPS < 8 ? STEPS : 8;
