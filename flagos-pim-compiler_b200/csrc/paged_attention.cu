@@ -34,6 +34,7 @@
 // the scores and the second adds the probabilities (4 bytes per key and query head, written
 // and read back mostly in L2).
 
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "paged.cuh"
@@ -52,7 +53,8 @@ struct PagedAttnArgs {
   int64_t w_row_stride, w_head_stride;
   int* err;
   int head_tiles;   // of a kv head's query group
-  int whole_warps;  // a CTA of so many warps per unit (paged_whole_kernel); 0: split
+  int whole_warps;  // CTAs of so many warps for whole units (paged_whole_kernel); 0: split
+  int cluster;      // CTAs that share a unit there
   int ctas;
   int64_t* cost;    // [rows + 1] cost of the units of the rows before, and of all
   float* part_stat; // [ctas][2][NH][2]  max, sum
@@ -63,6 +65,7 @@ struct PagedAttnArgs {
 };
 
 constexpr int kTile = 64;          // keys of a tile
+constexpr int kMaxCluster = 8;
 constexpr int kUnitCost = 2;       // what a unit costs beside its tiles, in tiles: see the head of the file
 constexpr int kSplitWarps = 4;     // of a CTA that walks a range of tiles
 // CTAs of the splitting kernel per SM: what its registers allow without spilling.
@@ -517,33 +520,80 @@ struct Joint {
   }
 };
 
-// A CTA per unit: rows short enough for one to walk, with their scores in shared memory where the weights are asked
-// for.  One launch and no workspace.
+// A CTA, or a cluster of a.cluster CTAs, per unit: rows short enough for it to walk, with their scores in shared memory
+// where the weights are asked for.  One launch and no workspace: a cluster's CTAs take an equal part of the tiles each and
+// join through one another's shared memory.
 template <typename Core, int HD, int NH, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) paged_whole_kernel(PagedAttnArgs a) {
   using T = typename Core::T;
+  constexpr int THREADS = WARPS * 32;
   extern __shared__ float sm_scores[];  // [NH][score_stride]
   __shared__ Joint<Core, HD, NH, WARPS> joint;
+  __shared__ float sm_part[NH * HD], sm_stat[kMaxCluster][NH][2];  // this CTA's part; every CTA's max and sum
   const int tid = threadIdx.x;
   pdl_trigger();
   pdl_wait();
-  const int units = a.kv.hkv * a.head_tiles;
-  const int row = blockIdx.x / units, unit = blockIdx.x - row * units;
+  const int units = a.kv.hkv * a.head_tiles, at = blockIdx.x / a.cluster, rank = blockIdx.x - at * a.cluster;
+  const int row = at / units, unit = at - row * units;
   const int kvh = unit / a.head_tiles, ht = unit - kvh * a.head_tiles;
   const int head0 = kvh * a.group + ht * NH, nh = min(NH, a.group - ht * NH);
-  const int len = row_length(a, row);
+  const int len = row_length(a, row), tiles = (len + kTile - 1) / kTile;
   if (tid == 0 && len != a.lengths[row]) raise_flag(a.err);
-  joint.run(a, row, kvh, head0, nh, 0, len, a.weights ? sm_scores : nullptr, [&](int h, int d, float A) {
-    const float L = joint.sum[h];
-    static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+  const int begin = rank * tiles / a.cluster * kTile, end = min(len, (rank + 1) * tiles / a.cluster * kTile);
+  T* out = static_cast<T*>(a.out) + row * a.out_stride + (int64_t)head0 * HD;
+  // (the scores of this CTA's keys: key `begin` is at sm_scores[0])
+  joint.run(a, row, kvh, head0, nh, begin, end, a.weights ? sm_scores - begin : nullptr, [&](int h, int d, float A) {
+    if (a.cluster > 1) {
+      sm_part[h * HD + d] = A;
+    } else {
+      const float L = joint.sum[h];
+      out[h * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+    }
   });
+  if (a.cluster > 1) {
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    for (int i = tid; i < a.cluster * nh; i += THREADS) {
+      const int r = i / nh, h = i - r * nh;
+      const auto* theirs = cluster.map_shared_rank(&joint, r);
+      sm_stat[r][h][0] = theirs->none[h] ? -INFINITY : theirs->top[h];
+      sm_stat[r][h][1] = theirs->sum[h];
+    }
+    __syncthreads();
+    for (int i = rank * THREADS + tid; i < nh * HD; i += a.cluster * THREADS) {
+      const int h = i / HD;
+      float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < a.cluster) M = fmaxf(M, sm_stat[r][h][0]);
+      const float safe = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < a.cluster) {
+          const float f = exp2f(sm_stat[r][h][0] - safe);
+          L += sm_stat[r][h][1] * f;
+          A += cluster.map_shared_rank(sm_part, r)[i] * f;
+        }
+      out[i] = from_f<T>(L > 0.f ? A / L : 0.f);
+    }
+    cluster.sync();  // (the others may still read this CTA's part; and joint's statistics become the unit's below)
+    if (a.weights && tid < nh) {
+      float M = -INFINITY, L = 0.f;
+      for (int r = 0; r < a.cluster; ++r) M = fmaxf(M, sm_stat[r][tid][0]);
+      const float safe = M == -INFINITY ? 0.f : M;
+      for (int r = 0; r < a.cluster; ++r) L += sm_stat[r][tid][1] * exp2f(sm_stat[r][tid][0] - safe);
+      joint.top[tid] = safe;
+      joint.sum[tid] = L;
+    }
+    __syncthreads();
+  }
   if (!a.weights) return;
   float* w = a.weights + row * a.w_row_stride + (int64_t)kvh * a.w_head_stride;
-  for (int key = tid; key < len; key += WARPS * 32) {
+  for (int key = begin + tid; key < end; key += THREADS) {
     float p = 0.f;
     for (int h = 0; h < nh; ++h) {
       const float L = joint.sum[h];
-      p += L > 0.f ? exp2f(sm_scores[h * a.score_stride + key] - joint.top[h]) * (1.f / L) : 0.f;
+      p += L > 0.f ? exp2f(sm_scores[h * a.score_stride + key - begin] - joint.top[h]) * (1.f / L) : 0.f;
     }
     w[key] += p;
   }
@@ -838,8 +888,10 @@ static cudaError_t launch_whole(const PagedAttnArgs& a, cudaStream_t st) {
   const size_t smem = a.weights ? (size_t)NH * a.score_stride * 4 : 0;
   cudaError_t e;
   if (resident_ctas(paged_whole_kernel<Core, HD, NH, WARPS>, WARPS * 32, smem, cache, &e) < 0) return e;
-  return launch_pdl(paged_whole_kernel<Core, HD, NH, WARPS>, dim3(a.kv.rows * a.kv.hkv * a.head_tiles),
-                    dim3(WARPS * 32), smem, st, a);
+  const dim3 grid(a.kv.rows * a.kv.hkv * a.head_tiles * a.cluster);
+  return a.cluster > 1 ? launch_pdl_cluster(paged_whole_kernel<Core, HD, NH, WARPS>, a.cluster, grid, dim3(WARPS * 32), smem,
+                                            st, a)
+                       : launch_pdl(paged_whole_kernel<Core, HD, NH, WARPS>, grid, dim3(WARPS * 32), smem, st, a);
 }
 
 template <typename Core, int HD, int NH>
@@ -898,7 +950,7 @@ static const char* paged_attention_error(const pim_paged_attention_args* a, int 
 struct PagedLayout {
   int nh, tiles, ctas;
   bool whole;
-  int whole_warps;
+  int whole_warps, cluster;
   int64_t score_stride, stat, acc, row_stat, scores, bytes;
 };
 static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
@@ -908,17 +960,27 @@ static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
   p.tiles = ceil_div(group, p.nh);
   p.ctas = paged_ctas(dtype, a->kv.head_dim);
   const int64_t slots = (int64_t)a->kv.max_pages * a->kv.page_size, units = (int64_t)a->kv.rows * a->kv.kv_heads * p.tiles;
-  // A CTA per unit saves the second launch and the join, and loses where rows are long: with few units 8 warps a CTA win
-  // up to 512 slots (1 row x 32 heads bf16: 4.4, 5.5, 7.3, 11.2 us at 128, 256, 512, 1024 slots against 8.3, 9.0, 9.6, 9.9
-  // split; 16 x 4 fp32: 3.4, 5.0, 7.8, 16.5 against 8.4, 8.8, 10.1, 12.5).  With more units than SMs fewer warps a CTA are
-  // better, bf16 2 up to 256 slots (128 rows x 8 heads x 8: 22.6, 35.6, 60.8 us at 128, 256, 512 against 38.6, 46.7,
-  // 61.7), fp32 4 up to 512 (64 x 8 x 4: 8.6, 16.6, 30.5, 56.7 at 128 .. 1024 against 17.3, 24.7, 34.7, 55.8).  A query
-  // group of several tiles would add to the same weights from several CTAs: it is split.
-  const bool many = units > 2 * 148;
-  p.whole_warps = many ? (dtype == PIM_BF16 ? 2 : 4) : p.nh > 8 ? 4 : 8;
-  p.whole = slots <= (many && dtype == PIM_BF16 ? 256 : 512) && (!a->weights || p.tiles == 1);
+  // Whole units in a CTA or a cluster save the second launch and the join, and lose where rows are long or units many.
+  // Few units: 8 warps a CTA and the largest cluster that leaves every CTA an SM, up to 512 slots a CTA (fp32 256); one CTA
+  // up to 256 slots, where a cluster gains nothing.  Device us by slots 256, 512, 1024, 2048, 4000:
+  //   1 row x 8 heads x 4    clusters of 8  5.6  5.7  6.5  7.6  9.5   one CTA 5.6  7.5          split - 8.5  9.5  9.9 11.8
+  //   1 row x 32 heads x 1   clusters of 4  5.4  6.3  7.4 12.1    -   one CTA 5.5  7.3 11.2     split 9.0 9.6  9.4 12.9 18.4
+  //   8 rows x 8 heads x 8   clusters of 2  7.2  8.2 11.2 20.9    -   one CTA 6.0  7.9 13.9     split 11.5 11.9 13.0 18.4
+  //   fp32 1 row x 4 heads   clusters of 8  5.6  5.9  6.4  8.0 11.3                             split   -   -  7.2  7.9  9.7
+  // More units than SMs twice over: fewer warps a CTA, bf16 2 up to 256 slots (128 rows x 8 heads x 8: 22.6, 35.6, 60.8 us
+  // at 128, 256, 512 against 38.6, 46.7, 61.7 split), fp32 4 up to 512 (64 x 8 x 4: 8.6, 16.6, 30.5, 56.7 at 128 .. 1024
+  // against 17.3, 24.7, 34.7, 55.8).  A query group of several tiles would add to the same weights from several CTAs: it is
+  // split.
+  const bool bf16 = dtype == PIM_BF16, many = units > 2 * 148;
+  p.whole_warps = many ? (bf16 ? 2 : 4) : p.nh > 8 ? 4 : 8;
+  p.cluster = 1;
+  if (slots > 256)
+    while (p.cluster < kMaxCluster && units * p.cluster * 2 * p.whole_warps <= 8 * 148) p.cluster *= 2;
+  const int64_t most = p.cluster > 1 ? (bf16 ? 512 : 256) * p.cluster : many && bf16 ? 256 : 512;
+  p.whole = slots <= (most > 512 || many ? most : 512) && (!a->weights || p.tiles == 1);
   p.score_stride = (slots + 63) / 64 * 64;
   if (p.whole) {
+    p.score_stride = (p.score_stride / p.cluster + 127) / 64 * 64;  // a CTA's part is a tile more at most
     p.stat = p.acc = p.row_stat = p.scores = p.bytes = 0;
     return p;
   }
@@ -973,6 +1035,7 @@ extern "C" int pim_paged_attention(const pim_paged_attention_args* a, int32_t dt
   d.head_tiles = p.tiles;
   d.ctas = p.ctas;
   d.whole_warps = p.whole ? p.whole_warps : 0;
+  d.cluster = p.cluster;
   d.score_stride = p.score_stride;
   if (!p.whole) {
     char* ws = static_cast<char*>(workspace);

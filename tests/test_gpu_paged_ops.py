@@ -112,13 +112,19 @@ def _check_attention(pool, q, out, w0, weights, dt, scale=None, lengths=None):
         assert np.array_equal(got_w[:, n:], old[:, n:])
 
 
+# One CTA per unit, a cluster per unit, and the split: by the slots that the table holds.
+LENGTHS = {"one": [1, 0, 7, 8, 9, 63, 64, 65, 130, 200, 0, 256], "cluster": [1, 0, 7, 8, 9, 63, 64, 65, 130, 257, 0, 513],
+           "split": [1, 0, 7, 8, 9, 63, 64, 65, 130, 257, 0, 4200]}
+
+
 @pytest.mark.parametrize("track", [False, True])
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 @pytest.mark.parametrize("hd", [32, 64, 128])
 @pytest.mark.parametrize("group,heads,ps", [(1, 3, 16), (2, 2, 8), (4, 1, 32), (7, 2, 64), (8, 1, 16), (12, 1, 128),
                                             (16, 2, 16), (33, 1, 8)])
-def test_attention_groups_and_dims(group, heads, ps, hd, dt, track):
-    lengths = [1, 0, 7, 8, 9, 63, 64, 65, 130, 257, 0, 513]
+@pytest.mark.parametrize("form", list(LENGTHS))
+def test_attention_groups_and_dims(form, group, heads, ps, hd, dt, track):
+    lengths = LENGTHS[form]
     pool, q, out, w0, weights, op = _attention_case(lengths, group, heads, ps, hd, dt, track=track)
     assert op() is out
     _check_attention(pool, q, out, w0, weights, dt)
@@ -127,7 +133,8 @@ def test_attention_groups_and_dims(group, heads, ps, hd, dt, track):
 
 @pytest.mark.parametrize("track", [False, True])
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
-@pytest.mark.parametrize("lengths", [[1], [130], [0], [0, 0, 5, 0], [4097], [2, 9001, 1, 3000], [300] * 70])
+@pytest.mark.parametrize("lengths", [[1], [130], [0], [0, 0, 5, 0], [4090], [4097], [1025], [2, 9001, 1, 3000], [300] * 70,
+                                     [1] * 3 + [2000] + [5] * 12])
 def test_attention_lengths(lengths, dt, track):
     pool, q, out, w0, weights, op = _attention_case(lengths, 4, 2, 16, 128, dt, seed=3, track=track)
     op()
@@ -137,7 +144,7 @@ def test_attention_lengths(lengths, dt, track):
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 def test_attention_many_rows_and_heads(dt):
     rng = np.random.default_rng(5)
-    pool, q, out, w0, weights, op = _attention_case(list(rng.integers(0, 200, 150)), 1, 32, 16, 128, dt, seed=5)
+    pool, q, out, w0, weights, op = _attention_case(list(rng.integers(0, 200, 150)), 1, 32, 16, 128, dt, seed=5, track=True)
     op()
     _check_attention(pool, q, out, w0, weights, dt)
 
