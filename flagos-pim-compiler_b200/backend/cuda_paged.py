@@ -167,7 +167,8 @@ class _Op:
         self._fn = getattr(nat.lib, self.name)
         self._ws, extra = None, ()
         if self.workspace:
-            need = getattr(nat.lib, self.name + "_workspace_bytes")(self._ref, code)
+            with torch.cuda.device(dev):  # (the split goes by the device's SMs)
+                need = getattr(nat.lib, self.name + "_workspace_bytes")(self._ref, code)
             if need < 0:  # the call itself names what is wrong
                 nat.check(self._fn(self._ref, code, None, 0, None), self.name)
             self._ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)

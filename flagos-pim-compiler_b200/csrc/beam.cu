@@ -231,11 +231,6 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
     const int done = a.done ? a.done[row] : 0;
     const float score = a.scores[row];
     unsigned long long* keys = sm_keys + w * a.k;
-    if (done || !isfinite(score)) {
-      for (int j = lane; j < a.k; j += 32) keys[j] = j == 0 && isfinite(score) ? beam_key(0x80000000u, a.pad) : 0;
-      if (lane == 0) sm_shift[w] = score, sm_done[w] = done;
-      continue;
-    }
     // lane i merges lists i, i + 32, ..: the first kDeep keys of each are at hand
     unsigned long long key[Q][kDeep];
     int taken[Q], count[Q];
@@ -253,7 +248,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
         const BeamStats st = a.stats[(int64_t)row * a.splits + l];
         lm[q] = st.max;
         ls[q] = st.sum;
-        count[q] = st.count;
+        count[q] = done ? 0 : st.count;
       }
 #pragma unroll
       for (int d = 0; d < kDeep; ++d) {
@@ -265,11 +260,17 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
       for (int d = 0; d < kDeep; ++d) key[q][d] = d < count[q] ? key[q][d] : 0;
       m = fmaxf(m, lm[q]);
     }
+    // (an ended beam's lists were not written, and are not looked at: its loads only ran beside its flag's)
+    if (done || !isfinite(score)) {
+      for (int j = lane; j < a.k; j += 32) keys[j] = j == 0 && isfinite(score) ? beam_key(0x80000000u, a.pad) : 0;
+      if (lane == 0) sm_shift[w] = score, sm_done[w] = done;
+      continue;
+    }
     m = warp_max(m);
     double s = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-      if (lm[q] != -INFINITY) s += ls[q] * exp2((double)lm[q] - (double)m);
+      if (lm[q] != -INFINITY) s += ls[q] * exp2f(lm[q] - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
@@ -342,7 +343,8 @@ struct BeamReorderArgs {
   int* err;
 };
 
-constexpr int kReorderThreads = 64;  // (at least kMaxBeams)
+constexpr int kReorderThreads = 64;
+static_assert(kReorderThreads >= kMaxBeams, "a thread per beam");
 constexpr int kCopyPieces = 8 * kReorderThreads;
 
 __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(BeamReorderArgs a) {

@@ -935,6 +935,7 @@ static const char* paged_attention_error(const pim_paged_attention_args* a, int 
   if (a->kv.rows > 65535) return "more than 65535 rows";
   if (a->q_heads <= 0 || a->q_heads > 65535 || a->q_heads % a->kv.kv_heads)
     return "q_heads must be a multiple of kv_heads, at most 65535";
+  if ((int64_t)a->kv.rows * a->q_heads > (1 << 27)) return "more than 2^27 rows times heads";
   const int64_t row = (int64_t)a->q_heads * a->kv.head_dim;
   if (a->q_stride < row || a->out_stride < row) return "q or out stride is less than a row";
   if (!aligned16(a->q) || !aligned16(a->out) || a->q_stride * es % 16 || a->out_stride * es % 16)

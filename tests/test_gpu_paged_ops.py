@@ -676,3 +676,84 @@ def test_calls_on_another_stream_and_captured_replays_follow_the_device_values()
     assert one["n2"].tolist() == [24, 14, 24]
     for op in ops1 + ops2:
         op.check()
+
+
+def test_first_call_inside_a_capture():
+    """A capture of calls that have not run before (kernels are loaded and sized during it) replays to the right result."""
+    from backend.cuda_paged import BeamSelect, PagedEvict
+
+    torch = _torch()
+    pool, q, out, _, _, op = _attention_case([5000, 77], 8, 1, 64, 32, "bfloat16", seed=31)
+    logits = torch.randn(1, 3, 777, device="cuda")
+    outs = (torch.zeros(1, 9, device="cuda"), *(torch.zeros(1, 9, dtype=torch.int32, device="cuda") for _ in range(2)))
+    select = BeamSelect(logits, torch.zeros(1, 3, device="cuda"), *outs)
+    w = torch.rand(2, 1, pool.slots, device="cuda")
+    p = torch.arange(pool.slots, device="cuda", dtype=torch.int32).repeat(2, 1, 1)
+    n = _ints([0, 0])
+    evict = PagedEvict(pool.k.clone(), pool.v.clone(), pool.table, pool.lengths, w, p, pool.lengths, torch.zeros_like(w),
+                       torch.zeros_like(p), n, budget=1500, recent=10)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op()
+        select()
+        evict()
+    graph.replay()
+    _check_attention(pool, q, out, None, None, "bfloat16")
+    want = ref.beam_select(_host(logits)[0], np.zeros(3), 9)
+    assert _host(outs[1])[0].tolist() == want[1].tolist() and _host(outs[2])[0].tolist() == want[2].tolist()
+    assert n.tolist() == [1500, 77]
+
+
+def test_two_operators_at_once_on_two_streams():
+    """Each with its own workspace and outputs, over the same pages; as if one ran after the other."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    pool, q, out, _, _, op = _attention_case([9000, 4500, 3, 0], 4, 2, 16, 128, "bfloat16", seed=32)
+    q2 = torch.randn_like(q)
+    out2 = torch.empty_like(q2)
+    op2 = PagedAttention(q2, pool.k, pool.v, pool.table, pool.lengths, out2)
+    op(), op2()
+    want, want2 = out.clone(), out2.clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        out.zero_(), out2.zero_()
+        torch.cuda.synchronize()
+        for st, o in zip(streams, (op, op2)):
+            with torch.cuda.stream(st):
+                o()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out2, want2)
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_of_many_rows(dt):
+    """More rows than a scan's threads take one each, most of them empty or short, one long; more CTAs than tiles and fewer."""
+    rng = np.random.default_rng(33)
+    lengths = list(rng.integers(0, 3, 700)) + [5000] + list(rng.integers(0, 90, 300))
+    pool, q, out, w0, weights, op = _attention_case(lengths, 2, 1, 8, 32, dt, seed=33, track=True)
+    op()
+    _check_attention(pool, q, out, w0, weights, dt)
+
+
+def test_an_operator_dropped_while_its_work_is_pending_keeps_its_memory():
+    """The workspace of an operator used on another stream is not handed out again before that stream's work is done."""
+    torch = _torch()
+    want = None
+    for i in range(6):
+        pool, q, out, _, _, op = _attention_case([30000, 20000], 8, 2, 64, 128, "bfloat16", seed=34)
+        if want is None:
+            op()
+            want = out.clone()
+            out.zero_()
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                op()
+        op = None
+        junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(32)]  # would land in a freed workspace
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        del junk

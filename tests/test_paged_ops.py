@@ -91,6 +91,31 @@ def test_attention_refusals(kw, message):
     assert _status("pim_paged_attention", _attention(), dtype=2)[0] == 1
 
 
+def test_attention_refuses_grids_beyond_its_index_range():
+    rc, said = _status("pim_paged_attention", _attention(_kv(rows=65535, kv_heads=4, page_stride=4 * 16 * 64), q_heads=4096,
+                                                         q_stride=4096 * 64, out_stride=4096 * 64))
+    assert rc == 1 and "2^27" in said
+    rc, said = _status("pim_paged_attention", _attention(_kv(rows=65536)))
+    assert rc == 1 and "65535 rows" in said
+
+
+def test_workspace_follows_the_form():
+    """Short rows run in one launch without a workspace; long ones need the partials, and with weights the scores too."""
+    from backend import _native as nat
+
+    def need(**kw):
+        return nat.lib.pim_paged_attention_workspace_bytes(ctypes.byref(_attention(**kw)), 1)
+
+    assert need() == 0
+    long = _kv(max_pages=1000, table_stride=1000)
+    plain = need(kv=long)
+    assert plain > 0
+    tracked = need(kv=long, weights=P, weights_head_stride=16000, weights_row_stride=32000)
+    assert tracked >= plain + 3 * 4 * 16000 * 4  # rows x heads x slots, fp32
+    rc, said = _status("pim_paged_attention", _attention(kv=long), ws=False)
+    assert rc == 1 and "workspace" in said
+
+
 @pytest.mark.parametrize("kw,message", [
     (dict(tokens=-1), "number of tokens"), (dict(k=None), "null k"), (dict(lengths=None), "null k"),
     (dict(tokens=4), "one token per row"), (dict(q=P), "go together"), (dict(q=P, q_out=P, q_heads=0), "q_heads"),
