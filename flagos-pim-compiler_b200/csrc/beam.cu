@@ -17,6 +17,11 @@
 // logits can make the collection overflow; then the K-th largest of the threads' (unique)
 // 64-bit maxima is the bound, and only K threads can hold keys at or above it.
 //
+// Measured (the three kernels one after another): 4 beams of one prompt, 32000 bf16 logits, 32 layers' pages
+// 12.5 us, three launches' latency; 32 x 8 beams 82 us, of which the page copies, 354 MB, take 61 (5.8 TB/s); 8 x 16
+// beams of 131072 fp32 logits 58 us: the pass over the logits 19.5 us for 53 MB, bound by instructions (51 %
+// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 12, the copies 30.
+//
 // Reordering.  See pim_beam_reorder in pim_b200.h: the table entries of full pages follow
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
 // copies read pages of beams with children and write pages of beams without.

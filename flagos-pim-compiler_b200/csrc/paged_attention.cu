@@ -8,12 +8,23 @@
 //
 // Split.  Lengths are read on the device and differ, so no grid fits them: the units' keys
 // are cut into tiles of 64 and the tiles of all units, in order, are dealt out evenly to as
-// many CTAs as the GPU holds at once (CTA c takes tiles [c T / G, (c + 1) T / G)).  A CTA walks
-// its range unit by unit; units that lie in one CTA are written at once, a unit that spans
-// several leaves a partial (max, sum, o) per CTA, of which a CTA has at most two: its first
-// and its last.  paged_finish_kernel joins them: which CTAs hold a unit follows from the
-// lengths alone, so there are no tickets, no atomics and nothing that must be zero before a
-// call, and the result does not depend on timing.
+// many CTAs as the GPU holds at once (CTA c takes [c T / G, (c + 1) T / G)).  A CTA walks its
+// range unit by unit; units that lie in one CTA are written at once, a unit that spans several
+// leaves a partial (max, sum, o) per CTA, of which a CTA has at most two: its first and its
+// last.  A unit begun costs loads that wait and a join of the warps, about as much as two
+// tiles, and is dealt out at that price (40 rows of 0 to 8192 keys x 64 heads over 8: 129.9 us
+// without the charge, where one CTA drew ten short units and ended at 131 us, the others at 111;
+// 121.4, 115.2, 115.8 and 117.1 with 1, 2, 3 and 5 tiles).  paged_finish_kernel joins the
+// partials: which CTAs hold a unit follows from the lengths alone, so there are no tickets, no
+// atomics and nothing that must be zero before a call, and the result does not depend on timing.
+// Measured: 64 rows x 4096 keys x 32 heads 4.27 GB in 665 us, 6.4 TB/s; the ragged rows above
+// 662 MB in 116 us, 5.7 TB/s (DRAM 70 % busy, tensor pipe 17 %, 8 warps an SM that mostly wait
+// for their loads); what did not help there: a third CTA per SM with fewer registers (139 us),
+// asking L2 for tiles ahead (134 to 145), loads that run on into the next unit (136), 32-byte
+// loads (117), CTAs of 1 or 2 warps (119, 118).
+//
+// Short rows, and longer ones of few units, run in one launch instead, a CTA or a cluster of
+// CTAs per unit: paged_whole_kernel, chosen in paged_layout().
 //
 // bf16: the products run on warp-level MMA (m16n8k16) straight from registers.  The order of
 // the summed dims is free, so a lane takes the 16 bytes at dim 8 t + 32 i of key g (lane = 4 g +
@@ -25,7 +36,7 @@
 // product as two bf16 parts (p = hi + lo, 16 bits of it, so its rounding does not show
 // in the result); with at most 8 heads in a tile the rows 8..15 of the MMA, otherwise idle,
 // carry lo.  tcgen05 would add staging in shared memory and TMEM for a product of 8 rows that
-// the memory system bounds: the warp MMAs are busy for a fifth of the time that K and V take.
+// the memory system bounds.
 //
 // fp32: a key's dims are spread over head_dim / 4 lanes; the partial dot products of several
 // keys and heads are summed by one butterfly that leaves one score per lane.

@@ -14,6 +14,10 @@
 // evict_select_kernel: one CTA per (row, head), keys in shared memory where they fit; it
 // reads 8 bytes a slot and writes the state and the list of moves.  evict_move_kernel: moves
 // the K and V rows, a grid over (row, head) x blocks of moves; bound by DRAM.
+// Measured: 8 prompts of 1500 to 8190 slots x 32 heads cut to 2048 68 us, the selection 19 and the
+// moves, 232 MB in rows of 256 bytes, 40 to 45 (5.2 to 5.8 TB/s); longer lists moved by the
+// selecting CTA itself would take 84 -> 90 us, a single row's 36 -> 52.  16 rows x 8 heads one
+// token over 1024: 3.8 us in one launch (9.9 with histograms and scans, 11.7 in two launches).
 
 #include "paged.cuh"
 
