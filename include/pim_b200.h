@@ -464,8 +464,8 @@ typedef struct pim_paged_evict_args {
  * first into the first; all others stay where they are.  Attention does not depend on the
  * order of slots (K is rotated already) and slot_positions says which token a slot holds.
  * Slots >= lengths_out are left as they were.  Rows must not share pages.  A length out of
- * range is clamped and a row with a page id out of range moves nothing there; both raise
- * *err_flag.  No counterpart in the reference. */
+ * range is clamped, and of a move whose freed or kept slot has a page id out of range only the
+ * state follows, not K and V; both raise *err_flag.  No counterpart in the reference. */
 int pim_paged_evict(const pim_paged_evict_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
                     void* stream);
 int64_t pim_paged_evict_workspace_bytes(const pim_paged_evict_args* a, int32_t dtype);
