@@ -39,9 +39,9 @@ constexpr int kMaxBeams = 64;
 constexpr int kMaxSplits = 128;
 
 struct BeamStats {
-  float max;   // as a power of two: sum counts 2^max; -inf where there is no finite logit
+  float max;   // -inf where there is no finite logit
   int count;   // entries of the chunk's list
-  double sum;  // of exp(x) / 2^max over the chunk's finite logits
+  double sum;  // of exp(x - max) over the chunk's finite logits
 };
 
 struct BeamSelectArgs {
@@ -156,14 +156,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
         if (at < kBeamCand) sm_cand[at] = beam_key(logit_order(x[i]), base + tok(i));
       }
   }
-  // exp(x - m) = 2^(x log2(e) - m2), m2 the rounded m log2(e), with log2(e) in two parts so that the argument carries one
-  // rounding; a thread's 16 or 32 of them in fp32, the sum over threads in fp64.
-  const float m = top ? order_logit(top) : -INFINITY;
-  const float m2 = top ? m * kLog2eHi : 0.f;
+  // exp(x - m) = 2^((x - m) log2(e)), log2(e) in two parts; the difference first, so that logits near the type's limits
+  // (a mask of its lowest value) stay in range.  A thread's 16 or 32 of them in fp32, the sum over threads in fp64.
+  const float m = top ? order_logit(top) : 0.f;
   float part = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i)  // (-inf gives 0: kLog2eLo is positive)
-    part += exp2_approx(fmaf(x[i], kLog2eLo, fmaf(x[i], kLog2eHi, -m2)));
+  for (int i = 0; i < kBeamVals; ++i) {  // (-inf gives 0: kLog2eLo is positive)
+    const float d = x[i] - m;
+    part += exp2_approx(fmaf(d, kLog2eHi, d * kLog2eLo));
+  }
   double s = part;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
 #pragma unroll
       for (int i = 0; i < kBeamVals; ++i) {
         const unsigned long long k = x[i] != -INFINITY ? beam_key(logit_order(x[i]), base + tok(i)) : 0;
-        if (k >= bound) sm_cand[atomicAdd(&sm_n, 1)] = k;  // at most k threads come here, with 16 keys each
+        if (k >= bound) sm_cand[atomicAdd(&sm_n, 1)] = k;  // at most k threads come here, with kBeamVals keys each
       }
     }
     __syncthreads();
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   }
   if (tid == 0) {
     BeamStats st;
-    st.max = top ? m2 : -INFINITY;
+    st.max = top ? m : -INFINITY;
     st.count = min(n, a.k);
     st.sum = 0;
     for (int w = 0; w < kBeamWarps; ++w) st.sum += sm_s[w];
@@ -226,7 +227,8 @@ __device__ __forceinline__ unsigned long long score_order(double s) {
 template <int Q>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArgs a) {
   __shared__ unsigned long long sm_keys[kMaxBeams * kMaxBeams];  // [beams][k], sorted, 0: none
-  __shared__ double sm_shift[kMaxBeams];                         // score_w - lse_w
+  __shared__ double sm_shift[kMaxBeams];                         // score_w - log(sum of exp(x - max))
+  __shared__ float sm_max[kMaxBeams];                            // largest logit; 0 for a beam that has ended
   __shared__ int sm_done[kMaxBeams];
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
@@ -268,18 +270,19 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
     // (an ended beam's lists were not written, and are not looked at: its loads only ran beside its flag's)
     if (done || !isfinite(score)) {
       for (int j = lane; j < a.k; j += 32) keys[j] = j == 0 && isfinite(score) ? beam_key(0x80000000u, a.pad) : 0;
-      if (lane == 0) sm_shift[w] = score, sm_done[w] = done;
+      if (lane == 0) sm_shift[w] = score, sm_max[w] = 0.f, sm_done[w] = done;
       continue;
     }
     m = warp_max(m);
     double s = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-      if (lm[q] != -INFINITY) s += ls[q] * exp2f(lm[q] - m);
+      if (lm[q] != -INFINITY) s += ls[q] * expf(lm[q] - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
-      sm_shift[w] = m == -INFINITY ? 0.0 : (double)score - ((double)m + log2(s)) * 0.69314718055994530942;
+      sm_shift[w] = m == -INFINITY ? 0.0 : (double)score - log(s);
+      sm_max[w] = m;
       sm_done[w] = 0;
     }
     for (int j = 0; j < a.k; ++j) {
@@ -307,7 +310,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
   auto look = [&](int i) {
     const int w = lane + 32 * i;
     const unsigned long long k = w < a.beams && at[i] < a.k ? sm_keys[w * a.k + at[i]] : 0;
-    score[i] = k ? score_order(sm_shift[w] + (sm_done[w] ? 0.0 : (double)order_logit((uint32_t)(k >> 32)))) : 0;
+    // (the maximum is taken off first: at logits of 1e38 the sum's logarithm would be lost beside it)
+    score[i] = k ? score_order(sm_shift[w] + ((double)order_logit((uint32_t)(k >> 32)) - (double)sm_max[w])) : 0;
   };
   look(0);
   look(1);

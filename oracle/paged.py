@@ -101,7 +101,8 @@ def beam_select(logits, scores, k, done=None, eos=-1, pad=0):
         if np.isinf(x).all():
             continue
         top = x.max()
-        c = float(scores[w]) + (x - (top + math.log(np.exp(x - top).sum())))
+        # (the maximum first: at logits of 1e38 the sum's logarithm would be lost beside it)
+        c = float(scores[w]) + ((x - top) - math.log(np.exp(x - top).sum()))
         at = np.nonzero(np.isfinite(c))[0]
         at = at[np.lexsort((at, -c[at]))][:k]
         cand += [(-c[t], w * vocab + int(t)) for t in at]

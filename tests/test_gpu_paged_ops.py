@@ -550,6 +550,23 @@ def test_beam_select_infinities_and_ended_beams(dt):
     _check_select(logits, scores, 8, done, eos=3, pad=4)
 
 
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [40, 9001, 70000])
+def test_beam_select_logits_near_the_types_limits(vocab, dt):
+    """Rows masked whole or in part with the type's lowest value, and logits of its largest: the formula still."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    lim = torch.finfo(_tdt(dt))
+    logits = torch.randn(1, 6, vocab, device="cuda", generator=g).to(_tdt(dt))
+    logits[0, 0] = lim.min                   # a constant row: every token at -log(vocab)
+    logits[0, 1, : vocab - 3] = lim.min      # whole chunks of nothing else
+    logits[0, 2, 7] = lim.max                # one token has it all
+    logits[0, 3, 3:9] = lim.max              # six have
+    logits[0, 4, ::2], logits[0, 4, 1::2] = lim.max, lim.min
+    _check_select(logits, torch.tensor([[0.0, 0.3, -4.0, -2.0, 3.0, 0.1]], device="cuda"), 20)
+    _check_select(logits[:, :1], torch.tensor([[-1.5]], device="cuda"), 5)
+
+
 def test_beam_select_strided_logits():
     torch = _torch()
     for dt in ("float32", "bfloat16"):
