@@ -95,6 +95,8 @@ __device__ __forceinline__ int row_cost(const PagedAttnArgs& a, int row) {
   const int n = row_tiles(a, row);
   return n ? n + kUnitCost : 0;
 }
+// A share of a row's sum: 0 where no key had a score above -inf, NaN where a score was NaN.
+__device__ __forceinline__ float quotient(float a, float sum) { return sum == 0.f ? 0.f : a / sum; }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(WARPS * 32) paged_whole_kernel(PagedAttnArgs a
       sm_part[h * HD + d] = A;
     } else {
       const float L = joint.sum[h];
-      out[h * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+      out[h * HD + d] = from_f<T>(quotient(A, L));
     }
   });
   if (a.cluster > 1) {
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(WARPS * 32) paged_whole_kernel(PagedAttnArgs a
           L += sm_stat[r][h][1] * f;
           A += cluster.map_shared_rank(sm_part, r)[i] * f;
         }
-      out[i] = from_f<T>(L > 0.f ? A / L : 0.f);
+      out[i] = from_f<T>(quotient(A, L));
     }
     cluster.sync();  // (the others may still read this CTA's part; and joint's statistics become the unit's below)
     if (a.weights && tid < nh) {
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(WARPS * 32) paged_whole_kernel(PagedAttnArgs a
     float p = 0.f;
     for (int h = 0; h < nh; ++h) {
       const float L = joint.sum[h];
-      p += L > 0.f ? exp2f(sm_scores[h * a.score_stride + key - begin] - joint.top[h]) * (1.f / L) : 0.f;
+      p += exp2f(sm_scores[h * a.score_stride + key - begin] - joint.top[h]) * quotient(1.f, L);
     }
     w[key] += p;
   }
@@ -692,7 +694,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, paged_ctas_per_sm(Core::kBf1
                   const float L = joint.sum[h];
                   if (whole) {
                     static_cast<T*>(a.out)[row * a.out_stride + (int64_t)(head0 + h) * HD + d] =
-                        from_f<T>(L > 0.f ? A / L : 0.f);
+                        from_f<T>(quotient(A, L));
                   } else {
                     a.part_acc[(slot + h) * HD + d] = A;
                   }
@@ -799,7 +801,7 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
         L += sm_l[w] * f;
         A += sm_acc[w][d] * f;
       }
-      static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(L > 0.f ? A / L : 0.f);
+      static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(quotient(A, L));
     }
     return;
   }
@@ -841,7 +843,7 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
         l = warp_sum(l * exp2f(m - safe));
         m = safe;
       }
-      if (lane == 0) sm_stat[i][0] = m, sm_stat[i][1] = l > 0.f ? 1.f / l : 0.f;
+      if (lane == 0) sm_stat[i][0] = m, sm_stat[i][1] = quotient(1.f, l);
     }
     __syncthreads();
     for (int i0 = 0; i0 < nh; i0 += AHEAD) {

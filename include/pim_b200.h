@@ -434,8 +434,9 @@ typedef struct pim_paged_attention_args {
 /* Attention of one new token per row over its pages: the decode form of pim_attention over
  * a paged cache, with query groups that share a kv head reading it once.  Rows may share
  * pages.  A length outside [0, max_pages * page_size] is clamped and a page id out of
- * range hides its slots; both raise *err_flag.  fp32 scores, softmax and sums; the output
- * is rounded once.  The result does not depend on timing: no atomics. */
+ * range hides its slots; both raise *err_flag.  A row without slots, or without a score above
+ * -inf, gives zeros; a NaN in a score of a head makes its output and probabilities NaN.  fp32
+ * scores, softmax and sums; the output is rounded once.  The result does not depend on timing: no atomics. */
 int pim_paged_attention(const pim_paged_attention_args* a, int32_t dtype, void* workspace, int64_t workspace_bytes,
                         void* stream);
 /* Bytes of the workspace of a call with these arguments (its lengths are not read); -1 for

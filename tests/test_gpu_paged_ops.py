@@ -158,6 +158,28 @@ def test_attention_scale_and_sharp_scores(dt):
     _check_attention(pool, q, out, w0, weights, dt, scale=0.5)
 
 
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form,slot", [("one", 70), ("one", 199), ("cluster", 0), ("cluster", 300), ("split", 64),
+                                       ("split", 4000)])
+def test_attention_nan_in_a_key_comes_out_and_stays_in_its_head(form, slot, dt, track):
+    """A NaN key makes its row's outputs of the heads that read it NaN, and their probabilities; nothing else."""
+    lengths = {"one": [256, 5], "cluster": [513, 5], "split": [4200, 300, 5] + [1000] * 40}[form]
+    pool, q, out, w0, weights, op = _attention_case(lengths, 4, 2, 16, 64, dt, seed=4, track=track)
+    pool.k[pool.table_np[0, slot // 16], 1, slot % 16, 3] = float("nan")
+    op()
+    op.check()
+    got = _host(out)
+    assert np.isnan(got[0, 4:]).all()
+    got[0, 4:] = 0
+    assert np.isfinite(got).all()
+    if track:
+        w = _host(weights)
+        assert np.isnan(w[0, 1, :lengths[0]]).all()
+        w[0, 1, :lengths[0]] = 0
+        assert np.isfinite(w).all()
+
+
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 def test_attention_keys_of_minus_infinity_get_no_weight(dt):
     """A key whose score is -inf (here alone in its first tiles) has probability 0; the row's sum stays finite."""
