@@ -76,6 +76,7 @@ class PagedLlama:
         self.slots = np.zeros(rows, np.int64)  # slots in use after the steps enqueued so far
         self.pos_host = 0                      # position of the rows' next token
         self._beam_tables = False              # the device has the only true table (beam search)
+        self._beam_slots = 0                   # slots that each beam has pages for
 
     # -- one step ---------------------------------------------------------------------------------------------
     def _weight(self, name: str) -> int:
@@ -157,6 +158,8 @@ class PagedLlama:
     def step(self) -> None:
         """Enqueues one step for the tokens in ``ids`` (a graph replay from the second one on)."""
         torch = self.torch
+        if self._beam_tables and (self.slots + 1 > self._beam_slots).any():  # (no page behind them)
+            raise ValueError(f"the search took pages for {self._beam_slots} slots a beam, and all are in use")
         if (self.slots + 1 > self.spec.slots).any() or int(self.pos_host) >= self.cfg.max_seq:
             raise ValueError(f"no room: {int(self.slots.max())} of {self.spec.slots} slots, position {self.pos_host} of "
                              f"{self.cfg.max_seq}")
@@ -257,6 +260,8 @@ class PagedLlama:
         """[rows, steps] tokens; ``keep_logits`` (a list) receives each step's [rows, vocab] logits."""
         torch = self.torch
         prompts = np.asarray(prompts, np.int32)
+        if steps < 1:
+            raise ValueError(f"steps must be positive, got {steps}")
         if prompts.shape != (self.rows, self.prog.prompt_len):
             raise ValueError(f"expected prompts of shape {(self.rows, self.prog.prompt_len)}, got {prompts.shape}")
         self._start(prompts)
@@ -281,6 +286,8 @@ class PagedLlama:
         if self.budget is not None:
             raise ValueError("beam search shares pages between beams: it takes a cache without a budget")
         torch, w, n = self.torch, self.rows, self.prog.prompt_len
+        if steps < 1:
+            raise ValueError(f"steps must be positive, got {steps}")
         if n + steps - 1 > self.spec.slots:
             raise ValueError(f"{n} + {steps - 1} slots, the table holds {self.spec.slots}")
         self._start([prompt])
@@ -290,6 +297,7 @@ class PagedLlama:
             c.share_prompt(n)
             c.upload()
             self._beam_tables = True  # from here on the table is the device's
+            self._beam_slots = n + steps - 1
             scores, next_scores = (torch.zeros(1, w, device=self.device) for _ in range(2))
             done, next_done, parents, tokens = (torch.zeros(1, w, dtype=torch.int32, device=self.device) for _ in range(4))
             table_out = torch.zeros_like(c.table)

@@ -228,3 +228,20 @@ def test_refusals():
         gen.greedy(np.zeros((1, 16), np.int32), 12)
     with pytest.raises(ValueError, match="one rank"):
         PagedLlama(type("R", (), {"prog": tiny_program(2), "hal": None})(), rows=1, max_slots=40)
+
+
+def test_a_step_behind_a_search_stays_within_its_pages():
+    """The pages that a search took are all that its beams have: a further step is refused, not written elsewhere."""
+    from runtime.paged import PagedLlama
+
+    gen = PagedLlama(_runner(tiny_hf_model()), rows=2, max_slots=40, page_size=8)
+    prompt = np.arange(16, dtype=np.int32)
+    with pytest.raises(ValueError, match="steps must be positive"):
+        gen.greedy(np.stack([prompt, prompt]), 0)
+    with pytest.raises(ValueError, match="steps must be positive"):
+        gen.beam_search(prompt, 0)
+    first = gen.beam_search(prompt, 9)  # 24 slots, the third page full
+    with pytest.raises(ValueError, match="all are in use"):
+        gen.step()
+    again = gen.beam_search(prompt, 9)
+    assert again.tokens.tolist() == first.tokens.tolist() and again.scores.tolist() == first.scores.tolist()
