@@ -18,9 +18,9 @@
 // 64-bit maxima is the bound, and only K threads can hold keys at or above it.
 //
 // Measured (the three kernels one after another): 4 beams of one prompt, 32000 bf16 logits, 32 layers' pages
-// 12.5 us, three launches' latency; 32 x 8 beams 82 us, of which the page copies, 354 MB, take 61 (5.8 TB/s); 8 x 16
-// beams of 131072 fp32 logits 58 us: the pass over the logits 19.5 us for 53 MB, bound by instructions (51 %
-// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 12, the copies 30.
+// 11.4 us, three launches' latency; 32 x 8 beams 84 us, of which the page copies, 354 MB, take 63 (5.6 TB/s); 8 x 16
+// beams of 131072 fp32 logits 56 us: the pass over the logits 19.5 us for 53 MB, bound by instructions (51 %
+// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 12, the copies 28.
 //
 // Reordering.  See pim_beam_reorder in pim_b200.h: the table entries of full pages follow
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
@@ -357,68 +357,71 @@ static_assert(kReorderThreads >= kMaxBeams, "a thread per beam");
 constexpr int kCopyPieces = 8 * kReorderThreads;
 
 __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(BeamReorderArgs a) {
-  __shared__ int sm_parent[kMaxBeams], sm_page[kMaxBeams], sm_first[kMaxBeams], sm_childless[kMaxBeams];
-  __shared__ int sm_bad, sm_take;
-  const int row = blockIdx.x, b = row / a.beams, j = row - b * a.beams, tid = threadIdx.x;
+  // A beam's parent and partly filled page; the pages that further children are copied from and to.
+  __shared__ int sm_parent[kMaxBeams], sm_page[kMaxBeams], sm_from[kMaxBeams], sm_to[kMaxBeams];
+  __shared__ unsigned sm_further[kReorderThreads / 32], sm_childless[kReorderThreads / 32];
+  const int row = blockIdx.x, b = row / a.beams, j = row - b * a.beams, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
   pdl_wait();
   // (the length and the parents come together; only the partly filled pages wait for them)
   const int n = a.lengths[b], ps = 1 << a.ps_log2;
   const int p = tid < a.beams ? a.parents[b * a.beams + tid] : 0;
   const int full = n >> a.ps_log2, fill = n & (ps - 1);
-  bool mine_bad = n < 0 || n > (int64_t)a.max_pages << a.ps_log2 || p < 0 || p >= a.beams;
-  if (tid == 0) sm_bad = 0, sm_take = 0;
-  __syncthreads();
-  if (tid < a.beams) {
-    sm_parent[tid] = p;
-    if (!mine_bad && fill) {
-      const int page = a.table[(int64_t)(b * a.beams + tid) * a.table_stride + full];
-      sm_page[tid] = page;
-      mine_bad = page < 0 || page >= a.num_pages;
-    }
-  }
-  if (mine_bad) sm_bad = 1;
-  __syncthreads();
-  const bool bad = sm_bad;
-  if (bad && tid == 0 && blockIdx.y == 0) raise_flag(a.err);
-  if (tid < a.beams && !bad) {
-    bool first = true, childless = true;
-    for (int i = 0; i < a.beams; ++i) {
-      if (i < tid && sm_parent[i] == sm_parent[tid]) first = false;
-      if (sm_parent[i] == tid) childless = false;
-    }
-    sm_first[tid] = first;
-    sm_childless[tid] = childless;
-  }
-  __syncthreads();
-  const int parent = bad ? j : sm_parent[j];
-  const bool copies = !bad && fill && !sm_first[j];
-  if (copies && tid < a.beams) {  // the i-th further child takes the page of the i-th beam without a child
-    int nth = 0, order = 0;
-    for (int i = 0; i < j; ++i) nth += !sm_first[i];
-    for (int i = 0; i < tid; ++i) order += sm_childless[i];
-    if (sm_childless[tid] && order == nth) sm_take = tid;
-  }
-  __syncthreads();
-  const int take = copies ? sm_take : parent;
-  if (blockIdx.y == 0) {
-    const int* mine = a.table + row * a.table_stride;
-    const int* theirs = a.table + (int64_t)(b * a.beams + parent) * a.table_stride;
-    for (int i = tid; i < a.max_pages; i += blockDim.x) {
-      int page = bad || i > full || (i == full && !fill) ? mine[i] : theirs[i];
-      if (!bad && fill && i == full) page = sm_page[take];
-      a.table_out[row * a.table_stride + i] = page;
-    }
-  }
-  if (!copies) return;
-  // 16-byte pieces of the slots in use, kCopyPieces of them per step of a CTA, four in flight per thread
+  const bool n_ok = n >= 0 && n <= (int64_t)a.max_pages << a.ps_log2;
+  // 16-byte pieces of the slots in use, kCopyPieces of them per step of a CTA
   const int per_head = fill * a.row_bytes / 16, head_pieces = a.row_bytes << a.ps_log2 >> 4;
   const int pieces = a.hkv * per_head, steps = (pieces + kCopyPieces - 1) / kCopyPieces;
-  for (int64_t item = blockIdx.y; item < (int64_t)a.num_blocks * steps; item += gridDim.y) {
-    const int blk = (int)(item / steps), i0 = (int)(item - (int64_t)blk * steps) * kCopyPieces + tid;
+  const int64_t per_copy = (int64_t)a.num_blocks * steps, cta = (int64_t)blockIdx.y * a.beams + j;
+  if (blockIdx.y > 0 && (!n_ok || cta >= (a.beams - 1) * per_copy)) return;  // (made for full pages)
+  int page = 0;
+  if (tid < a.beams) {
+    if (n_ok && fill) page = a.table[(int64_t)(b * a.beams + tid) * a.table_stride + full];
+    sm_parent[tid] = p;
+  }
+  bool bad = __syncthreads_or(!n_ok || p < 0 || p >= a.beams);
+  bool further = false, childless = tid < a.beams;
+  if (tid < a.beams)
+    for (int i = 0; i < a.beams; ++i) {
+      further |= i < tid && sm_parent[i] == p;
+      childless &= sm_parent[i] != tid;
+    }
+  const unsigned who = __ballot_sync(0xffffffffu, further), free = __ballot_sync(0xffffffffu, childless);
+  if (lane == 0) sm_further[warp] = who, sm_childless[warp] = free;
+  if (tid < a.beams) sm_page[tid] = page;
+  bad |= (bool)__syncthreads_or(page < 0 || page >= a.num_pages);
+  if (bad && tid == 0 && blockIdx.y == 0) raise_flag(a.err);
+  // the i-th further child takes the page of the i-th beam without a child (there are equally many)
+  auto before = [&](const unsigned* mask, int i) {
+    int count = __popc(mask[i / 32] & ((1u << i % 32) - 1));
+    for (int w = 0; w < i / 32; ++w) count += __popc(mask[w]);
+    return count;
+  };
+  if (!bad && further) sm_from[before(sm_further, tid)] = sm_page[p];
+  if (!bad && childless) sm_to[before(sm_childless, tid)] = page;
+  __syncthreads();
+  if (blockIdx.y == 0) {
+    const int parent = bad ? j : sm_parent[j];
+    const int* mine = a.table + row * a.table_stride;
+    const int* theirs = a.table + (int64_t)(b * a.beams + parent) * a.table_stride;
+    const bool copied = sm_further[j / 32] >> j % 32 & 1;
+    for (int i = tid; i < a.max_pages; i += blockDim.x) {
+      int at = bad || i > full || (i == full && !fill) ? mine[i] : theirs[i];
+      if (!bad && fill && i == full && copied) at = sm_to[before(sm_further, j)];
+      a.table_out[row * a.table_stride + i] = at;
+    }
+  }
+  if (bad || !fill) return;
+  int copies = 0;
+#pragma unroll
+  for (int w = 0; w < kReorderThreads / 32; ++w) copies += __popc(sm_further[w]);
+  // All CTAs of the batch entry share its copies, eight pieces a thread in flight; neighbours work on different copies
+  // (on one after the other 32 x 8 beams take 97 us with the selection instead of 83).
+  for (int64_t item = cta; item < copies * per_copy; item += (int64_t)gridDim.y * a.beams) {
+    const int rest = (int)(item / copies), c = (int)(item - (int64_t)rest * copies);
+    const int blk = rest / steps, i0 = (rest - blk * steps) * kCopyPieces + tid;
     char* block = a.pages + blk * a.block_bytes;
-    const int4* src = reinterpret_cast<const int4*>(block + sm_page[parent] * a.page_bytes);
-    int4* dst = reinterpret_cast<int4*>(block + sm_page[take] * a.page_bytes);
+    const int4* src = reinterpret_cast<const int4*>(block + sm_from[c] * a.page_bytes);
+    int4* dst = reinterpret_cast<int4*>(block + sm_to[c] * a.page_bytes);
     int4 v[kCopyPieces / kReorderThreads];
     int64_t off[kCopyPieces / kReorderThreads];
 #pragma unroll
@@ -560,10 +563,16 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   d.row_bytes = a->head_dim * es;
   d.err = a->err_flag;
   if (page * es / 16 > (1 << 30)) return bad("a page of more than 16 GiB");
-  // About a third of the rows copy: enough CTAs per row that those fill the GPU, and no more than there are steps.
+  // The copies follow from the parents and the lengths.  A CTA per step of those that half-filled pages and a third of the
+  // beams give, at least as many as run at once and at most a few rounds of them: a thousand CTAs cost 1.1 us to launch,
+  // with nothing to do too, and a step per CTA balances best (device us with the selection at 24, 48 and 96 CTAs an SM: 32 x 8
+  // beams with 354 MB to copy 92, 87, 83; 16 x 12 beams with eight slots in use 17.5, 21.1, 26.4; at a sixth of the full pages'
+  // steps 84 and 17.5).
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
   const int rows = a->batch * a->beams;
-  int64_t by = ceil_div(96 * 148, rows);
+  int64_t by = (steps + 5) / 6;
+  const int64_t least = ceil_div(24 * 148, rows), most = ceil_div(96 * 148, rows);
+  by = by < least ? least : by > most ? most : by;
   by = by < steps ? by : steps;
   return report_cuda(launch_pdl(beam_reorder_kernel, dim3(rows, (unsigned)by), dim3(kReorderThreads), 0,
                                 (cudaStream_t)stream, d),
