@@ -52,6 +52,7 @@ struct BeamSelectArgs {
   float* scores_out;
   int *parents, *tokens, *done_out;
   int batch, beams, k, vocab, eos, pad, splits;
+  int chunk;  // tokens of a split: a multiple of 8
   BeamStats* stats;           // [batch * beams][splits]
   unsigned long long* lists;  // [batch * beams][splits][k]
 };
@@ -100,15 +101,16 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   pdl_wait();
   if (a.done && a.done[row]) return;  // offers one candidate, which the merge adds
   const T* row_x = static_cast<const T*>(a.logits) + row * a.stride;
-  const int base = split * (kBeamThreads * kBeamVals);
+  const int base = split * a.chunk, size = min(a.chunk, a.vocab - base);
   float x[kBeamVals];  // -inf: no candidate
   // value i of this thread is token base + tok(i)
   auto tok = [&](int i) { return ALIGNED ? (i / V) * kBeamThreads * V + tid * V + i % V : i * kBeamThreads + tid; };
   if (ALIGNED) {
+    constexpr int kNone = V == 8 ? (int)0xff80ff80u : (int)0xff800000u;  // -inf: two bf16, or a float
     int4 raw[kBeamVals / V];
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i)
-      raw[i] = ld_once_if(reinterpret_cast<const int4*>(row_x + base + tok(i * V)), base + tok(i * V) < a.vocab);
+      raw[i] = ld_once_if(reinterpret_cast<const int4*>(row_x + base + tok(i * V)), tok(i * V) < size, kNone);
 #pragma unroll
     for (int i = 0; i < kBeamVals / V; ++i) {
       float f[V];
@@ -118,12 +120,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) x[i] = base + tok(i) < a.vocab ? to_f(row_x[base + tok(i)]) : -INFINITY;
-  }
-  if (ALIGNED && base + kBeamThreads * kBeamVals > a.vocab) {  // the last chunk
-#pragma unroll
-    for (int i = 0; i < kBeamVals; ++i)
-      if (base + tok(i) >= a.vocab) x[i] = -INFINITY;
+    for (int i = 0; i < kBeamVals; ++i) x[i] = tok(i) < size ? to_f(row_x[base + tok(i)]) : -INFINITY;
   }
   float mine_x = -INFINITY;
 #pragma unroll
@@ -459,6 +456,9 @@ static int beam_vals(const pim_beam_select_args* a) {
   return (int64_t)a->batch * a->beams * ceil_div(a->vocab, 2 * kBeamChunk) >= 2 * 148 ? 32 : 16;
 }
 static int beam_splits(const pim_beam_select_args* a) { return ceil_div(a->vocab, kBeamThreads * beam_vals(a)); }
+// The splits' chunks are as good as equal: in a short last one most warps would have nothing, which leaves no bound, and
+// every logit of it would be a candidate (256 rows of 26080 bf16 logits: see the figures at the head of the file).
+static int beam_chunk(const pim_beam_select_args* a) { return (ceil_div(a->vocab, beam_splits(a)) + 7) / 8 * 8; }
 
 static int64_t beam_stats_bytes(const pim_beam_select_args* a) {
   return (int64_t)a->batch * a->beams * beam_splits(a) * (int64_t)sizeof(BeamStats);
@@ -512,6 +512,7 @@ extern "C" int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, voi
   d.eos = a->eos;
   d.pad = a->pad;
   d.splits = beam_splits(a);
+  d.chunk = beam_chunk(a);
   d.stats = static_cast<BeamStats*>(workspace);
   d.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + beam_stats_bytes(a));
   cudaStream_t st = (cudaStream_t)stream;

@@ -70,10 +70,10 @@ __device__ __forceinline__ int4 ld_once(const int4* p) {
   return r;
 }
 
-// The same where `ok`, else zeros: one predicated instruction, so that several in a row are all
-// under way (a branch around a load makes the compiler wait for it where the paths join).
-__device__ __forceinline__ int4 ld_once_if(const int4* p, bool ok) {
-  int4 r = make_int4(0, 0, 0, 0);
+// The same where `ok`, else `fill` in every word: one predicated instruction, so that several in a row are
+// all under way (a branch around a load makes the compiler wait for it where the paths join).
+__device__ __forceinline__ int4 ld_once_if(const int4* p, bool ok, int fill = 0) {
+  int4 r = make_int4(fill, fill, fill, fill);
   asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
                " @q ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];\n}"
                : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
