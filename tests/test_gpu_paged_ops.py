@@ -589,6 +589,25 @@ def test_beam_select_logits_near_the_types_limits(vocab, dt):
     _check_select(logits[:, :1], torch.tensor([[-1.5]], device="cuda"), 5)
 
 
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [8200, 26080, 4100])
+def test_beam_select_of_rows_that_crowd_in_a_few_warps(vocab, dt):
+    """Ranges masked to nothing or to one value, sorted rows and vocabularies a little longer than a chunk."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = torch.randn(1, 7, vocab, device="cuda", generator=g).to(_tdt(dt))
+    logits[0, 0, 1500:] = -float("inf")
+    logits[0, 1, :-700] = -float("inf")
+    logits[0, 2, 900:] = torch.finfo(_tdt(dt)).min
+    logits[0, 3] = torch.arange(vocab, device="cuda") / 1000
+    logits[0, 4] = -torch.arange(vocab, device="cuda") / 1000
+    logits[0, 5] = torch.randint(0, 5, (vocab,), device="cuda", generator=g).to(logits.dtype)
+    scores = torch.tensor([[0.0, -0.5, 0.25, 1.0, 1.5, 3.0, 0.1]], device="cuda")
+    _check_select(logits, scores, 64)
+    for w in range(7):
+        _check_select(logits[:, w:w + 1], scores[:, w:w + 1].contiguous(), 13)
+
+
 def test_beam_select_strided_logits():
     torch = _torch()
     for dt in ("float32", "bfloat16"):
