@@ -476,6 +476,32 @@ def test_evict_rows_longer_than_shared_memory():
     _evict_case([52000, 48000], 1, 64, 32, "bfloat16", 40001, 0, 0, seed=8, ties=True, in_place=True)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lengths,heads,ps,budget,recent,sink", [
+    ([4096], 3, 64, 1000, 100, 4), ([9000, 5, 0, 6000], 1, 8, 2000, 0, 0), ([16500, 20, 9001], 2, 256, 90, 10, 2),
+    ([8193], 8, 32, 8000, 50, 0), ([8200, 8100] * 6, 1, 16, 2500, 40, 4), ([33000], 1, 128, 16384, 1, 1)])
+def test_evict_long_rows_of_few_units(lengths, heads, ps, budget, recent, sink, in_place):
+    """Several CTAs share a row's slots: short rows leave some of them none, and lists start where others end."""
+    for ties in (False, True):
+        _evict_case(lengths, heads, ps, 32, "bfloat16", budget, recent, sink, seed=11, ties=ties, in_place=in_place)
+    weights = np.zeros((len(lengths), heads, -(-max(lengths) // ps) * ps), np.float32)
+    _evict_case(lengths, heads, ps, 32, "bfloat16", budget, 0, 0, weights=weights, in_place=in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("over", [1, 2, 5, 8, 9, 40])
+def test_evict_a_few_tokens_of_long_rows(over, in_place):
+    budget = 8190
+    _evict_case([budget + over, budget, budget + 1, 17], 2, 64, 64, "bfloat16", budget, 20, 3, seed=over, in_place=in_place)
+    _evict_case([budget + over], 1, 64, 32, "float32", budget, 0, 0, seed=over, ties=True, in_place=in_place)
+
+
+def test_evict_long_rows_that_one_cta_takes():
+    """Too many units for clusters, and rows too long for the shared memory of one."""
+    _evict_case([50000] + [30] * 74, 1, 256, 32, "bfloat16", 300, 20, 4, seed=12)
+    _evict_case([400001], 1, 256, 32, "bfloat16", 250, 20, 4, seed=13, ties=True)
+
+
 def test_evict_reports_bad_lengths_and_pages():
     from backend.cuda_paged import PagedEvict
 
