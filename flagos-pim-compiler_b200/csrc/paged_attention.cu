@@ -735,7 +735,9 @@ __device__ __forceinline__ Holders holders(int64_t start, int tiles, int64_t tot
 template <typename T, int HD, int NH>
 __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnArgs a, int join_ctas, int key_chunks) {
   constexpr int WARPS = kFinishThreads / 32;
-  __shared__ float sm_m[WARPS], sm_l[WARPS], sm_acc[WARPS][HD];
+  constexpr int G = HD / 4, PARTS = kFinishThreads / G;  // lanes of a part (16 bytes each), parts at a time
+  __shared__ float sm_m[WARPS], sm_l[WARPS];
+  __shared__ alignas(16) float sm_acc[PARTS][HD];
   __shared__ float sm_stat[32][2];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
@@ -771,36 +773,59 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
     const Holders p = holders_of(head);
     if (p.first == p.last) return;  // written by its one CTA
     const int hl = head % a.group % NH;
-    constexpr int DPL = HD / 32;
-    float m = -INFINITY, l = 0.f, acc[DPL];
-#pragma unroll
-    for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
-    for (int c = p.first + warp; c <= p.last; c += WARPS) {
-      const int64_t s = slot_of(p, c) + hl;
-      const float pm = a.part_stat[s * 2], pl = a.part_stat[s * 2 + 1];
-      const float mn = fmaxf(m, pm);
-      const float safe = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2f(m - safe), pf = exp2f(pm - safe);
-      l = l * f + pl * pf;
-#pragma unroll
-      for (int e = 0; e < DPL; ++e) acc[e] = acc[e] * f + a.part_acc[s * HD + lane + 32 * e] * pf;
+    const int pg = tid / G, d4 = 4 * (tid % G);
+    float m = -INFINITY, l = 0.f;
+    for (int c = p.first + tid; c <= p.last; c += kFinishThreads) {
+      const float2 st = *reinterpret_cast<const float2*>(a.part_stat + (slot_of(p, c) + hl) * 2);
+      const float mn = fmaxf(m, st.x), safe = mn == -INFINITY ? 0.f : mn;
+      l = l * exp2f(m - safe) + st.y * exp2f(st.x - safe);
       m = mn;
     }
-    if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float safe = 0.f;
+    // The loads of FLY parts a thread are under way together: a unit of few and long rows lies in every CTA.
+    auto add = [&](auto fly) {
+      constexpr int kFly = decltype(fly)::value;
+      for (int c0 = p.first + pg, round = 0; round * kFly * PARTS <= p.last - p.first; ++round, c0 += kFly * PARTS) {
+        int4 v[kFly];
+        float f[kFly];
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) sm_acc[warp][lane + 32 * e] = acc[e];
+        for (int u = 0; u < kFly; ++u) {
+          const int c = c0 + u * PARTS;
+          const int64_t at = slot_of(p, c) + hl;
+          v[u] = ld_once_if(reinterpret_cast<const int4*>(a.part_acc + at * HD + d4), c <= p.last);
+          f[u] = __uint_as_float(ld4_if(a.part_stat + at * 2, c <= p.last));
+        }
+        if (round == 0) {  // the unit's maximum and sum, beside the first loads
+          const float M = warp_max(m), here = M == -INFINITY ? 0.f : M;
+          l = warp_sum(l * exp2f(m - here));
+          if (lane == 0) sm_m[warp] = M, sm_l[warp] = l;
+          __syncthreads();
+          float top = sm_m[0];
+#pragma unroll
+          for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w]);
+          safe = top == -INFINITY ? 0.f : top;
+        }
+#pragma unroll
+        for (int u = 0; u < kFly; ++u) {
+          const float g = c0 + u * PARTS <= p.last ? exp2f(f[u] - safe) : 0.f;
+          acc.x += __int_as_float(v[u].x) * g;
+          acc.y += __int_as_float(v[u].y) * g;
+          acc.z += __int_as_float(v[u].z) * g;
+          acc.w += __int_as_float(v[u].w) * g;
+        }
+      }
+    };
+    if (p.last - p.first < PARTS) add(std::integral_constant<int, 1>());
+    else add(std::integral_constant<int, 8>());
+    *reinterpret_cast<float4*>(&sm_acc[pg][d4]) = acc;
     __syncthreads();
     for (int d = tid; d < HD; d += kFinishThreads) {
-      float M = -INFINITY, L = 0.f, A = 0.f;
+      float L = 0.f, A = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w]);
-      const float safe = M == -INFINITY ? 0.f : M;
+      for (int w = 0; w < WARPS; ++w) L += sm_l[w] * exp2f(sm_m[w] - safe);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = exp2f(sm_m[w] - safe);
-        L += sm_l[w] * f;
-        A += sm_acc[w][d] * f;
-      }
+      for (int w = 0; w < PARTS; ++w) A += sm_acc[w][d];
       static_cast<T*>(a.out)[row * a.out_stride + (int64_t)head * HD + d] = from_f<T>(quotient(A, L));
     }
     return;
@@ -833,11 +858,21 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(PagedAttnA
         l = a.row_stat[((int64_t)row * a.hq + h) * 2 + 1];
       } else {
         const int hl = h % a.group % NH;
-        for (int c = p.first + lane; c <= p.last; c += 32) {
-          const float2 st = *reinterpret_cast<const float2*>(a.part_stat + (slot_of(p, c) + hl) * 2);
-          const float mn = fmaxf(m, st.x), safe = mn == -INFINITY ? 0.f : mn;
-          l = l * exp2f(m - safe) + st.y * exp2f(st.x - safe);
-          m = mn;
+        for (int c0 = p.first + lane; c0 <= p.last; c0 += 32 * 4) {
+          float x[4], y[4];  // (four parts under way)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float* st = a.part_stat + (slot_of(p, c0 + 32 * u) + hl) * 2;
+            x[u] = __uint_as_float(ld4_if(st, c0 + 32 * u <= p.last));
+            y[u] = __uint_as_float(ld4_if(st + 1, c0 + 32 * u <= p.last));
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (c0 + 32 * u > p.last) break;
+            const float mn = fmaxf(m, x[u]), safe = mn == -INFINITY ? 0.f : mn;
+            l = l * exp2f(m - safe) + y[u] * exp2f(x[u] - safe);
+            m = mn;
+          }
         }
         const float M = warp_max(m), safe = M == -INFINITY ? 0.f : M;
         l = warp_sum(l * exp2f(m - safe));
@@ -917,6 +952,7 @@ static cudaError_t launch_paged(const PagedAttnArgs& a, cudaStream_t st) {
   }
   if (a.whole_warps == 4) return launch_whole<Core, HD, NH, 4>(a, st);
   if (a.whole_warps == 2) return launch_whole<Core, HD, NH, 2>(a, st);
+  if (a.whole_warps == 1) return launch_whole<Core, HD, NH, 1>(a, st);
   cudaError_t e = launch_pdl(paged_attn_kernel<Core, HD, NH>, dim3(a.ctas), dim3(kSplitWarps * 32), 0, st, a);
   if (e != cudaSuccess) return e;
   const int join = a.kv.rows * a.hq;
@@ -983,10 +1019,15 @@ static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
   //   fp32 1 row x 4 heads   clusters of 8  5.6  5.9  6.4  8.0 11.3                             split   -   -  7.2  7.9  9.7
   // More units than SMs twice over: fewer warps a CTA, bf16 2 up to 256 slots (128 rows x 8 heads x 8: 22.6, 35.6, 60.8 us
   // at 128, 256, 512 against 38.6, 46.7, 61.7 split), fp32 4 up to 512 (64 x 8 x 4: 8.6, 16.6, 30.5, 56.7 at 128 .. 1024
-  // against 17.3, 24.7, 34.7, 55.8).  A query group of several tiles would add to the same weights from several CTAs: it is
+  // against 17.3, 24.7, 34.7, 55.8).  More than the GPU holds at once: fewer still, as a warp has all the keys of 16 or 32 slots
+  // and a CTA's warps wait for one another: bf16 1 up to 128 slots (123 rows x 32 heads of 10, 62, 126, 250 keys 14.8, 39.8,
+  // 69.6, 127 us, with 2 23.0, 44.0, 70.5, 122; 40 x 16 of 10 4.6 and 6.4, 64 x 8 5.9 and 4.7), fp32 2 (128 x 8 x 4 of 10, 62,
+  // 250 5.1, 9.8, 30.8, with 4 6.8, 10.9, 32.2), and 1 for many short ones (123 x 32 of 10, 62, 126 11.7, 33.0, 58.7, with 2
+  // 18.5, 34.9, 57.6; 128 x 8 x 4 of 10 6.9 and 5.1).  A query group of several tiles would add to the same weights from several CTAs: it is
   // split.
   const bool bf16 = dtype == PIM_BF16, many = units > 2 * 148;
-  p.whole_warps = many ? (bf16 ? 2 : 4) : p.nh > 8 ? 4 : 8;
+  p.whole_warps = !many ? (p.nh > 8 ? 4 : 8) : !bf16 && units <= 4 * 148 ? 4 : 2;
+  if (bf16 ? units > 4 * 148 && slots <= 128 : units > 16 * 148 && slots <= 64) p.whole_warps = 1;
   p.cluster = 1;
   if (slots > 256)
     while (p.cluster < kMaxCluster && units * p.cluster * 2 * p.whole_warps <= 8 * 148) p.cluster *= 2;

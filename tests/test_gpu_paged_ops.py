@@ -149,6 +149,43 @@ def test_attention_many_rows_and_heads(dt):
     _check_attention(pool, q, out, w0, weights, dt)
 
 
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,heads,group,most,hd", [(80, 32, 1, 17, 64), (90, 8, 4, 129, 32), (40, 16, 12, 60, 128),
+                                                      (90, 27, 2, 65, 128)])
+def test_attention_of_many_short_rows(rows, heads, group, most, hd, dt, track):
+    """Units by the thousand, of a warp or two each; 12 heads a group make a second, partly filled tile in fp32."""
+    lengths = list(np.random.default_rng(rows).integers(0, most, rows))
+    pool, q, out, w0, weights, op = _attention_case(lengths, group, heads, 8, hd, dt, seed=6, track=track)
+    op()
+    _check_attention(pool, q, out, w0, weights, dt)
+    op.check()
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_attention_of_one_long_row_lies_in_every_cta(dt):
+    """A unit in some hundred parts, with and without weights, and keys of -inf that leave whole parts empty."""
+    for track in (False, True):
+        pool, q, out, w0, weights, op = _attention_case([30011], 3, 1, 16, 64, dt, seed=14, track=track)
+        op()
+        _check_attention(pool, q, out, w0, weights, dt)
+    for page in pool.table_np[0, :1200]:
+        pool.k[page, 0, :, 0] = -float("inf")
+    q[:] = 0
+    q[:, :, 0] = 1
+    weights.zero_()
+    op()
+    v = ref.slots(_host(pool.v), pool.table_np[0], 30011)[0][19200:].astype(np.float64)
+    s = ref.slots(_host(pool.k), pool.table_np[0], 30011)[0][19200:, 0].astype(np.float64) / 8
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    want = p @ v
+    # as in ref.attention: the scores' roundings, the exponentials', and those of two sums of as many terms
+    rel = 2 * (64 + 2) * 2.0**-23 * np.abs(s).max() + EXP[dt] + 2 * len(p) * 2.0**-23
+    assert (np.abs(_host(out)[0] - want) <= HALF[dt] * np.abs(want) + rel * (p @ np.abs(v)) + 1e-30).all()
+    assert (_host(weights)[0, 0, :19200] == 0).all()
+
+
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 def test_attention_scale_and_sharp_scores(dt):
     """Scores of tens: all the weight on few keys, and a running maximum that grows along the row."""
