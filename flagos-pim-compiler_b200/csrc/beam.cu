@@ -20,7 +20,7 @@
 // Measured (the three kernels one after another): 4 beams of one prompt, 32000 bf16 logits, 32 layers' pages
 // 11.4 us, three launches' latency; 32 x 8 beams 84 us, of which the page copies, 354 MB, take 63 (5.6 TB/s); 8 x 16
 // beams of 131072 fp32 logits 56 us: the pass over the logits 19.5 us for 53 MB, bound by instructions (51 %
-// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 12, the copies 28.
+// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 10, the copies 28.
 //
 // Reordering.  See pim_beam_reorder in pim_b200.h: the table entries of full pages follow
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
