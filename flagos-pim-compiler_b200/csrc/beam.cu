@@ -574,6 +574,7 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   // beams with 354 MB to copy 92, 87, 83; 16 x 12 beams with eight slots in use 17.5, 21.1, 26.4; at a sixth of the full pages'
   // steps 84 and 17.5).
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
+  if (steps > INT32_MAX) return bad("more than 2^31 steps of 8 KiB to copy a page of every block");
   const int rows = a->batch * a->beams;
   int64_t by = (steps + 5) / 6;
   const int64_t least = ceil_div(24 * 148, rows), most = ceil_div(96 * 148, rows);
