@@ -31,12 +31,15 @@
 // t) for K, which are two k-steps of its B fragment, and the query the same; for V it takes 16
 // bytes at dim 8 g of keys 2t, 2t+1, 2t+8, 2t+9 and pairs two keys' elements with one byte
 // permutation each.  Nothing goes through shared memory, every load is 16 bytes and
-// 64 (K) or 128 (V) contiguous bytes a row.  The next tile's K loads start as soon as this
-// one's scores are formed, its V loads after this one's products.  P enters the second
-// product as two bf16 parts (p = hi + lo, 16 bits of it, so its rounding does not show
-// in the result); with at most 8 heads in a tile the rows 8..15 of the MMA, otherwise idle,
-// carry lo.  tcgen05 would add staging in shared memory and TMEM for a product of 8 rows that
-// the memory system bounds.
+// 64 (K) or 128 (V) contiguous bytes a row.  The scores come out as (heads) x (keys), which is the
+// layout that the second product's B fragment needs, so that one is taken as V^T P^T: 16 dims
+// by 8 heads a tile.  P enters as three bf16 parts, each what is left of a probability rounded
+// towards zero: 3 x 8 bits are all 24 of a float, and a probability is not rounded at all.  (Two
+// parts: sums of p v that cancel are off by 2^-18 of their terms; 650 us for the 64 rows above
+// against 661, 117.0 for the ragged ones against 117.5.)  The next tile's K loads start as soon as this
+// one's scores are formed, its V loads once this one's V is paired, before the products that read
+// the pairs (688 us behind them).  tcgen05 would add staging in shared memory and TMEM for a product
+// of 8 rows that the memory system bounds.
 //
 // fp32: a key's dims are spread over head_dim / 4 lanes; the partial dot products of several
 // keys and heads are summed by one butterfly that leaves one score per lane.
@@ -112,13 +115,14 @@ struct MmaCore {
   static constexpr int KC = HD / 32;     // 16-byte pieces of a K row per lane
   static constexpr int VE = HD >= 64 ? 8 : HD / 8;  // dims of a V load
   static constexpr int VC = HD / (8 * VE);          // V loads of a row per lane
-  static constexpr int NT = VC * VE;     // n-tiles of the output
+  static constexpr int NT = VC * VE / 2; // m-tiles of the output: 16 dims each
   static constexpr int HI = NH / 8;      // head rows of a lane: g (and g + 8)
   static constexpr int kParts = 1;       // states of a warp
+  static constexpr int kPParts = 3;      // bf16 parts of a probability: 3 x 8 bits, all of a float
   uint4 q[HI][KC];
   uint4 kr[2][KC];
   uint32_t vr[4][VC][VE / 2];
-  float acc[NT][4];
+  float acc[HI][NT][4];
   float m[HI], l[HI];
   int64_t at[2], at_next[2];
   int lim[2], lim_next[2];
@@ -140,9 +144,11 @@ struct MmaCore {
       l[i] = 0.f;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int h = 0; h < HI; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[h][n][e] = 0.f;
   }
 
   // Page ids of the 16 keys at key0 (two halves of 8, which never straddle a page).
@@ -204,23 +210,22 @@ struct MmaCore {
 
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
-  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
+  // A float's upper 16 bits, as a float and of two floats side by side: what bf16 holds of them, rounded towards zero.
+  static __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+  static __device__ __forceinline__ uint32_t tops(float lo, float hi) {
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
   }
-  static __device__ __forceinline__ float low(uint32_t p) { return __uint_as_float(p << 16); }
-  static __device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-  // The step's keys key0 .. key0 + 15; the caller loads the next step's K and V in between.
+  // The step's keys key0 .. key0 + 15; next_k() and next_v() load the next step's once the registers are free.
   // `scores`: where the unit's first head has its scores, or nullptr.
-  template <typename NextK>
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k) {
+  template <typename NextK, typename NextV>
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k,
+                                       NextV&& next_v) {
     float s[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -234,28 +239,28 @@ struct MmaCore {
       }
     }
     next_k();
-    uint32_t hi[2][HI], lo[2][HI];
+    uint32_t part[kPParts][2][HI];
     float alpha[HI];
     bool grew = false;
 #pragma unroll
     for (int h = 0; h < HI; ++h) {
-      float top = -INFINITY;
+      float best = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& x = s[i][2 * h + e];
           x = 2 * t + e < lim[i] ? x * a.scale_log2 : -INFINITY;
-          top = fmaxf(top, x);
+          best = fmaxf(best, x);
         }
       if (scores && g + 8 * h < nh) {
         float* sp = scores + (g + 8 * h) * a.score_stride + key0 + 2 * t;
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(sp + 8 * i) = make_float2(s[i][2 * h], s[i][2 * h + 1]);
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(m[h], top);
+      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+      const float mn = fmaxf(m[h], best);
       const float safe = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is 0, not NaN
       grew |= mn > m[h];
       alpha[h] = exp2_fast(m[h] - safe);
@@ -265,33 +270,41 @@ struct MmaCore {
       for (int i = 0; i < 2; ++i) {
         const float p0 = exp2_fast(s[i][2 * h] - safe), p1 = exp2_fast(s[i][2 * h + 1] - safe);
         sum += p0 + p1;
-        hi[i][h] = pack2(p0, p1);
-        lo[i][h] = pack2(p0 - low(hi[i][h]), p1 - high(hi[i][h]));
+        float r0 = p0, r1 = p1;
+#pragma unroll
+        for (int x = 0; x < kPParts; ++x) {
+          part[x][i][h] = tops(r0, r1);
+          r0 -= top(r0);
+          r1 -= top(r1);
+        }
       }
       l[h] = l[h] * alpha[h] + sum;
     }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < HI; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] *= alpha[e / 2 < HI ? e / 2 : 0];
+        for (int e = 0; e < 2; ++e) {  // (column 2t + e is head 2t + e of the eight, whose lanes are 4 (2t + e) ..)
+          const float f = __shfl_sync(0xffffffffu, alpha[h], 8 * t + 4 * e);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[h][n][e] *= f, acc[h][n][2 + e] *= f;
+        }
     }
+    uint32_t v[NT][4];
 #pragma unroll
     for (int c = 0; c < VC; ++c)
 #pragma unroll
       for (int w = 0; w < VE / 2; ++w)
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const uint32_t b0 = __byte_perm(vr[0][c][w], vr[1][c][w], o ? 0x7632 : 0x5410);
-          const uint32_t b1 = __byte_perm(vr[2][c][w], vr[3][c][w], o ? 0x7632 : 0x5410);
-          float(&d)[4] = acc[c * VE + 2 * w + o];
-          if (HI == 1) {
-            mma(d, hi[0][0], lo[0][0], hi[1][0], lo[1][0], b0, b1);
-          } else {
-            mma(d, hi[0][0], hi[0][HI - 1], hi[1][0], hi[1][HI - 1], b0, b1);
-            mma(d, lo[0][0], lo[0][HI - 1], lo[1][0], lo[1][HI - 1], b0, b1);
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          v[c * VE / 2 + w][i] = __byte_perm(vr[i / 2 * 2][c][w], vr[i / 2 * 2 + 1][c][w], i % 2 ? 0x7632 : 0x5410);
+    next_v();
+#pragma unroll
+    for (int x = 0; x < kPParts; ++x)
+#pragma unroll
+      for (int h = 0; h < HI; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma(acc[h][n], v[n][0], v[n][1], v[n][2], v[n][3], part[x][0][h], part[x][1][h]);
   }
 
   // The state of part `warp` into shared memory: [parts][NH] max and sum, [parts][NH][HD] output.
@@ -300,23 +313,18 @@ struct MmaCore {
     for (int h = 0; h < HI; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int at = warp * NH + g + 8 * h;
-      if (t == 0) sm_m[at] = m[h], sm_l[at] = l[h];
-      // column n of n-tile (c, j) is dim 8 VE c + VE n + j; this lane has columns 2t and 2t + 1
+      const int at = warp * NH + 8 * h;
+      if (t == 0) sm_m[at + g] = m[h], sm_l[at + g] = l[h];
+      // rows g and g + 8 of m-tile (c, w) are dims 8 VE c + VE g + 2 w and the next; this lane has heads 2t and 2t + 1
 #pragma unroll
       for (int c = 0; c < VC; ++c)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int j = 0; j < VE; j += 4) {
-            float4 x;
-            float* xs = &x.x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float(&d)[4] = acc[c * VE + j + i];
-              xs[i] = HI == 1 ? d[e] + d[2 + e] : d[2 * h + e];
-            }
-            *reinterpret_cast<float4*>(sm_acc + at * HD + 8 * VE * c + (2 * t + e) * VE + j) = x;
+          for (int w = 0; w < VE / 2; w += 2) {
+            const float(&x)[4] = acc[h][c * VE / 2 + w], (&y)[4] = acc[h][c * VE / 2 + w + 1];
+            *reinterpret_cast<float4*>(sm_acc + (at + 2 * t + e) * HD + 8 * VE * c + VE * g + 2 * w) =
+                make_float4(x[e], x[2 + e], y[e], y[2 + e]);
           }
     }
   }
@@ -396,8 +404,9 @@ struct FmaCore {
 #pragma unroll
     for (int u = 0; u < NK; ++u) at[u] = at_next[u];
   }
-  template <typename NextK>
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k) {
+  template <typename NextK, typename NextV>
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, float* scores, int nh, int key0, NextK&& next_k,
+                                       NextV&& next_v) {
     bool mine_ok = false;
 #pragma unroll
     for (int u = 0; u < NK; ++u) mine_ok |= at[u] >= 0 && u == key_of;
@@ -456,6 +465,7 @@ struct FmaCore {
         acc[h].z = fmaf(f, v[u].z, acc[h].z);
         acc[h].w = fmaf(f, v[u].w, acc[h].w);
       }
+    next_v();
   }
   __device__ __forceinline__ void store(float* sm_m, float* sm_l, float* sm_acc, int warp) {
 #pragma unroll
@@ -468,7 +478,7 @@ struct FmaCore {
 };
 
 // One warp's keys of [begin, end) (begin a multiple of 64), the CTA's WARPS warps taking turns: page ids two steps
-// ahead, the next step's K loads once this one's scores are formed, its V loads after this one's products.
+// ahead, the next step's K loads once this one's scores are formed, its V loads once this one's V was taken up.
 template <int WARPS, typename Core>
 __device__ __forceinline__ void walk(Core& core, const PagedAttnArgs& a, const int* trow, float* scores, int kvh, int nh,
                                      int begin, int end) {
@@ -482,13 +492,17 @@ __device__ __forceinline__ void walk(Core& core, const PagedAttnArgs& a, const i
   core.load_v(a);
   core.fetch_pages(a, trow, key0 + STRIDE, end);
   for (; key0 < end; key0 += STRIDE) {
-    core.step(a, scores, nh, key0, [&] {
-      core.place(a, kvh, key0 + STRIDE, end);
-      core.fetch_pages(a, trow, key0 + 2 * STRIDE, end);
-      core.load_k(a);
-    });
-    core.advance();
-    core.load_v(a);
+    core.step(
+        a, scores, nh, key0,
+        [&] {
+          core.place(a, kvh, key0 + STRIDE, end);
+          core.fetch_pages(a, trow, key0 + 2 * STRIDE, end);
+          core.load_k(a);
+        },
+        [&] {
+          core.advance();
+          core.load_v(a);
+        });
   }
 }
 

@@ -218,6 +218,42 @@ def test_attention_nan_in_a_key_comes_out_and_stays_in_its_head(form, slot, dt, 
 
 
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("group", [1, 5, 12])
+@pytest.mark.parametrize("form", ["one", "cluster", "split"])
+def test_attention_probabilities_keep_32_bits_where_their_products_cancel(form, group, dt):
+    """Three keys of probabilities 1 : p : 2^-10 whose values are such that the sum of p v all but vanishes, so that what is
+    left of a probability's rounding shows.  Scores are exact: q is one-hot, keys are short binary fractions and the scale
+    is log 2, so a score is a power of two's exponent.  Off by at most, before the last rounding: 2^-22 of p v = 1 (the
+    exponential; 2^-24 for the scale's rounding) and six steps of 2^-23 of sums whose terms are 1."""
+    torch = _torch()
+    heads, hd, rows = 2, 128, 9
+    scale = float(np.float32(np.log(2)))
+    lengths = [3] * rows + {"one": [200], "cluster": [513], "split": [4200]}[form]
+    pool, q, out, w0, weights, op = _attention_case(lengths, group, heads, 16, hd, dt, seed=21, scale=scale)
+    rng = np.random.default_rng(group)
+    q.zero_()
+    q[:, :, 0] = 1
+    bf16 = lambda x: torch.tensor(x).to(torch.bfloat16).double().numpy()  # noqa: E731
+    for b in range(rows):
+        page = int(pool.table_np[b, 0])
+        a = rng.integers(1, 256, heads) / 256.0
+        p2, p3 = np.exp(-scale * a)[:, None], np.exp(-scale * 10)
+        v2 = bf16(bf16(1 / p2) + (np.arange(hd) % 4 - 2) * 2.0**-7)
+        v3 = bf16((1 - p2 * v2) / p3)
+        for j, (key, value) in enumerate(((0 * a, -np.ones((heads, hd))), (-a, v2), (-10 + 0 * a, v3))):
+            pool.k[page, :, j] = 0
+            pool.k[page, :, j, 0] = torch.tensor(key, device="cuda").to(pool.k.dtype)
+            pool.v[page, :, j] = torch.tensor(value, device="cuda").to(pool.v.dtype)
+    op()
+    want = ref.attention(_host(q), _host(pool.k), _host(pool.v), pool.table_np, lengths, scale)
+    for b in range(rows):
+        o, p = want[b][:2]
+        one = p.max(1, keepdims=True)  # what a probability of 1 became by the division
+        off = np.abs(_host(out)[b] - o) / one
+        assert (off <= HALF[dt] * np.abs(o) / one + 2.0**-22 + 2.0**-24 + 6 * 2.0**-23).all(), (b, float(off.max() * 2.0**20))
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 def test_attention_keys_of_minus_infinity_get_no_weight(dt):
     """A key whose score is -inf (here alone in its first tiles) has probability 0; the row's sum stays finite."""
     torch = _torch()
