@@ -34,7 +34,7 @@
 // 64 (K) or 128 (V) contiguous bytes a row.  The scores come out as (heads) x (keys), which is the
 // layout that the second product's B fragment needs, so that one is taken as V^T P^T: 16 dims
 // by 8 heads a tile.  P enters as three bf16 parts, each what is left of a probability rounded
-// towards zero: 3 x 8 bits are all 24 of a float, and a probability is not rounded at all.  (Two
+// towards zero: 3 x 8 bits are all 24 of a float.  (Two
 // parts: sums of p v that cancel are off by 2^-18 of their terms; 650 us for the 64 rows above
 // against 661, 117.0 for the ragged ones against 117.5.)  The next tile's K loads start as soon as this
 // one's scores are formed, its V loads once this one's V is paired, before the products that read
@@ -274,8 +274,9 @@ struct MmaCore {
 #pragma unroll
         for (int x = 0; x < kPParts; ++x) {
           part[x][i][h] = tops(r0, r1);
-          r0 -= top(r0);
-          r1 -= top(r1);
+          // (at least 2^-30 of p, so that no part of a positive p is 0: an infinite V times 0 would be NaN, not infinite)
+          r0 = fmaxf(r0 - top(r0), p0 * 0x1p-30f);
+          r1 = fmaxf(r1 - top(r1), p1 * 0x1p-30f);
         }
       }
       l[h] = l[h] * alpha[h] + sum;

@@ -254,6 +254,34 @@ def test_attention_probabilities_keep_32_bits_where_their_products_cancel(form, 
 
 
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("group", [1, 6, 12])
+@pytest.mark.parametrize("form", ["one", "cluster", "split"])
+def test_attention_infinite_values_come_out_as_the_sum_has_them(form, group, dt):
+    """An infinite V element that is attended to makes its dim infinite, of both signs NaN; whatever the probability is (here
+    also 1 before the division, and powers of two, which short formats hold exactly).  The other dims stay as they are."""
+    torch = _torch()
+    inf = float("inf")
+    lengths = [40, {"one": 200, "cluster": 513, "split": 4200}[form], 9]
+    pool, q, out, w0, weights, op = _attention_case(lengths, group, 2, 16, 64, dt, seed=23, scale=float(np.float32(np.log(2))))
+    q.zero_()
+    q[:, :, 0] = 1
+    pool.k[..., 0] = torch.round(pool.k[..., 0] * 2)  # scores are whole powers of two
+    n = lengths[1]
+    for row, slot, dim, x in ((0, 3, 5, inf), (0, 39, 6, -inf), (1, n - 1, 7, inf), (1, 0, 7, -inf), (1, n // 2, 8, -inf),
+                              (2, 0, 9, inf), (2, 8, 9, inf), (2, 4, 10, float("nan"))):
+        pool.v[pool.table_np[row, slot // 16], :, slot % 16, dim] = x
+    op()
+    op.check()
+    got = _host(out)
+    with np.errstate(invalid="ignore"):
+        want = ref.attention(_host(q), _host(pool.k), _host(pool.v), pool.table_np, lengths, np.float32(np.log(2)), EXP[dt])
+    for b, (o, _, bound, _) in enumerate(want):
+        fine = np.isfinite(o)
+        assert (~fine).any() and np.array_equal(got[b][~fine], o[~fine], equal_nan=True), b
+        assert (np.abs(got[b][fine] - o[fine]) <= HALF[dt] * np.abs(o[fine]) + bound[fine]).all(), b
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 def test_attention_keys_of_minus_infinity_get_no_weight(dt):
     """A key whose score is -inf (here alone in its first tiles) has probability 0; the row's sum stays finite."""
     torch = _torch()
