@@ -53,11 +53,12 @@ class PagedKVSpec:
 
 
 class PageAllocator:
-    """Free pages of a pool; taken lowest first, so a run is reproducible."""
+    """Free pages of a pool; taken lowest first, so a run is reproducible.  A page may have several holders (``share``) and
+    is free again when the last one gave it back."""
 
     def __init__(self, num_pages: int) -> None:
         self._free = list(range(num_pages - 1, -1, -1))
-        self._taken: set[int] = set()
+        self._holders: dict[int, int] = {}
 
     @property
     def free(self) -> int:
@@ -67,15 +68,30 @@ class PageAllocator:
         if count > len(self._free):
             raise MemoryError(f"{count} pages wanted, {len(self._free)} free")
         got = [self._free.pop() for _ in range(count)]
-        self._taken.update(got)
+        self._holders.update((p, 1) for p in got)
         return got
 
-    def give(self, pages) -> None:
+    def holders(self, page: int) -> int:
+        return self._holders.get(page, 0)
+
+    def share(self, pages) -> None:
+        """One holder more for each page."""
         for p in pages:
-            if p not in self._taken:
+            if p not in self._holders:
                 raise ValueError(f"page {p} is not taken")
-            self._taken.remove(p)
-        self._free = sorted(self._free + list(pages), reverse=True)
+        for p in pages:
+            self._holders[p] += 1
+
+    def give(self, pages) -> None:
+        freed = []
+        for p in pages:
+            if p not in self._holders:
+                raise ValueError(f"page {p} is not taken")
+            self._holders[p] -= 1
+            if not self._holders[p]:
+                del self._holders[p]
+                freed.append(p)
+        self._free = sorted(self._free + freed, reverse=True)
 
 
 class PagedKVCache:
@@ -100,7 +116,7 @@ class PagedKVCache:
             self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
             self.slot_positions = torch.zeros(shape, dtype=torch.int32, device=device)
         self.allocator = PageAllocator(spec.num_pages)
-        self.held: list[list[int]] = [[] for _ in range(spec.rows)]  # pages that each row took
+        self.held: list[list[int]] = [[] for _ in range(spec.rows)]  # each row's pages, in the order of its table
         self._host_table = np.zeros((spec.rows, spec.max_pages), np.int32)
 
     def k(self, layer: int):
@@ -136,17 +152,27 @@ class PagedKVCache:
         self.held[row] = []
 
     def trim(self, slots) -> None:
-        """Gives back the pages behind ``slots[row]`` slots of every row."""
+        """Gives back the pages behind ``slots[row]`` slots of every row.  A row cannot end inside a page that other rows
+        hold too: its next token would be written there."""
+        ps = self.spec.page_size
         for row, n in enumerate(slots):
-            keep = -(-int(n) // self.spec.page_size)
+            if n % ps and n // ps < len(self.held[row]) and self.allocator.holders(self.held[row][n // ps]) > 1:
+                raise ValueError(f"row {row}: slot {n} lies in a page that other rows hold")
+        for row, n in enumerate(slots):
+            keep = -(-int(n) // ps)
             if len(self.held[row]) > keep:
                 self.allocator.give(self.held[row][keep:])
                 self.held[row] = self.held[row][:keep]
 
     def share_prompt(self, slots: int) -> None:
-        """Every row's first full pages become row 0's (of ``slots`` slots that row 0 has); its own are given back."""
+        """Every row's first full pages become row 0's (of ``slots`` slots that row 0 has); what the rows had in their place
+        is given back.  Rows need not have any pages yet: a ``reserve`` behind it takes their tails."""
         full = slots // self.spec.page_size
+        if full > len(self.held[0]):
+            raise ValueError(f"{slots} slots fill {full} pages, row 0 has {len(self.held[0])} pages")
+        shared = self.held[0][:full]
         for row in range(1, self.spec.rows):
+            self.allocator.share(shared)
             self.allocator.give(self.held[row][:full])
-            self.held[row] = self.held[row][full:]
-            self._host_table[row, :full] = self._host_table[0, :full]
+            self.held[row] = shared + self.held[row][full:]
+            self._host_table[row, :full] = shared

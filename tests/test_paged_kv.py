@@ -72,3 +72,64 @@ def test_shared_prompt_pages_leave_every_row_its_own_tail():
     for row in range(3):
         c.release(row)
     assert c.allocator.free == 12
+
+
+def test_reserving_after_sharing_keeps_the_shared_pages_and_the_tails():
+    c = PagedKVCache(_spec(num_pages=12), device="cpu")
+    c.reserve([20, 20, 20])
+    c.share_prompt(19)
+    c.upload()
+    before, free = c.table.clone(), c.allocator.free
+    assert not c.reserve([24, 24, 20])  # what the rows have already
+    c.upload()
+    assert c.table.tolist() == before.tolist() and c.allocator.free == free
+    assert c.reserve([20, 25, 32])  # a page more for the last two rows, behind the ones that they have
+    c.upload()
+    t = c.table.tolist()
+    assert [r[:3] for r in t] == before[:, :3].tolist() and c.allocator.free == free - 2
+    assert t[1][3] != t[2][3] and not {t[1][3], t[2][3]} & {p for r in t for p in r[:3]}
+
+
+def test_a_shared_page_is_free_when_its_last_holder_goes():
+    c = PagedKVCache(_spec(num_pages=12), device="cpu")
+    c.reserve([20, 20, 20])
+    c.share_prompt(19)
+    shared = c.held[0][:2]
+    c.release(0)
+    assert c.allocator.free == 12 - 2 - 2  # row 0's tail went, the two shared pages and two tails did not
+    c.reserve([24, 0, 0])
+    c.upload()
+    assert not set(c.table[0, :3].tolist()) & set(c.held[1] + c.held[2])
+    assert c.table[1, :2].tolist() == c.table[2, :2].tolist() == shared
+    c.trim([24, 16, 0])
+    assert c.held[1] == shared and c.held[2] == []
+    c.trim([24, 0, 0])
+    c.release(0)
+    assert c.allocator.free == 12
+
+
+def test_rows_that_take_the_prompt_of_row_0_need_pages_for_their_tails_only():
+    c = PagedKVCache(_spec(num_pages=5), device="cpu")
+    c.reserve([19])
+    c.share_prompt(19)
+    assert c.reserve([19, 19, 19]) and c.allocator.free == 0
+    c.upload()
+    t = c.table.tolist()
+    assert t[0][:2] == t[1][:2] == t[2][:2] and len({r[2] for r in t}) == 3
+    c.share_prompt(19)  # again: nothing changes
+    c.upload()
+    assert c.table.tolist() == t and c.allocator.free == 0
+    with pytest.raises(ValueError, match="row 0 has 3 pages"):
+        c.share_prompt(32)
+
+
+def test_a_row_is_not_cut_inside_a_page_that_others_hold():
+    """The row's next token would go into that page, which is part of the other rows' prompt."""
+    c = PagedKVCache(_spec(num_pages=12), device="cpu")
+    c.reserve([20, 20, 20])
+    c.share_prompt(19)
+    for slots in ([19, 9, 19], [12, 19, 19]):
+        with pytest.raises(ValueError, match="other rows hold"):
+            c.trim(slots)
+        assert [len(h) for h in c.held] == [3, 3, 3]
+    c.trim([19, 16, 17])
