@@ -11,6 +11,7 @@ bookkeeping (which rows need another page); nothing is read back from the device
 
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass
 
 import numpy as np
@@ -83,15 +84,16 @@ class PageAllocator:
             self._holders[p] += 1
 
     def give(self, pages) -> None:
-        freed = []
-        for p in pages:
-            if p not in self._holders:
-                raise ValueError(f"page {p} is not taken")
-            self._holders[p] -= 1
+        """One holder less for each page (all of them or, on an error, none)."""
+        count = Counter(pages)
+        for p, n in count.items():
+            if n > self.holders(p):
+                raise ValueError(f"page {p} is not taken" + (" as often" if p in self._holders else ""))
+        for p, n in count.items():
+            self._holders[p] -= n
             if not self._holders[p]:
                 del self._holders[p]
-                freed.append(p)
-        self._free = sorted(self._free + freed, reverse=True)
+        self._free = sorted(self._free + [p for p in count if p not in self._holders], reverse=True)
 
 
 class PagedKVCache:

@@ -133,3 +133,13 @@ def test_a_row_is_not_cut_inside_a_page_that_others_hold():
             c.trim(slots)
         assert [len(h) for h in c.held] == [3, 3, 3]
     c.trim([19, 16, 17])
+
+
+def test_giving_a_page_twice_changes_nothing():
+    a = PageAllocator(4)
+    a.take(3)
+    with pytest.raises(ValueError, match="page 1"):
+        a.give([0, 1, 1])
+    assert a.free == 1
+    a.give([0, 1])
+    assert a.free == 3
