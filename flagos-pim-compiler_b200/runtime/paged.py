@@ -293,8 +293,8 @@ class PagedLlama:
         self._start([prompt])
         with torch.cuda.device(self.device), torch.cuda.stream(self.stream):
             c = self.cache
-            c.reserve([n + steps - 1] * w)
             c.share_prompt(n)
+            c.reserve([n + steps - 1] * w)  # a tail for each beam: its partly filled page and what the search will fill
             c.upload()
             self._beam_tables = True  # from here on the table is the device's
             self._beam_slots = n + steps - 1

@@ -245,3 +245,21 @@ def test_a_step_behind_a_search_stays_within_its_pages():
         gen.step()
     again = gen.beam_search(prompt, 9)
     assert again.tokens.tolist() == first.tokens.tolist() and again.scores.tolist() == first.scores.tolist()
+
+
+def test_beam_search_needs_the_prompts_pages_once_and_a_tail_for_each_beam():
+    """Ten pages are enough for eight beams over two pages of prompt and one of new tokens; nine are refused."""
+    from runtime.paged import PagedLlama
+
+    runner = _runner(tiny_gqa_hf_model())
+    prompt = np.random.default_rng(3).integers(0, 1024, 16)
+    want = PagedLlama(runner, rows=8, max_slots=40, page_size=8).beam_search(prompt, 9)
+    gen = PagedLlama(runner, rows=8, max_slots=40, page_size=8, num_pages=10)
+    for _ in range(2):
+        got = gen.beam_search(prompt, 9)
+        assert got.tokens.tolist() == want.tokens.tolist() and got.scores.tolist() == want.scores.tolist()
+    small = PagedLlama(runner, rows=8, max_slots=40, page_size=8, num_pages=9)
+    with pytest.raises(MemoryError):
+        small.beam_search(prompt, 9)
+    small.reset()
+    assert small.cache.allocator.free == 9
