@@ -7,9 +7,10 @@
 // largest logits: beam_partial_kernel reads every logit once, into registers, and leaves per
 // chunk the sorted K largest (as 64-bit keys: the logit's order-preserving bits above the
 // complement of its token, so keys are unique and equal logits rank by token) and the
-// chunk's maximum and sum of exponentials.  beam_merge_kernel joins the sums to the beams' lse
-// in fp64 (neighbouring candidates decide which tokens come out), merges each beam's lists
-// with one warp and then the beams.
+// chunk's maximum and sum of exponentials.  beam_merge_kernel joins the sums to the beams' lse,
+// merges each beam's lists with one warp and then the beams.  Exponentials and sums are fp64
+// throughout: candidates of different beams that lie next to one another decide which tokens come
+// out, and fp32's error (3e-7 in a row of equal logits) is the same for every term of such a row.
 //
 // The K largest of a chunk: if every warp's ceil(K / warps)-th largest lane maximum is at least
 // tau, then K values are, so only those >= tau, a few times K of them, are collected and ranked
@@ -18,9 +19,9 @@
 // only K threads can hold keys at or above it.
 //
 // Measured (the three kernels one after another): 4 beams of one prompt, 32000 bf16 logits, 32 layers' pages
-// 11.4 us, three launches' latency; 32 x 8 beams 84 us, of which the page copies, 354 MB, take 63 (5.6 TB/s); 8 x 16
-// beams of 131072 fp32 logits 56 us: the pass over the logits 19.5 us for 53 MB, bound by instructions (51 %
-// issued; 29 us with keys made of every logit, 65 with a 256-way ranking), the merge 10, the copies 28.
+// 13 us, three launches' latency; 32 x 8 beams 84 us, of which the page copies, 354 MB, take 63 (5.6 TB/s) and the pass
+// over the logits 16; 8 x 16 beams of 131072 fp32 logits 65 us: the pass 29 us for 53 MB (20 with fp32 exponentials; bound by
+// instructions, the 64-bit pipe's 11 a logit alone 10 us), the merge 11, the copies 25.
 //
 // Reordering.  See pim_beam_reorder in pim_b200.h: the table entries of full pages follow
 // the parent, the partly filled pages of an entry's beams are dealt out again, and the
@@ -70,14 +71,22 @@ __device__ __forceinline__ unsigned long long beam_key(uint32_t order, int token
 }
 __device__ __forceinline__ int key_token(unsigned long long key) { return (int)~(uint32_t)key; }
 
-// log2(e) in two parts, and 2^x.
-constexpr float kLog2eHi = 1.4426950408889634f;
-constexpr float kLog2eLo = (float)(1.4426950408889634 - (double)kLog2eHi);
-static_assert(kLog2eLo > 0, "-inf x kLog2eLo must stay -inf");
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// sum + e^d for d <= 0 in 64 bits, by a table of 2^(j / 32) (P. T. P. Tang, "Table-driven implementation of the
+// exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989): d = (32 k + j) log(2) / 32 + r with
+// |r| < 0.011, e^d = 2^k 2^(j / 32) e^r, and e^r by its series to r^6 / 6! (what is left is below 2^-57).  Below -700: 0.
+// (8 x 16 beams of 131072 logits with the reordering: 66.5 us; 66.2 with 64 entries and 67.8 with 16, a term less and more.)
+constexpr int kExpTable = 32;
+__device__ __forceinline__ double add_exp(double sum, double d, const double* table) {
+  constexpr double kRound = 6755399441055744.0;  // 1.5 x 2^52: a sum with it has a whole number in its low word
+  const double z = fma(d, kExpTable * 1.4426950408889634074, kRound);
+  const int n = __double2loint(z);
+  const double r = fma(z - kRound, -0.69314718055994530942 / kExpTable, d);
+  double e = fma(r, fma(r, fma(r, 1.0 / 720, 1.0 / 120), 1.0 / 24), 1.0 / 6);
+  e = fma(r, fma(r, fma(r, e, 0.5), 1.0), 1.0);
+  const double t = table[n & (kExpTable - 1)];
+  const double scaled = __hiloint2double(__double2hiint(t) + (n >> 5) * (1 << 20), __double2loint(t));
+  // (a negative number's upper word grows with its magnitude, up to -infinity's; -700's is 0xc085e000)
+  return (uint32_t)__double2hiint(d) > 0xc085e000u ? sum : fma(scaled, e, sum);
 }
 
 // The largest of the lanes' 64-bit keys: two 32-bit warp reductions.
@@ -97,11 +106,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   constexpr int V = VecW<T>::n, kBeamCand = kMaxBeams * kBeamVals;
   __shared__ unsigned long long sm_cand[kBeamCand];
   __shared__ uint32_t sm_top[kBeamWarps], sm_low[kBeamWarps];
-  __shared__ double sm_s[kBeamWarps];
+  __shared__ double sm_s[kBeamWarps], sm_exp[kExpTable];
   __shared__ unsigned long long sm_tau;
   __shared__ int sm_n;
   const int split = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   pdl_trigger();
+  if (tid < kExpTable) sm_exp[tid] = exp2((double)tid / kExpTable);
   pdl_wait();
   if (a.done && a.done[row]) return;  // offers one candidate, which the merge adds
   const T* row_x = static_cast<const T*>(a.logits) + row * a.stride;
@@ -157,16 +167,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
         if (at < kBeamCand) sm_cand[at] = beam_key(logit_order(x[i]), base + tok(i));
       }
   }
-  // exp(x - m) = 2^((x - m) log2(e)), log2(e) in two parts; the difference first, so that logits near the type's limits
-  // (a mask of its lowest value) stay in range.  A thread's 16 or 32 of them in fp32, the sum over threads in fp64.
-  const float m = top ? order_logit(top) : 0.f;
-  float part = 0.f;
+  // The sum in 64 bits: neighbouring candidates of different beams decide which tokens come out, and an error of the
+  // exponential in 32 bits does not average out over a row of equal logits.
+  const double m = top ? (double)order_logit(top) : 0.0;
+  double s = 0;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) {  // (-inf gives 0: kLog2eLo is positive)
-    const float d = x[i] - m;
-    part += exp2_approx(fmaf(d, kLog2eHi, d * kLog2eLo));
-  }
-  double s = part;
+  for (int i = 0; i < kBeamVals; ++i) s = add_exp(s, (double)x[i] - m, sm_exp);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   if (lane == 0) sm_s[warp] = s;
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   }
   if (tid == 0) {
     BeamStats st;
-    st.max = top ? m : -INFINITY;
+    st.max = top ? (float)m : -INFINITY;
     st.count = min(n, a.k);
     st.sum = 0;
     for (int w = 0; w < kBeamWarps; ++w) st.sum += sm_s[w];
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
     double s = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-      if (lm[q] != -INFINITY) s += ls[q] * expf(lm[q] - m);
+      if (lm[q] != -INFINITY) s += ls[q] * exp((double)lm[q] - (double)m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {

@@ -716,6 +716,53 @@ def test_beam_select_logits_near_the_types_limits(vocab, dt):
     _check_select(logits[:, :1], torch.tensor([[-1.5]], device="cuda"), 5)
 
 
+def _crowded_rows(vocab, dt):
+    """Rows whose sums of exponentials have as many equal terms as can be: a rounding of one is a rounding of the sum."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    rows = torch.empty(6, vocab, device="cuda")
+    for i, rest in enumerate((-0.1, -0.7, -3.3, -9.0, -17.0)):
+        rows[i] = rest
+        rows[i, vocab // 3] = 0.0
+    rows[5] = torch.linspace(-12, 4, vocab, device="cuda")[torch.randperm(vocab, device="cuda", generator=g)]
+    return rows.to(_tdt(dt))
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [7, 1003, 8192, 50001, 131072])
+def test_beam_select_sums_in_64_bits(vocab, dt):
+    """A beam's score is chosen so that it all but cancels the logarithm of its sum: what is left comes out rounded once.
+    The sum's own error: 2^-50 a term (an exponential in 64 bits) and 2^-53 an addition, of which a term passes fewer than
+    200 (32 in a thread, 13 across a CTA, 128 chunks); its logarithm and the subtractions, at numbers below 32, 2^-48."""
+    torch = _torch()
+    logits = _crowded_rows(vocab, dt)[:, None]
+    x = _host(logits)[:, 0]
+    lse = np.log(np.exp(x - x.max(1, keepdims=True)).sum(1)) + x.max(1)
+    scores = torch.tensor(lse - x.max(1), dtype=torch.float32, device="cuda")[:, None]
+    got = _select(logits, scores, 1)
+    want = _host(scores)[:, 0] + (x.max(1) - lse)
+    assert (got[2][:, 0] == x.argmax(1)).all()
+    assert (np.abs(got[0][:, 0] - want) <= 2.0**-24 * np.abs(want) + 2.0**-50 + 200 * 2.0**-53 + 2.0**-48).all()
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [1003, 8192, 131072])
+def test_beam_select_orders_beams_that_lie_close_together(vocab, dt):
+    """A beam against an ended one whose score is 2e-9 above or below its best candidate's: the better one comes first."""
+    torch = _torch()
+    rows = _crowded_rows(vocab, dt)
+    x = _host(rows)
+    below = x.max(1) - (np.log(np.exp(x - x.max(1, keepdims=True)).sum(1)) + x.max(1))  # the best token's log-probability
+    score = (-below - 1e-3).astype(np.float32)
+    best = score.astype(np.float64) + below  # about -1e-3, where fp32 has steps of 1e-10
+    logits = torch.stack([rows, rows], dim=1)
+    done = _ints([[0, 1]] * 6)
+    for off in (-2e-9, 2e-9):
+        scores = torch.tensor(np.stack([score, best + off], 1), dtype=torch.float32, device="cuda")
+        got = _select(logits, scores, 2, done, pad=5)
+        assert got[1][:, 0].tolist() == [1 if off > 0 else 0] * 6, off
+
+
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 @pytest.mark.parametrize("vocab", [8200, 26080, 4100])
 def test_beam_select_of_rows_that_crowd_in_a_few_warps(vocab, dt):
