@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <utility>
 
 namespace pim {
@@ -171,7 +172,10 @@ bool pdl_enabled();
 // attribute calls after the first eager run -- then the occupancy API answers (the last
 // 16 sizes are cached, more than any plan uses per kernel, so a capture that follows an
 // eager run of its plan queries nothing).  Returns -1 with the CUDA error in *err on failure.
+// Threads take turns: with sizes that differ from call to call the smaller of two limits, set
+// last, would otherwise stand under a record of the larger, and refuse the larger's launches.
 struct ResidentCache {
+  std::mutex turn;
   size_t attr_bytes[64] = {};
   bool carveout[64] = {};
   size_t smem[64][16] = {};
@@ -188,6 +192,7 @@ int resident_ctas(Kern kern, int threads, size_t smem, ResidentCache& c, cudaErr
     *err = cudaErrorInvalidDevice;
     return -1;
   }
+  const std::lock_guard<std::mutex> hold(c.turn);
   if (!c.carveout[dev]) {
     *err = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
                                 (int)cudaSharedmemCarveoutMaxShared);
