@@ -17,7 +17,7 @@ with the same stride between pages), float32 or bfloat16.  An operator owns its 
 its calls, and replays of graphs that hold them, must not overlap on the GPU; make another one
 for another stream.  Its tensors must stay alive while a graph that holds a call can be
 replayed: keep the operator.  A bad length, position, page id or parent found on the device
-raises the operator's error flag, which ``check()`` turns into an exception (it synchronises).
+raises the operator's error flag, which ``check()`` turns into an exception (it waits for the device).
 """
 
 from __future__ import annotations
@@ -176,6 +176,11 @@ class _Op:
         self._extra = extra
         self._index = dev.index
         self._seen = {_raw_stream(torch, dev.index)}
+        # the flag's zero, and what used the workspace's memory before, lie on this stream: others wait for it once
+        self._made = None
+        if not torch.cuda.is_current_stream_capturing():
+            self._made = torch.cuda.Event()
+            self._made.record(torch.cuda.current_stream(dev))
 
     def _run(self) -> None:
         torch, index = self._torch, self._index
@@ -183,6 +188,8 @@ class _Op:
         if st not in self._seen and not torch.cuda.is_current_stream_capturing():
             self._seen.add(st)  # its memory is given back only after this stream's work, too
             stream = torch.cuda.current_stream(self._dev)
+            if self._made is not None:
+                stream.wait_event(self._made)
             for t in (*self._keep, self._ws, self._err):
                 if t is not None:
                     t.record_stream(stream)
@@ -195,9 +202,14 @@ class _Op:
             nat.check(rc, self.name)
 
     def check(self) -> None:
-        """Raises if a call so far met a bad length, position, page id or parent; clears the flag."""
-        if self._err is not None and int(self._err.item()):
+        """Waits for the device, and raises if a call so far, on whichever stream, met a bad length, position, page id or
+        parent; clears the flag."""
+        if self._err is None:
+            return
+        self._torch.cuda.synchronize(self._dev)
+        if int(self._err.item()):
             self._err.zero_()
+            self._torch.cuda.synchronize(self._dev)  # (calls that follow on other streams raise it anew)
             raise ValueError(f"{self.name}: a length, position, page id or parent was out of range")
 
 

@@ -989,3 +989,72 @@ def test_an_operator_dropped_while_its_work_is_pending_keeps_its_memory():
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
         del junk
+
+
+def _wait_a_moment():
+    _torch().cuda._sleep(100_000_000)  # about 50 ms of the current stream
+
+
+def test_check_sees_errors_of_calls_on_other_streams():
+    """A call that is still waiting on another stream when ``check`` is asked on this one."""
+    torch = _torch()
+    pool, q, out, _, _, op = _attention_case([40, 30], 2, 2, 16, 64, "bfloat16", seed=41)
+    pool.lengths.copy_(_ints([40, -1]))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            _wait_a_moment()
+            op()
+        with pytest.raises(ValueError, match="out of range"):
+            op.check()
+    op.check()  # cleared
+
+
+def test_an_operator_made_behind_pending_work_keeps_what_another_stream_reports():
+    """The flag's zero waits on the stream that the operator was made on: a call on another one comes behind it."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    pool, q, out, _, _, first = _attention_case([9000, 30], 2, 2, 16, 64, "bfloat16", seed=42)
+    first()
+    want = out.clone()
+    bad = _ints([9000, 10**6])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for lengths in (bad, pool.lengths):
+        out.zero_()
+        torch.cuda.synchronize()
+        _wait_a_moment()
+        op = PagedAttention(q, pool.k, pool.v, pool.table, lengths, out)
+        with torch.cuda.stream(side):
+            op()
+        torch.cuda.synchronize()
+        if lengths is bad:
+            with pytest.raises(ValueError, match="out of range"):
+                op.check()
+        else:
+            op.check()
+            assert torch.equal(out, want)
+
+
+def test_an_operator_made_and_called_inside_a_capture():
+    """Its flag and workspace belong to the graph; replays report what they meet."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    pool, q, out, _, _, first = _attention_case([9000, 30], 2, 2, 16, 64, "bfloat16", seed=43)
+    first()
+    want = out.clone()
+    out.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op = PagedAttention(q, pool.k, pool.v, pool.table, pool.lengths, out)
+        op()
+    graph.replay()
+    op.check()
+    assert torch.equal(out, want)
+    pool.lengths.copy_(_ints([9000, -3]))
+    graph.replay()
+    with pytest.raises(ValueError, match="out of range"):
+        op.check()
