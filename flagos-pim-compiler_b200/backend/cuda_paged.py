@@ -201,6 +201,11 @@ class _Op:
         if rc:
             nat.check(rc, self.name)
 
+    def clear(self) -> None:
+        """Forgets, on the device's current stream, what the calls so far met."""
+        if self._err is not None:
+            self._err.zero_()
+
     def check(self) -> None:
         """Waits for the device, and raises if a call so far, on whichever stream, met a bad length, position, page id or
         parent; clears the flag."""

@@ -184,12 +184,15 @@ class PagedLlama:
 
     # -- prompts ------------------------------------------------------------------------------------------------
     def reset(self) -> None:
-        """Gives every page back and empties the rows."""
+        """Gives every page back and empties the rows; errors that nobody asked for are forgotten."""
         with self.torch.cuda.device(self.device), self.torch.cuda.stream(self.stream):
             for row in range(self.rows):
                 self.cache.release(row)
             self.lengths.zero_()
             self.positions.zero_()
+            self.err.zero_()
+            for op in self.ops:
+                op.clear()
         self.slots[:] = 0
         self.pos_host = 0
         self._beam_tables = False
@@ -249,12 +252,22 @@ class PagedLlama:
         self.pos_host = n
 
     # -- generation -------------------------------------------------------------------------------------------------
-    def check(self) -> None:
-        """Raises if a step met a bad id, length, position or page (synchronises)."""
+    def check(self, *more) -> None:
+        """Raises if a step (or a call of the operators ``more``) met a bad id, length, position or page.  Waits for the
+        device; every flag is cleared, so what follows is judged by itself."""
+        self.torch.cuda.synchronize(self.device)
+        said = []
         if bool(self.err.any()):
-            raise ValueError("a token id was outside the vocabulary, or a projection's wait ran out")
-        for op in self.ops:
-            op.check()
+            self.err.zero_()
+            said.append("a token id was outside the vocabulary, or a projection's wait ran out")
+        for op in (*self.ops, *more):
+            try:
+                op.check()
+            except ValueError as e:
+                said.append(str(e))
+        if said:
+            self.torch.cuda.synchronize(self.device)
+            raise ValueError("; ".join(dict.fromkeys(said)))
 
     def greedy(self, prompts, steps: int, keep_logits: list | None = None) -> np.ndarray:
         """[rows, steps] tokens; ``keep_logits`` (a list) receives each step's [rows, vocab] logits."""
@@ -331,6 +344,5 @@ class PagedLlama:
             for i in range(steps - 1, -1, -1):
                 result.tokens[j, i] = tok[i, at]
                 at = par[i, at]
-        reorder.check()
-        self.check()
+        self.check(reorder)
         return result

@@ -263,3 +263,26 @@ def test_beam_search_needs_the_prompts_pages_once_and_a_tail_for_each_beam():
         small.beam_search(prompt, 9)
     small.reset()
     assert small.cache.allocator.free == 9
+
+
+def test_an_error_is_reported_once_and_the_next_run_is_judged_by_itself():
+    """A token id outside the vocabulary, and lengths that every layer's operators find bad."""
+    from runtime.paged import PagedLlama
+
+    gold = tiny_golden()
+    gen = PagedLlama(_runner(tiny_hf_model()), rows=1, max_slots=40, page_size=8)
+    prompt = gold["prompt"][None]
+    for spoil, said in ((lambda: gen.ids.fill_(10**6), "vocabulary"), (lambda: gen.lengths.fill_(-7), "pim_paged_append")):
+        gen._start(prompt)
+        gen.ids.fill_(1)
+        spoil()
+        gen.step()
+        with pytest.raises(ValueError, match=said):
+            gen.check()
+        gen.check()
+        assert gen.greedy(prompt, 8)[0].tolist() == gold["tokens"].tolist()
+        gen._start(prompt)
+        gen.ids.fill_(1)
+        spoil()
+        gen.step()
+        assert gen.greedy(prompt, 8)[0].tolist() == gold["tokens"].tolist()  # (a new start: what was before is not its error)
