@@ -69,6 +69,39 @@ def _overlap(a, b) -> bool:
     return _meet(_span(a), _span(b))
 
 
+def _layout(t):
+    """(elements, byte stride) of the dimensions of more than one element, the widest stride first."""
+    item = t.element_size()
+    return sorted(((n, st * item) for n, st in zip(t.shape, t.stride()) if n > 1), key=lambda d: -d[1])
+
+
+def _share(a, b) -> bool:
+    """Whether two tensors whose ranges meet share a byte.  Told exactly for tensors of equal strides (parts of one buffer's
+    rows); others are taken to."""
+    da, db = _layout(a), _layout(b)
+    if [st for _, st in da] != [st for _, st in db]:
+        return True
+    ia, ib = a.element_size(), b.element_size()
+    # an element of b lies `at` + sum of (difference of indices) x stride behind one of a
+    dims = [(na, nb, st) for (na, st), (nb, _) in zip(da, db)]
+
+    def meets(at: int, k: int) -> bool:
+        if k == len(dims):
+            return -ib < at < ia
+        na, nb, st = dims[k]
+        # the inner dimensions' differences lie between -(a's extent) and b's
+        down = sum((n - 1) * s for _, n, s in dims[k + 1:]) + ib - 1
+        up = sum((n - 1) * s for n, _, s in dims[k + 1:]) + ia - 1
+        if st == 0:
+            return meets(at, k + 1)
+        first, last = max(-(na - 1), -((at + down) // st)), min(nb - 1, (up - at) // st)
+        if last - first > 16:  # (strides that nest in no order)
+            return True
+        return any(meets(at + i * st, k + 1) for i in range(first, last + 1))
+
+    return meets(b.data_ptr() - a.data_ptr(), 0)
+
+
 def _rows_apart(a, b) -> bool:
     """Whether two [tokens, heads, head_dim] views share no element; views of one buffer of equal rows (the parts of a
     fused qkv row) are told apart by where in the row they lie."""
@@ -87,11 +120,11 @@ def _rows_apart(a, b) -> bool:
 
 def _apart(outputs: dict, others: dict) -> None:
     """No output shares memory with another output or with an input."""
-    outs = [(n, _span(t)) for n, t in outputs.items() if t is not None]
-    ins = [(n, _span(t)) for n, t in others.items() if t is not None]
-    for i, (n, span) in enumerate(outs):
-        for m, other in outs[i + 1:] + ins:
-            if _meet(span, other):
+    outs = [(n, t, _span(t)) for n, t in outputs.items() if t is not None]
+    ins = [(n, t, _span(t)) for n, t in others.items() if t is not None]
+    for i, (n, t, span) in enumerate(outs):
+        for m, other, where in outs[i + 1:] + ins:
+            if _meet(span, where) and _share(t, other):
                 raise ValueError(f"{n} shares memory with {m}")
 
 
@@ -107,8 +140,7 @@ def _paged_kv(k_pages, v_pages, table) -> nat.PagedKV:
     stride = k_pages.stride(0) if num > 1 else heads * ps * hd
     if num > 1 and v_pages.stride(0) != stride:
         raise ValueError("k_pages and v_pages: the stride between pages must be the same")
-    if _overlap(k_pages, v_pages) and stride < 2 * heads * ps * hd:
-        raise ValueError("k_pages shares memory with v_pages")
+    _apart(dict(k_pages=k_pages), dict(v_pages=v_pages))
     _want(table, "table", (None, None), "int32", contiguous=False)
     return nat.PagedKV(k_pages=k_pages.data_ptr(), v_pages=v_pages.data_ptr(), page_stride=stride,
                        table=table.data_ptr(), table_stride=table.stride(0) if table.shape[0] > 1 else table.shape[1],
@@ -276,10 +308,12 @@ class PagedAppend(_Op):
                 raise ValueError("slot_positions and weights: their strides must be the same")
             a.slot_positions, a.weights = slot_positions.data_ptr(), weights.data_ptr()
             a.state_row_stride, a.state_head_stride = _state_strides(weights)
-        _apart(dict(lengths_out=lengths_out, positions_out=positions_out),
-               dict(lengths=lengths, positions=positions, starts=starts, table=table))
+        read = dict(lengths=lengths, positions=positions, starts=starts, table=table, cos=cos, sin=sin)
+        _apart(dict(lengths_out=lengths_out, positions_out=positions_out, slot_positions=slot_positions, weights=weights),
+               dict(read, k_pages=k_pages, v_pages=v_pages, k=k, v=v, q=q, q_out=q_out))
         for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
-            _apart({name: pages}, dict(k=k, v=v, q=q, q_out=q_out))
+            _apart({name: pages}, dict(read, k=k, v=v, q=q, q_out=q_out))
+        _apart(dict(q_out=q_out), read)
         if q is not None:
             for name, t in (("q", q), ("k", k), ("v", v)):
                 if not (t is q and q_out.data_ptr() == q.data_ptr()) and not _rows_apart(q_out, t):
@@ -357,6 +391,9 @@ class PagedEvict(_Op):
                 raise ValueError(f"{name} shares part of its input's memory: it must be its input or apart")
         _apart(dict(weights_out=weights_out, slot_positions_out=slot_positions_out, lengths_out=lengths_out),
                dict(k_pages=k_pages, v_pages=v_pages, table=table, lengths=lengths, positions=positions))
+        read = dict(table=table, lengths=lengths, positions=positions, weights=weights, slot_positions=slot_positions)
+        for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _apart({name: pages}, read)
         _apart(dict(weights_out=weights_out, lengths_out=lengths_out), dict(slot_positions=slot_positions))
         _apart(dict(slot_positions_out=slot_positions_out, lengths_out=lengths_out), dict(weights=weights))
         row, head = _state_strides(weights)
@@ -447,7 +484,7 @@ class BeamReorder(_Op):
                                 lengths=lengths.data_ptr(), parents=parents.data_ptr(), batch=b, beams=w,
                                 num_blocks=blocks, max_pages=table.shape[1], num_pages=num, page_size=ps,
                                 kv_heads=heads, head_dim=hd)
-        _apart(dict(table_out=table_out), dict(table=table, lengths=lengths, parents=parents, pages=pages))
+        _apart(dict(table_out=table_out, pages=pages), dict(table=table, lengths=lengths, parents=parents))
         self._bind(a, _code(pages, "pages"), (pages, table, lengths, parents, table_out))
         self.table_out = table_out
 

@@ -324,3 +324,82 @@ def test_oracle_beam_reorder_gives_every_beam_its_parents_slots():
                 assert np.array_equal(ref.slots(after[blk], out[j], length), ref.slots(pages[blk], table[p], length))
         tails = out[:, full:].flatten().tolist()
         assert sorted(tails) == sorted(table[:, full:].flatten().tolist())  # no page is lost or held twice
+
+
+def test_pools_that_overlap_are_refused_and_interleaved_ones_are_not():
+    """K and V as halves of each page of one buffer share nothing; V half a page behind K does, as do single pages."""
+    from backend.cuda_paged import PagedAttention
+
+    heads, ps, hd, num = 2, 16, 64, 6
+    page = heads * ps * hd
+    t = _tensors(heads=heads, ps=ps, hd=hd)
+    q, out = torch.zeros(3, 4, hd, dtype=torch.bfloat16), torch.zeros(3, 4, hd, dtype=torch.bfloat16)
+    buf = torch.zeros(3 * num * page, dtype=torch.bfloat16)
+
+    def pool(at, pitch, n=num):
+        return buf.as_strided((n, heads, ps, hd), (pitch, ps * hd, hd, 1), at)
+
+    for k, v, ok in ((pool(0, 2 * page), pool(page, 2 * page), True), (pool(page, 2 * page), pool(0, 2 * page), True),
+                     (pool(0, 2 * page), pool(page // 2, 2 * page), False), (pool(0, 2 * page), pool(page + 8, 2 * page), False),
+                     (pool(0, 3 * page), pool(page + page // 2, 3 * page), True),
+                     (pool(0, 2 * page), pool(2 * page, 2 * page), False), (pool(0, page), pool(num * page, page), True),
+                     (pool(0, page, 1), pool(page - 8, page, 1), False), (pool(0, page, 1), pool(page, page, 1), True)):
+        with pytest.raises(ValueError, match="needs CUDA" if ok else "k_pages shares memory with v_pages"):
+            PagedAttention(q, k, v, t["table"], t["lengths"], out)
+
+
+def test_append_class_keeps_all_that_it_writes_apart():
+    from backend.cuda_paged import PagedAppend
+
+    t = _tensors()
+    k, v = (torch.zeros(3, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    w, p = torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, dtype=torch.int32)
+    f = torch.float32
+    both = torch.zeros(3, 2, 2, 64)  # [rows, heads, positions | weights, slots]: interleaved, nothing shared
+    floats = torch.zeros(12 * 2 * 16 * 64 // 2)
+    paged = floats.view(torch.bfloat16).view(12, 2, 16, 64)
+
+    def make(pages=None, **kw):
+        a = {**t, **(pages or {})}
+        PagedAppend(k, v, a["k_pages"], a["v_pages"], a["table"], a["lengths"], **kw)
+
+    for said, pages, kw in [
+            ("needs CUDA", None, dict(slot_positions=p, weights=w)),
+            ("needs CUDA", None, dict(slot_positions=both[:, :, 0].view(torch.int32), weights=both[:, :, 1])),
+            ("slot_positions shares memory with weights", None, dict(slot_positions=w.view(torch.int32), weights=w)),
+            ("slot_positions shares memory with weights", None,
+             dict(slot_positions=both.view(3, 2, 128)[:, :, 8:72].view(torch.int32), weights=both[:, :, 0])),
+            ("weights shares memory with k_pages", dict(k_pages=paged), dict(slot_positions=p, weights=floats[:384].view(3, 2, 64))),
+            ("slot_positions shares memory with v_pages", dict(v_pages=paged),
+             dict(slot_positions=floats[:384].view(3, 2, 64).view(torch.int32), weights=w)),
+            ("slot_positions shares memory with lengths", dict(lengths=p.view(-1)[:3]), dict(slot_positions=p, weights=w)),
+            ("slot_positions shares memory with table", dict(table=p.view(-1)[:12].view(3, 4)), dict(slot_positions=p, weights=w)),
+            ("lengths_out shares memory with k_pages", dict(k_pages=paged), dict(lengths_out=floats[:3].view(torch.int32))),
+            ("k_pages shares memory with table", dict(k_pages=paged, table=floats.view(torch.int32)[:12].view(3, 4)), {}),
+            ("k_pages shares memory with cos", dict(k_pages=paged), dict(cos=floats[:320].view(10, 32), sin=torch.zeros(10, 32, dtype=f))),
+            ("q_out shares memory with lengths", dict(lengths=floats[:3].view(torch.int32)),
+             dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), q_out=floats.view(torch.bfloat16)[:768].view(3, 4, 64)))]:
+        with pytest.raises(ValueError, match=said):
+            make(pages, **kw)
+
+
+def test_evict_and_reorder_classes_keep_the_pages_apart_from_what_they_read():
+    from backend.cuda_paged import BeamReorder, PagedEvict
+
+    t = _tensors()
+    w, p = torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, dtype=torch.int32)
+    n, out = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    floats = torch.zeros(12 * 2 * 16 * 64 // 2)
+    paged = floats.view(torch.bfloat16).view(12, 2, 16, 64)
+    with pytest.raises(ValueError, match="v_pages shares memory with positions"):
+        PagedEvict(t["k_pages"], paged, t["table"], t["lengths"], w, p, floats.view(torch.int32)[:3], w.clone(), p.clone(), out, budget=8)
+    with pytest.raises(ValueError, match="k_pages shares memory with weights"):
+        PagedEvict(paged, t["v_pages"], t["table"], t["lengths"], floats[:384].view(3, 2, 64), p, n, w, p.clone(), out, budget=8)
+    pool = torch.zeros(2, 2, 6, 1, 8, 32)
+    ints = pool.view(-1).view(torch.int32)
+    table, lengths, parents = (torch.zeros(s, dtype=torch.int32) for s in ((8, 3), (2,), (2, 4)))
+    for kw, said in ((dict(table=ints[:24].view(8, 3)), "table"), (dict(lengths=ints[:2]), "lengths"),
+                     (dict(parents=ints[:8].view(2, 4)), "parents")):
+        a = {**dict(table=table, lengths=lengths, parents=parents), **kw}
+        with pytest.raises(ValueError, match=f"pages shares memory with {said}"):
+            BeamReorder(pool, a["table"], a["lengths"], a["parents"], torch.zeros(8, 3, dtype=torch.int32))
