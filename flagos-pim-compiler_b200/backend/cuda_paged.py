@@ -256,7 +256,8 @@ class PagedAppend(_Op):
     ``k``, ``v`` [tokens, kv_heads, head_dim] and ``q`` [tokens, q_heads, head_dim] may be strided views (of a fused
     qkv row, of a contiguous KV block); ``starts`` [rows + 1] gives each row's tokens (without it, one token per
     row).  The tokens of row b go to slots ``lengths[b]``, ``lengths[b] + 1``, ... at positions ``positions[b]``, ...
-    (``lengths`` where not given); ``lengths_out`` / ``positions_out`` receive the counts after the call.
+    (``lengths`` where not given); ``lengths_out`` / ``positions_out`` receive the counts after the call, tokens that
+    were left out for a bad slot, page or position (see ``check``) counted too.
     ``cos`` / ``sin`` [max_pos, head_dim / 2] fp32: without them nothing is rotated.  ``pair_order``: heads come in
     the row order of ``qkv_proj.weight`` (dims j and j + head_dim / 2 adjacent).  ``slot_positions`` / ``weights``
     [rows, kv_heads, slots]: the eviction state of the new slots is set.

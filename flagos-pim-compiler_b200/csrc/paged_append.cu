@@ -105,10 +105,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a, in
   pdl_wait();
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.starts && (a.starts[0] < 0 || a.starts[a.kv.rows] > a.tokens))
     raise_flag(a.err);
-  if ((int)blockIdx.x >= work_ctas) {  // the lengths after the call
+  if ((int)blockIdx.x >= work_ctas) {  // the rows' token counts, and the lengths after the call
     const int b = (blockIdx.x - work_ctas) * kAppendThreads + threadIdx.x;
     if (b < a.kv.rows) {
-      const int n = a.starts ? a.starts[b + 1] - a.starts[b] : 1;
+      int n = 1;
+      if (a.starts) {
+        const int64_t count = (int64_t)a.starts[b + 1] - a.starts[b];
+        if (count < 0) raise_flag(a.err);
+        n = (int)min(max(count, (int64_t)0), (int64_t)INT32_MAX);
+      }
       const int len = a.lengths[b];
       if (a.lengths_out) a.lengths_out[b] = len + n;
       if (a.positions_out) a.positions_out[b] = (a.positions ? a.positions[b] : len) + n;
@@ -182,7 +187,7 @@ static cudaError_t append(const AppendArgs& a, int hd, int dtype, cudaStream_t s
     constexpr int HD = decltype(d)::value;
     const int per = (a.hq + 2 * a.kv.hkv) * (HD / 2 / VecW<T>::n);
     const int64_t items = a.tokens * per;
-    const int tail = a.lengths_out || a.positions_out ? ceil_div(a.kv.rows, kAppendThreads) : 0;
+    const int tail = a.lengths_out || a.positions_out || a.starts ? ceil_div(a.kv.rows, kAppendThreads) : 0;
     // few: the items do not fill the GPU's threads
     if (items <= 2048 * 148) {
       const int work = ceil_div(items, kAppendThreads);

@@ -399,7 +399,8 @@ typedef struct pim_paged_append_args {
                                qkv_proj.weight, as pim_projection PLAIN leaves it); outputs are in dim order */
   int64_t tokens;
   const int32_t* starts;    /* [rows + 1]: row b has tokens starts[b] .. starts[b + 1) (0 or more); NULL: token b is
-                               row b's only one, tokens == rows.  Tokens behind starts[rows] are left out. */
+                               row b's only one, tokens == rows.  Tokens behind starts[rows] are left out; starts that
+                               decrease (the row counts as without tokens) or leave [0, tokens] raise *err_flag. */
   const int32_t* lengths;   /* [rows] slots in use: the row's tokens go to slots lengths[b], lengths[b] + 1, ... */
   const int32_t* positions; /* [rows] position of the row's first new token; NULL: lengths */
   int32_t* lengths_out;     /* [rows] lengths + new tokens (not `lengths` itself); may be NULL */
@@ -414,7 +415,8 @@ typedef struct pim_paged_append_args {
  * position (RoPE, halves rotated against one another as in pim_projection ROPE_KV,
  * computed in fp32 and rounded once), v as it is; q rotated into q_out.  Replaces
  * PIMStaticKVCache.update (memory/kv_layout.py:187-205) over pages.  A token whose slot,
- * page or position is out of range raises *err_flag and is left out. */
+ * page or position is out of range raises *err_flag and is left out, but counted in
+ * lengths_out and positions_out: what follows would read a slot that was not written. */
 int pim_paged_append(const pim_paged_append_args* a, int32_t dtype, void* stream);
 
 typedef struct pim_paged_attention_args {

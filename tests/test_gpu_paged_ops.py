@@ -489,6 +489,30 @@ def test_append_leaves_out_what_does_not_fit():
     assert not _host(q_out)[:3].any() and _host(q_out)[3].any()
 
 
+@pytest.mark.parametrize("outs", [True, False])
+def test_append_reports_starts_that_decrease(outs):
+    """Rows never lose slots by them, and what is written stays within the rows' new slots."""
+    from backend.cuda_paged import PagedAppend
+
+    torch = _torch()
+    past, rows = [4, 5, 6], 3
+    for starts in ([0, 5, 3, 8], [0, -1, 2, 8], [8, 8, 8, 0], [2, 1, 1, 8], [0, 9, 8, 8]):
+        pool = Pool([0] * rows, heads=1, ps=8, hd=32, dt="float32", room=24)
+        k = torch.randn(8, 1, 32, device="cuda")
+        lengths_out, positions_out = (_ints([-1] * rows) for _ in range(2)) if outs else (None, None)
+        op = PagedAppend(k, k.clone(), pool.k, pool.v, pool.table, _ints(past), lengths_out, positions=_ints([9, 9, 9]),
+                         positions_out=positions_out, starts=_ints(starts))
+        op()
+        with pytest.raises(ValueError, match="out of range"):
+            op.check()
+        new = np.maximum(np.diff(starts), 0)
+        if outs:
+            assert lengths_out.tolist() == (past + new).tolist() and positions_out.tolist() == (9 + new).tolist()
+        for b in range(rows):
+            written = ~np.isnan(ref.slots(_host(pool.v), pool.table_np[b], 24)[0]).all(-1)
+            assert not written[:past[b]].any() and not written[past[b] + new[b]:].any()
+
+
 # ---- eviction -----------------------------------------------------------------------------------------------------------------
 
 def _evict_case(lengths, heads, ps, hd, dt, budget, recent, sink, seed=0, ties=False, in_place=False, weights=None,
