@@ -11,7 +11,7 @@ import os
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent.parent / "csrc" / "libpim_b200.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 F32, BF16, I32, I64 = 0, 1, 2, 3
 PROJ_PLAIN, PROJ_ROPE_KV, PROJ_SILU_MUL = 0, 1, 2
@@ -161,7 +161,7 @@ class BeamSelectArgs(ctypes.Structure):
 
     _fields_ = [("logits", c_vp), ("logits_stride", c_i64), ("scores", c_vp), ("done", c_vp), ("scores_out", c_vp),
                 ("parents", c_vp), ("tokens", c_vp), ("done_out", c_vp), ("batch", c_i32), ("beams", c_i32),
-                ("beams_out", c_i32), ("vocab", c_i32), ("eos", c_i32), ("pad", c_i32)]
+                ("beams_out", c_i32), ("vocab", c_i32), ("eos", c_i32), ("pad", c_i32), ("err_flag", c_vp)]
 
 
 class BeamReorderArgs(ctypes.Structure):

@@ -16,7 +16,7 @@ Pages are ``[num_pages, kv_heads, page_size, head_dim]`` tensors (one for K, one
 with the same stride between pages), float32 or bfloat16.  An operator owns its workspace:
 its calls, and replays of graphs that hold them, must not overlap on the GPU; make another one
 for another stream.  Its tensors must stay alive while a graph that holds a call can be
-replayed: keep the operator.  A bad length, position, page id or parent found on the device
+replayed: keep the operator.  A bad length, position, page id, parent or logit found on the device
 raises the operator's error flag, which ``check()`` turns into an exception (it waits for the device).
 """
 
@@ -179,6 +179,7 @@ class _Op:
 
     name = ""
     workspace = False
+    complaint = "a length, position, page id or parent was out of range"
 
     def _bind(self, args, code: int, tensors) -> None:
         import torch
@@ -239,15 +240,15 @@ class _Op:
             self._err.zero_()
 
     def check(self) -> None:
-        """Waits for the device, and raises if a call so far, on whichever stream, met a bad length, position, page id or
-        parent; clears the flag."""
+        """Waits for the device, and raises if a call so far, on whichever stream, met a bad length, position, page id,
+        parent or logit; clears the flag."""
         if self._err is None:
             return
         self._torch.cuda.synchronize(self._dev)
         if int(self._err.item()):
             self._err.zero_()
             self._torch.cuda.synchronize(self._dev)  # (calls that follow on other streams raise it anew)
-            raise ValueError(f"{self.name}: a length, position, page id or parent was out of range")
+            raise ValueError(f"{self.name}: {self.complaint}")
 
 
 class PagedAppend(_Op):
@@ -417,11 +418,13 @@ class BeamSelect(_Op):
     """One step of beam search (``pim_beam_select``); returns (scores_out, parents, tokens).
 
     ``logits`` [batch, beams, vocab]; ``scores`` [batch, beams] fp32; the outputs [batch, beams_out] (as many beams as
-    ``scores_out`` has).  ``done`` / ``done_out`` int32: beams that have ended.
+    ``scores_out`` has).  ``done`` / ``done_out`` int32: beams that have ended.  Logits and scores of -inf are masked;
+    NaN and +inf are left out likewise, and reported by ``check``.
     """
 
     name = "pim_beam_select"
     workspace = True
+    complaint = "a logit or score was NaN or +infinity"
 
     def __init__(self, logits, scores, scores_out, parents, tokens, *, done=None, done_out=None, eos: int = -1,
                  pad: int = 0) -> None:

@@ -54,6 +54,7 @@ struct BeamSelectArgs {
   int *parents, *tokens, *done_out;
   int batch, beams, k, vocab, eos, pad, splits;
   int chunk;  // tokens of a split: a multiple of 8
+  int* err;
   BeamStats* stats;           // [batch * beams][splits]
   unsigned long long* lists;  // [batch * beams][splits][k]
 };
@@ -87,6 +88,13 @@ __device__ __forceinline__ double add_exp(double sum, double d, const double* ta
   const double scaled = __hiloint2double(__double2hiint(t) + (n >> 5) * (1 << 20), __double2loint(t));
   // (a negative number's upper word grows with its magnitude, up to -infinity's; -700's is 0xc085e000)
   return (uint32_t)__double2hiint(d) > 0xc085e000u ? sum : fma(scaled, e, sum);
+}
+
+// The larger of two; NaN if one is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
 
 // The largest of the lanes' 64-bit keys: two 32-bit warp reductions.
@@ -138,9 +146,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   }
   float mine_x = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kBeamVals; ++i) {
-    x[i] = fabsf(x[i]) < INFINITY ? x[i] : -INFINITY;
-    mine_x = fmaxf(mine_x, x[i]);
+  for (int i = 0; i < kBeamVals; ++i) mine_x = max_or_nan(mine_x, x[i]);
+  if (!(mine_x < INFINITY)) {  // there is a NaN or +inf: reported, and left out
+    raise_flag(a.err);
+    mine_x = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kBeamVals; ++i) {
+      x[i] = fabsf(x[i]) < INFINITY ? x[i] : -INFINITY;
+      mine_x = fmaxf(mine_x, x[i]);
+    }
   }
   const uint32_t mine = logit_order(mine_x);
   const int rounds = (a.k + kBeamWarps - 1) / kBeamWarps;
@@ -244,6 +258,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamSelectArg
     const int row = b * a.beams + w;
     const int done = a.done ? a.done[row] : 0;
     const float score = a.scores[row];
+    if (lane == 0 && !(score < INFINITY)) raise_flag(a.err);
     unsigned long long* keys = sm_keys + w * a.k;
     // lane i merges lists i, i + 32, ..: the first kDeep keys of each are at hand
     unsigned long long key[Q][kDeep];
@@ -523,6 +538,7 @@ extern "C" int pim_beam_select(const pim_beam_select_args* a, int32_t dtype, voi
   d.pad = a->pad;
   d.splits = beam_splits(a);
   d.chunk = beam_chunk(a);
+  d.err = a->err_flag;
   d.stats = static_cast<BeamStats*>(workspace);
   d.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + beam_stats_bytes(a));
   cudaStream_t st = (cudaStream_t)stream;

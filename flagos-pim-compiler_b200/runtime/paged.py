@@ -253,8 +253,8 @@ class PagedLlama:
 
     # -- generation -------------------------------------------------------------------------------------------------
     def check(self, *more) -> None:
-        """Raises if a step (or a call of the operators ``more``) met a bad id, length, position or page.  Waits for the
-        device; every flag is cleared, so what follows is judged by itself."""
+        """Raises if a step (or a call of the operators ``more``) met a bad id, length, position, page or logit.  Waits for
+        the device; every flag is cleared, so what follows is judged by itself."""
         self.torch.cuda.synchronize(self.device)
         said = []
         if bool(self.err.any()):
@@ -344,5 +344,5 @@ class PagedLlama:
             for i in range(steps - 1, -1, -1):
                 result.tokens[j, i] = tok[i, at]
                 at = par[i, at]
-        self.check(reorder)
+        self.check(first, select, reorder)
         return result

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define PIM_ABI_VERSION 14
+#define PIM_ABI_VERSION 15
 
 enum pim_dtype { PIM_F32 = 0, PIM_BF16 = 1, PIM_I32 = 2, PIM_I64 = 3 };
 enum pim_status { PIM_OK = 0, PIM_EINVAL = 1, PIM_ECUDA = 2, PIM_EUNSUPPORTED = 3 };
@@ -487,13 +487,15 @@ typedef struct pim_beam_select_args {
   int32_t vocab;            /* <= 2^19 */
   int32_t eos;              /* -1: no such token */
   int32_t pad;              /* the token a beam that has ended continues with, 0 <= pad < vocab */
+  int32_t* err_flag;
 } pim_beam_select_args;
 
 /* One step of beam search, per batch entry: the beams_out largest of
  * scores[w] + logits[w][t] - log(sum_u exp(logits[w][u])) over beams w and tokens t, ties to the
  * lowest w * vocab + t; a beam that has ended offers one candidate, `pad` at its score.  A
  * logit that is not finite is no candidate and no part of the sum; a beam whose score is
- * not finite offers none.  Where fewer than beams_out candidates are left, the rest get
+ * not finite offers none.  -inf is a mask, in either; NaN and +inf raise *err_flag (the logits
+ * of a beam that has ended are not looked at).  Where fewer than beams_out candidates are left, the rest get
  * score -inf, parent 0, token `pad`, done 1.  Candidates of one beam are compared by their
  * logits, those of different beams by their scores in fp64 (of equal ones the lower beam is
  * first); scores_out is rounded once.

@@ -740,6 +740,40 @@ def test_beam_select_logits_near_the_types_limits(vocab, dt):
     _check_select(logits[:, :1], torch.tensor([[-1.5]], device="cuda"), 5)
 
 
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [30, 5003, 70000])
+def test_beam_select_reports_nan_and_infinity(vocab, dt):
+    """-inf is a mask and no error, and nothing of an ended beam's logits is looked at; the results are as without it."""
+    from backend.cuda_paged import BeamSelect
+
+    torch = _torch()
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    clean = torch.randn(2, 3, vocab, device="cuda", generator=g).to(_tdt(dt))
+    clean[1, 0, ::2] = -inf
+    clean[0, 2] = -inf
+    logits, scores, done = clean.clone(), torch.zeros(2, 3, device="cuda"), _ints([[0, 0, 0], [0, 1, 0]])
+    scores[1, 2] = -inf
+    outs = (torch.zeros(2, 4, device="cuda"), *(torch.zeros(2, 4, dtype=torch.int32, device="cuda") for _ in range(2)))
+    op = BeamSelect(logits, scores, *outs, done=done)
+    logits[1, 1] = nan  # (ended)
+    op()
+    op.check()
+    for bad in (nan, inf):
+        for b, w, t in ((0, 0, 0), (0, 1, vocab - 1), (1, 0, vocab // 2)):
+            logits[b, w, t] = bad
+            op()
+            with pytest.raises(ValueError, match="a logit or score was NaN"):
+                op.check()
+            logits[b, w, t] = clean[b, w, t]
+            op()
+            op.check()
+    scores[0, 1] = nan
+    op()
+    with pytest.raises(ValueError, match="a logit or score was NaN"):
+        op.check()
+
+
 def _crowded_rows(vocab, dt):
     """Rows whose sums of exponentials have as many equal terms as can be: a rounding of one is a rounding of the sum."""
     torch = _torch()
