@@ -35,11 +35,12 @@
 // layout that the second product's B fragment needs, so that one is taken as V^T P^T: 16 dims
 // by 8 heads a tile.  P enters as three bf16 parts, each what is left of a probability rounded
 // towards zero: 3 x 8 bits are all 24 of a float.  (Two
-// parts: sums of p v that cancel are off by 2^-18 of their terms; 650 us for the 64 rows above
-// against 661, 117.0 for the ragged ones against 117.5.)  The next tile's K loads start as soon as this
-// one's scores are formed, its V loads once this one's V is paired, before the products that read
-// the pairs (688 us behind them).  tcgen05 would add staging in shared memory and TMEM for a product
-// of 8 rows that the memory system bounds.
+// parts: sums of p v that cancel are off by 2^-18 of their terms, and the 64 rows above take 1.7 %
+// less.)  A step's products are summed from zero and added to the rest in fp32: see step(); that
+// costs 0.6 % more.  The next tile's K loads start as soon as this one's scores are formed, its V
+// loads once this one's V is paired, before the products that read the pairs (4 % behind them).
+// tcgen05 would add staging in shared memory and TMEM for a product of 8 rows that the memory
+// system bounds.
 //
 // fp32: a key's dims are spread over head_dim / 4 lanes; the partial dot products of several
 // keys and heads are summed by one butterfly that leaves one score per lane.
@@ -300,12 +301,18 @@ struct MmaCore {
         for (int i = 0; i < 4; ++i)
           v[c * VE / 2 + w][i] = __byte_perm(vr[i / 2 * 2][c][w], vr[i / 2 * 2 + 1][c][w], i % 2 ? 0x7632 : 0x5410);
     next_v();
+    // A tile's products are summed from zero, the smallest part of P first, and added to the rest in fp32: the tensor cores'
+    // own additions round towards zero, which over thousands of keys adds up to several times the error of nearest.
 #pragma unroll
-    for (int x = 0; x < kPParts; ++x)
+    for (int h = 0; h < HI; ++h)
 #pragma unroll
-      for (int h = 0; h < HI; ++h)
+      for (int n = 0; n < NT; ++n) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma(acc[h][n], v[n][0], v[n][1], v[n][2], v[n][3], part[x][0][h], part[x][1][h]);
+        for (int x = kPParts - 1; x >= 0; --x) mma(d, v[n][0], v[n][1], v[n][2], v[n][3], part[x][0][h], part[x][1][h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[h][n][e] += d[e];
+      }
   }
 
   // The state of part `warp` into shared memory: [parts][NH] max and sum, [parts][NH][HD] output.

@@ -254,6 +254,35 @@ def test_attention_probabilities_keep_32_bits_where_their_products_cancel(form, 
 
 
 @pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("group", [1, 12])
+def test_attention_sums_over_long_rows_round_to_nearest(group, dt):
+    """Keys of the second half repeat the first half's with V negated: the sum is 0, and what comes out is what its additions
+    lost.  A warp adds its keys in up to S = 260 steps (448 units of 256 tiles on 444 CTAs or fewer, twice that where a group
+    makes two tiles); rounded to nearest, each is off by at most 2^-24 of a partial sum that grows to half of its share W of
+    the row's weight, as if at random: a deviation of 2^-24 / sqrt(3) sqrt(S / 3) W / 2 = 2.7 x 2^-24 W, halved again by the
+    four warps (and over more and shorter ones in fp32).  Eight deviations, doubled for units that two CTAs share: 22 x 2^-24.
+    Additions that round towards zero lose some 140 x 2^-24 here."""
+    from backend.cuda_paged import PagedAttention
+
+    torch = _torch()
+    n, ps, hd, rows = 16384, 256, 32, 448
+    rng = np.random.default_rng(group)
+    key = -rng.integers(0, 257, n // 2) / 256.0
+    value = np.where(rng.random((1, hd)) < 0.5, -1.0, 1.0) * np.ones((n // 2, hd))
+    key[::8], value[::8] = 0, 0  # every step begins with the largest score: the running maximum never moves
+    k = torch.zeros(n, hd, device="cuda")
+    k[:, 0] = torch.tensor(np.tile(key, 2), device="cuda")
+    v = torch.tensor(np.concatenate([value, -value]), device="cuda")
+    k, v = (x.to(_tdt(dt)).view(n // ps, 1, ps, hd) for x in (k, v))
+    table = _ints(np.tile(np.arange(n // ps), (rows, 1)))  # all rows read the same pages
+    q = torch.zeros(rows, group, hd, device="cuda", dtype=_tdt(dt))
+    q[:, :, 0] = 1
+    out = torch.full_like(q, float("nan"))
+    PagedAttention(q, k, v, table, _ints([n] * rows), out, scale=1.0)()
+    assert np.abs(_host(out)).max() <= 2.0**-19, np.abs(_host(out)).max() * 2.0**24
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
 @pytest.mark.parametrize("group", [1, 6, 12])
 @pytest.mark.parametrize("form", ["one", "cluster", "split"])
 def test_attention_infinite_values_come_out_as_the_sum_has_them(form, group, dt):
