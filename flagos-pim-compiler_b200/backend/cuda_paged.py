@@ -23,6 +23,7 @@ raises the operator's error flag, which ``check()`` turns into an exception (it 
 from __future__ import annotations
 
 import ctypes
+import operator
 
 from backend import _native as nat
 
@@ -46,6 +47,14 @@ def _want(t, what: str, shape, dtype: str, contiguous: bool = True):
     if not contiguous and t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: its last dimension must be contiguous")
     return t
+
+
+def _int32(value, what: str) -> int:
+    """``value`` as the argument structs hold it (ctypes would cut it down to 32 bits without a word)."""
+    value = operator.index(value)
+    if not -2**31 <= value < 2**31:
+        raise ValueError(f"{what}={value} does not fit 32 bits")
+    return value
 
 
 def _dt(t) -> str:
@@ -346,8 +355,8 @@ class PagedAttention(_Op):
         _want(q, "q", (kv.rows, None, kv.head_dim), dt, contiguous=False)
         _want(out, "out", tuple(q.shape), dt, contiguous=False)
         _want(lengths, "lengths", (kv.rows,), "int32")
-        if scale is not None and not scale > 0:
-            raise ValueError(f"scale must be positive, got {scale}")
+        if scale is not None and not 0 < ctypes.c_float(scale).value < float("inf"):  # (0 would stand for the default)
+            raise ValueError(f"scale must be a positive fp32 number, got {scale}")
         a = nat.PagedAttentionArgs(kv=kv, q=q.data_ptr(), out=out.data_ptr(), q_stride=_row_stride(q),
                                    out_stride=_row_stride(out), lengths=lengths.data_ptr(), q_heads=q.shape[1],
                                    scale=0.0 if scale is None else scale)
@@ -403,7 +412,8 @@ class PagedEvict(_Op):
                                weights=weights.data_ptr(), slot_positions=slot_positions.data_ptr(),
                                weights_out=weights_out.data_ptr(), slot_positions_out=slot_positions_out.data_ptr(),
                                lengths_out=lengths_out.data_ptr(), state_row_stride=row, state_head_stride=head,
-                               budget=budget, recent=recent, sink=sink)
+                               budget=_int32(budget, "budget"), recent=_int32(recent, "recent"),
+                               sink=_int32(sink, "sink"))
         self._bind(a, _code(k_pages, "k_pages"),
                    (k_pages, v_pages, table, lengths, weights, slot_positions, positions, weights_out,
                     slot_positions_out, lengths_out))
@@ -444,7 +454,7 @@ class BeamSelect(_Op):
             _want(done, "done", (b, w), "int32")
         a = nat.BeamSelectArgs(logits=logits.data_ptr(), logits_stride=stride, scores=scores.data_ptr(),
                                scores_out=scores_out.data_ptr(), parents=parents.data_ptr(), tokens=tokens.data_ptr(),
-                               batch=b, beams=w, beams_out=k, vocab=vocab, eos=eos, pad=pad)
+                               batch=b, beams=w, beams_out=k, vocab=vocab, eos=_int32(eos, "eos"), pad=_int32(pad, "pad"))
         if done is not None:
             a.done = done.data_ptr()
         if done_out is not None:

@@ -403,3 +403,26 @@ def test_evict_and_reorder_classes_keep_the_pages_apart_from_what_they_read():
         a = {**dict(table=table, lengths=lengths, parents=parents), **kw}
         with pytest.raises(ValueError, match=f"pages shares memory with {said}"):
             BeamReorder(pool, a["table"], a["lengths"], a["parents"], torch.zeros(8, 3, dtype=torch.int32))
+
+
+def test_numbers_that_the_argument_structs_cannot_hold_are_refused():
+    """A budget of 2^32 + 1 is not one of 1, and a scale that fp32 rounds to 0 is not the default scale."""
+    from backend.cuda_paged import BeamSelect, PagedAttention, PagedEvict
+
+    t = _tensors()
+    w, p = torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, dtype=torch.int32)
+    n, out = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    pages = (t["k_pages"], t["v_pages"], t["table"], t["lengths"])
+    for kw, said in ((dict(budget=2**32 + 1), "budget"), (dict(budget=9, recent=2**32), "recent"),
+                     (dict(budget=9, sink=-2**31 - 1), "sink")):
+        with pytest.raises(ValueError, match=f"{said}=.* 32 bits"):
+            PagedEvict(*pages, w, p, n, w, p, out, **kw)
+    q, o = (torch.zeros(3, 4, 64, dtype=torch.bfloat16) for _ in range(2))
+    for scale in (1e-50, 1e39, float("inf"), float("nan"), -1.0):
+        with pytest.raises(ValueError, match="scale must be"):
+            PagedAttention(q, *pages, o, scale=scale)
+    lg, sc = torch.zeros(2, 4, 100), torch.zeros(2, 4)
+    outs = (torch.zeros(2, 4), torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32))
+    for kw, said in ((dict(eos=2**32 + 5), "eos"), (dict(pad=2**32), "pad")):
+        with pytest.raises(ValueError, match=f"{said}=.* 32 bits"):
+            BeamSelect(lg, sc, *outs, **kw)
