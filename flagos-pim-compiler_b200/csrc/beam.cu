@@ -106,8 +106,9 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long key) 
 
 constexpr int kBeamWarps = kBeamThreads / 32;
 // Candidates that are ranked by counting; of more (warps that a mask leaves nothing set no bound, equal logits pass it
-// together, sorted ones crowd in one warp) the exact bound is found first.  256 rows of 32000 bf16 logits, of which 1500
-// are kept: 22.5 us at 256 or 512, 233 at 2048; ascending logits 37 and 492; random ones 15.3.
+// together, sorted ones crowd in one warp) the exact bound is found first.  256 rows of 32000 bf16 logits: random ones
+// 20.5 us, ascending 42, of which 1500 are kept 28.5.  (With the sums still in fp32, at 256 or 512 and at 2048: ascending 37
+// and 492, 1500 kept 22.5 and 233, random 15.3.)
 constexpr int kCountMost = 512;
 template <typename T, bool ALIGNED, int kBeamVals>
 __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectArgs a) {
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_partial_kernel(BeamSelectAr
   }
 }
 
-constexpr int kMergeThreads = 1024;  // (512: 4 x 16 beams 25.2 us, 4 x 64 78; with 1024 21.4 and 63, fewer beams the same)
+constexpr int kMergeThreads = 1024;  // (512, with fp32 sums: 4 x 16 beams and their reordering 25.2 us, 4 x 64 78; with 1024 21.4 and 63, fewer the same)
 constexpr int kDeep = 4;  // keys of a list at hand
 
 // Order-preserving bits of a finite double, never 0.
@@ -475,8 +476,8 @@ static const char* beam_select_error(const pim_beam_select_args* a, int dtype) {
 }
 
 // Logits of a thread: 32 where that leaves two chunks for every SM, which halves the lists and the work beside the
-// logits (8 x 16 beams of 131072 fp32 logits with the reordering: 64.2 us against 69.4; 32 x 8 of 32000 bf16: 85.5 against
-// 86.5); else 16, for more CTAs.
+// logits (8 x 16 beams of 131072 fp32 logits with the reordering: 65.7 us against 71.4; 32 x 8 of 32000 bf16: 85.2 against
+// 89.2); else 16, for more CTAs.
 static int beam_vals(const pim_beam_select_args* a) {
   return (int64_t)a->batch * a->beams * ceil_div(a->vocab, 2 * kBeamChunk) >= 2 * 148 ? 32 : 16;
 }
@@ -592,7 +593,7 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   if (page * es / 16 > (1 << 30)) return bad("a page of more than 16 GiB");
   // The copies follow from the parents and the lengths.  A CTA per step of those that half-filled pages and a third of the
   // beams give, at least as many as run at once and at most a few rounds of them: a thousand CTAs cost 1.1 us to launch,
-  // with nothing to do too, and a step per CTA balances best (device us with the selection at 24, 48 and 96 CTAs an SM: 32 x 8
+  // with nothing to do too, and a step per CTA balances best (device us with a selection of 16 at 24, 48 and 96 CTAs an SM: 32 x 8
   // beams with 354 MB to copy 92, 87, 83; 16 x 12 beams with eight slots in use 17.5, 21.1, 26.4; at a sixth of the full pages'
   // steps 84 and 17.5).
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);

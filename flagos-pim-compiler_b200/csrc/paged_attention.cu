@@ -17,9 +17,9 @@
 // 121.4, 115.2, 115.8 and 117.1 with 1, 2, 3 and 5 tiles).  paged_finish_kernel joins the
 // partials: which CTAs hold a unit follows from the lengths alone, so there are no tickets, no
 // atomics and nothing that must be zero before a call, and the result does not depend on timing.
-// Measured: 64 rows x 4096 keys x 32 heads 4.27 GB in 665 us, 6.4 TB/s; the ragged rows above
-// 662 MB in 116 us, 5.7 TB/s (DRAM 70 % busy, tensor pipe 17 %, 8 warps an SM that mostly wait
-// for their loads); what did not help there: a third CTA per SM with fewer registers (139 us),
+// Measured: 64 rows x 4096 keys x 32 heads 4.27 GB in 653 to 689 us on different GPUs, 6.2 to 6.5 TB/s;
+// the ragged rows above 662 MB in 117 to 123 us, 5.4 to 5.7 TB/s (DRAM 71 % busy, tensor pipe 21 %, 8 warps
+// an SM that mostly wait for their loads); what did not help there, at 116 us: a third CTA per SM with fewer registers (139 us),
 // asking L2 for tiles ahead (134 to 145), loads that run on into the next unit (136), 32-byte
 // loads (117), CTAs of 1 or 2 warps (119, 118).
 //
@@ -83,7 +83,8 @@ constexpr int kTile = 64;          // keys of a tile
 constexpr int kMaxCluster = 8;
 constexpr int kUnitCost = 2;       // what a unit costs beside its tiles, in tiles: see the head of the file
 constexpr int kSplitWarps = 4;     // of a CTA that walks a range of tiles
-// CTAs of the splitting kernel per SM: what its registers allow without spilling.
+// CTAs of the splitting kernel per SM: what its registers allow with next to no spilling (fp32 of 128 dims with 4 or 8 heads
+// 28 to 32 bytes, bf16 with 16 heads up to 8; the others none).
 constexpr int paged_ctas_per_sm(bool bf16, int hd) { return bf16 && hd == 128 ? 2 : 3; }
 constexpr int kFinishThreads = 128;
 constexpr int kFinishKeys = 4 * kFinishThreads;  // keys whose weights one CTA adds to
@@ -101,6 +102,7 @@ __device__ __forceinline__ int row_cost(const PagedAttnArgs& a, int row) {
 }
 // A share of a row's sum: 0 where no key had a score above -inf, NaN where a score was NaN.
 __device__ __forceinline__ float quotient(float a, float sum) { return sum == 0.f ? 0.f : a / sum; }
+// Off by at most 2 units in the last place, as exp2f is; results below 2^-126 come out 0 (the weights, by exp2f, have them).
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -1033,6 +1035,8 @@ static PagedLayout paged_layout(const pim_paged_attention_args* a, int dtype) {
   p.ctas = paged_ctas(dtype, a->kv.head_dim);
   const int64_t slots = (int64_t)a->kv.max_pages * a->kv.page_size, units = (int64_t)a->kv.rows * a->kv.kv_heads * p.tiles;
   // Whole units in a CTA or a cluster save the second launch and the join, and lose where rows are long or units many.
+  // "Slots" are the table's: lengths are on the device, so short rows of a wide table are split (1 row of 130 keys x 32
+  // heads: 4.9 us in a table of 144 slots, 5.4 in 512 to 2048, 8.2 in 4096 and more).
   // Few units: 8 warps a CTA and the largest cluster that leaves every CTA an SM, up to 512 slots a CTA (fp32 256); one CTA
   // up to 256 slots, where a cluster gains nothing.  Device us by slots 256, 512, 1024, 2048, 4000:
   //   1 row x 8 heads x 4    clusters of 8  5.6  5.7  6.5  7.6  9.5   one CTA 5.6  7.5          split - 8.5  9.5  9.9 11.8

@@ -664,7 +664,8 @@ static cudaError_t select_rows(EvictArgs a, cudaStream_t st) {
   // Long rows of few units in clusters, of CTAs that have an SM and 2048 slots each.  Device us by slots 4096, 8192, 16384, 32768
   // cut to a quarter, of one CTA and of clusters:  1 unit 10.4 14.1 21.1 35.4 and 11.5 12.7 15.4 17.4;  8 units 10.9 14.7 25.5 39.1
   // and 12.2 14.0 17.5 20.6;  32 units 15.5 18.1 28.0 51.6 and 13.8 19.1 24.9 33.6;  64 units 16.3 22.1 38.3 and 16.4 23.0 33.9;
-  // 8 heads of 131000 to 16384, which one CTA reads anew at each pass, 338 and 33; 8 heads one over 16384 8.7 and 5.5.
+  // 8 heads of 131000 to 16384, which one CTA reads anew at each pass, 338 and 35 (rows of 64 bytes; 53 with 256); 8 heads
+  // one over 16384 8.7 and 5.5.
   // CTAs of 1024 slots: 1 unit - 14.9 15.5 17.4;  two an SM: 32 units - - 32.0 43.2.
   a.cluster = 1;
   if (slots >= 8192)
@@ -676,6 +677,8 @@ static cudaError_t select_rows(EvictArgs a, cudaStream_t st) {
 template <int LPR>
 static cudaError_t evict_rows(const EvictArgs& a, cudaStream_t st) {
   // Where a unit cannot have more moves than the selecting CTA's warps do in one go, that CTA does them: a launch less.
+  // That goes by the table, not by the lengths, which are on the device: 16 rows x 8 heads one over 1024 3.6 us in a table
+  // of 1040 or 1152 slots, 9.5 in one of 2048 and more.
   if (a.max_moves <= kFusedMoves) return select_rows<LPR>(a, st);
   const cudaError_t e = select_rows<0>(a, st);
   if (e != cudaSuccess) return e;

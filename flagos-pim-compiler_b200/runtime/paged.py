@@ -8,9 +8,10 @@
     best = gen.beam_search(prompt, steps=64, eos=2)     # rows beams of one prompt
     gen = PagedLlama(runner, rows=4, max_slots=512, budget=256, recent=64, sink=4)   # evicts to 256 slots a head
 
-A prompt goes through the program's prefill plan, whose KV blocks are then copied into the row's pages; from there on a
-step is the decode plan's projections around ``PagedAppend`` / ``PagedAttention`` (and ``PagedEvict``) for all rows at
-once, captured into one CUDA graph after its first run.  Everything runs on the rank's stream.
+A prompt goes through the program's prefill plan (which overwrites the program's static cache), whose KV blocks are then
+copied into the row's pages, with accumulated weights of 0 where the cache is bounded; from there on a step is the decode
+plan's projections around ``PagedAppend`` / ``PagedAttention`` (and ``PagedEvict``) for all rows at once, captured into one
+CUDA graph after its first run.  Everything runs on the rank's stream.
 """
 
 from __future__ import annotations
