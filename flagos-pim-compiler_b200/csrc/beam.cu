@@ -593,9 +593,9 @@ extern "C" int pim_beam_reorder(const pim_beam_reorder_args* a, int32_t dtype, v
   if (page * es / 16 > (1 << 30)) return bad("a page of more than 16 GiB");
   // The copies follow from the parents and the lengths.  A CTA per step of those that half-filled pages and a third of the
   // beams give, at least as many as run at once and at most a few rounds of them: a thousand CTAs cost 1.1 us to launch,
-  // with nothing to do too, and a step per CTA balances best (device us with a selection of 16 at 24, 48 and 96 CTAs an SM: 32 x 8
-  // beams with 354 MB to copy 92, 87, 83; 16 x 12 beams with eight slots in use 17.5, 21.1, 26.4; at a sixth of the full pages'
-  // steps 84 and 17.5).
+  // with nothing to do too, and a step per CTA balances best (device us with a selection whose sums were fp32, at 24, 48 and
+  // 96 CTAs an SM: 32 x 8 beams with 354 MB to copy 92, 87, 83; 16 x 12 beams with eight slots in use 17.5, 21.1, 26.4; at a
+  // sixth of the full pages' steps 84 and 17.5).
   const int64_t steps = (int64_t)a->num_blocks * ceil_div(page * es / 16, kCopyPieces);
   if (steps > INT32_MAX) return bad("more than 2^31 steps of 8 KiB to copy a page of every block");
   const int rows = a->batch * a->beams;
