@@ -73,6 +73,7 @@ class PagedLlama:
             self.next_ids = buf(rows, dtype=torch.int32)
             self.err = buf(2, dtype=torch.int32)  # embedding, projections
             self._build(recent, sink)
+        self._imports: dict[int, list] = {}    # row -> the operators that take its prompt in
         self.graph, self._warm = None, False
         self.slots = np.zeros(rows, np.int64)  # slots in use after the steps enqueued so far
         self.pos_host = 0                      # position of the rows' next token
@@ -192,7 +193,7 @@ class PagedLlama:
             self.lengths.zero_()
             self.positions.zero_()
             self.err.zero_()
-            for op in self.ops:
+            for op in self._bound():
                 op.clear()
         self.slots[:] = 0
         self.pos_host = 0
@@ -223,6 +224,13 @@ class PagedLlama:
 
     def _import(self, row: int) -> None:
         """The prompt's K and V from the static cache into the row's pages."""
+        if row not in self._imports:
+            self._imports[row] = self._bind_import(row)
+        for op in self._imports[row]:
+            op()
+
+    def _bind_import(self, row: int) -> list:
+        """A row's operators for that, one a layer; kept, as those of a step are."""
         torch, c, n = self.torch, self.cache, self.prog.prompt_len
         starts = torch.tensor([0, n], dtype=torch.int32, device=self.device)
         zero = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -231,13 +239,10 @@ class PagedLlama:
             k, v = (t[:n] for t in self._blocks(l))
             track = {} if self.budget is None else dict(slot_positions=c.slot_positions[l, row:row + 1],
                                                         weights=c.weights[l, row:row + 1])
-            op = PagedAppend(k, v, c.k(l), c.v(l), c.table[row:row + 1], zero, self.lengths[row:row + 1],
-                             positions_out=self.positions[row:row + 1], positions=torch.zeros_like(zero), starts=starts,
-                             **track)
-            op()
-            ops.append(op)
-        for op in ops:
-            op.check()
+            ops.append(PagedAppend(k, v, c.k(l), c.v(l), c.table[row:row + 1], zero, self.lengths[row:row + 1],
+                                   positions_out=self.positions[row:row + 1], positions=torch.zeros_like(zero),
+                                   starts=starts, **track))
+        return ops
 
     def _start(self, prompts) -> None:
         """Every row's prompt into its pages and its last logits into ``logits``."""
@@ -252,6 +257,9 @@ class PagedLlama:
         self.slots[:len(prompts)] = n
         self.pos_host = n
 
+    def _bound(self) -> list:
+        return [*self.ops, *(op for ops in self._imports.values() for op in ops)]
+
     # -- generation -------------------------------------------------------------------------------------------------
     def check(self, *more) -> None:
         """Raises if a step (or a call of the operators ``more``) met a bad id, length, position, page or logit.  Waits for
@@ -261,7 +269,7 @@ class PagedLlama:
         if bool(self.err.any()):
             self.err.zero_()
             said.append("a token id was outside the vocabulary, or a projection's wait ran out")
-        for op in (*self.ops, *more):
+        for op in (*self._bound(), *more):
             try:
                 op.check()
             except ValueError as e:

@@ -286,3 +286,24 @@ def test_an_error_is_reported_once_and_the_next_run_is_judged_by_itself():
         spoil()
         gen.step()
         assert gen.greedy(prompt, 8)[0].tolist() == gold["tokens"].tolist()  # (a new start: what was before is not its error)
+
+
+def test_prompts_are_taken_in_by_operators_that_are_bound_once(monkeypatch):
+    """A later start binds nothing and waits for nothing of its own; a bad page met on the way in is reported by ``check``."""
+    import runtime.paged as module
+
+    gold = tiny_golden()
+    bound = []
+    monkeypatch.setattr(module, "PagedAppend", lambda *a, _make=module.PagedAppend, **kw: bound.append(1) or _make(*a, **kw))
+    gen = module.PagedLlama(_runner(tiny_hf_model()), rows=2, max_slots=40, page_size=8)
+    layers = gen.cfg.num_layers
+    prompts = np.stack([gold["prompt"]] * 2)
+    for _ in range(3):
+        assert gen.greedy(prompts, 8)[1].tolist() == gold["tokens"].tolist()
+        assert len(bound) == 3 * layers  # a step's, and one for each row
+    gen._start(prompts)
+    gen.cache.table.fill_(10**6)
+    gen._import(1)
+    with pytest.raises(ValueError, match="pim_paged_append"):
+        gen.check()
+    assert gen.greedy(prompts, 8)[0].tolist() == gold["tokens"].tolist()
