@@ -316,7 +316,11 @@ class PagedLlama:
         with torch.cuda.device(self.device), torch.cuda.stream(self.stream):
             c = self.cache
             c.share_prompt(n)
-            c.reserve([n + steps - 1] * w)  # a tail for each beam: its partly filled page and what the search will fill
+            try:  # a tail for each beam: its partly filled page and what the search will fill
+                c.reserve([n + steps - 1] * w)
+            except MemoryError:
+                self.reset()  # (rows that hold the prompt's pages and no tail must not take a step)
+                raise
             c.upload()
             self._beam_tables = True  # from here on the table is the device's
             self._beam_slots = n + steps - 1

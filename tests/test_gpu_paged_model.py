@@ -307,3 +307,15 @@ def test_prompts_are_taken_in_by_operators_that_are_bound_once(monkeypatch):
     with pytest.raises(ValueError, match="pim_paged_append"):
         gen.check()
     assert gen.greedy(prompts, 8)[0].tolist() == gold["tokens"].tolist()
+
+
+def test_a_search_that_finds_no_pages_leaves_the_rows_empty():
+    """Beams that hold the prompt's pages but have no tail would write their next token into them."""
+    from runtime.paged import PagedLlama
+
+    gold = tiny_golden()
+    gen = PagedLlama(_runner(tiny_hf_model()), rows=2, max_slots=40, page_size=8, num_pages=6)
+    with pytest.raises(MemoryError):
+        gen.beam_search(gold["prompt"], 25)
+    assert gen.cache.allocator.free == 6 and not gen.slots.any() and not any(gen.cache.held)
+    assert gen.greedy(np.stack([gold["prompt"]] * 2), 8)[0].tolist() == gold["tokens"].tolist()
