@@ -201,10 +201,8 @@ class _Op:
             raise ValueError(f"{self.name}: needs CUDA tensors (there is no CPU path)")
         self._torch, self._dev, self._keep = torch, dev, tensors
         self._args, self._code = args, code
-        self._err = None
-        if hasattr(args, "err_flag"):
-            self._err = torch.zeros(1, dtype=torch.int32, device=dev)
-            args.err_flag = self._err.data_ptr()
+        self._err = torch.zeros(1, dtype=torch.int32, device=dev)
+        args.err_flag = self._err.data_ptr()
         self._ref = ctypes.byref(args)
         self._fn = getattr(nat.lib, self.name)
         self._ws, extra = None, ()
@@ -243,21 +241,28 @@ class _Op:
         if rc:
             nat.check(rc, self.name)
 
-    def clear(self) -> None:
-        """Forgets, on the device's current stream, what the calls so far met."""
-        if self._err is not None:
-            self._err.zero_()
-
     def check(self) -> None:
         """Waits for the device, and raises if a call so far, on whichever stream, met a bad length, position, page id,
         parent or logit; clears the flag."""
-        if self._err is None:
-            return
-        self._torch.cuda.synchronize(self._dev)
-        if int(self._err.item()):
-            self._err.zero_()
-            self._torch.cuda.synchronize(self._dev)  # (calls that follow on other streams raise it anew)
-            raise ValueError(f"{self.name}: {self.complaint}")
+        for said in complaints([self]):
+            raise ValueError(said)
+
+
+def forget(ops) -> None:
+    """Clears the flags of operators of one device, on its current stream."""
+    ops[0]._torch._foreach_zero_([op._err for op in ops])
+
+
+def complaints(ops) -> list[str]:
+    """What the calls of these operators of one device met so far, each thing once.  Waits for the device, on whichever
+    streams they ran; their flags are cleared."""
+    torch, dev = ops[0]._torch, ops[0]._dev
+    torch.cuda.synchronize(dev)
+    said = [f"{op.name}: {op.complaint}" for op, bad in zip(ops, torch.cat([op._err for op in ops]).tolist()) if bad]
+    if said:
+        forget(ops)
+        torch.cuda.synchronize(dev)  # (calls that follow on other streams raise them anew)
+    return list(dict.fromkeys(said))
 
 
 class PagedAppend(_Op):

@@ -22,7 +22,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from backend import _native as nat
-from backend.cuda_paged import BeamReorder, BeamSelect, PagedAppend, PagedAttention, PagedEvict
+from backend.cuda_paged import BeamReorder, BeamSelect, PagedAppend, PagedAttention, PagedEvict, complaints, forget
 from memory.paged_kv import PagedKVCache, PagedKVSpec
 from runtime.executor import execute_plan
 
@@ -193,8 +193,7 @@ class PagedLlama:
             self.lengths.zero_()
             self.positions.zero_()
             self.err.zero_()
-            for op in self._bound():
-                op.clear()
+            forget(self._bound())
         self.slots[:] = 0
         self.pos_host = 0
         self._beam_tables = False
@@ -264,19 +263,13 @@ class PagedLlama:
     def check(self, *more) -> None:
         """Raises if a step (or a call of the operators ``more``) met a bad id, length, position, page or logit.  Waits for
         the device; every flag is cleared, so what follows is judged by itself."""
-        self.torch.cuda.synchronize(self.device)
-        said = []
+        said = complaints([*self._bound(), *more])
         if bool(self.err.any()):
             self.err.zero_()
-            said.append("a token id was outside the vocabulary, or a projection's wait ran out")
-        for op in (*self._bound(), *more):
-            try:
-                op.check()
-            except ValueError as e:
-                said.append(str(e))
-        if said:
             self.torch.cuda.synchronize(self.device)
-            raise ValueError("; ".join(dict.fromkeys(said)))
+            said.append("a token id was outside the vocabulary, or a projection's wait ran out")
+        if said:
+            raise ValueError("; ".join(said))
 
     def greedy(self, prompts, steps: int, keep_logits: list | None = None) -> np.ndarray:
         """[rows, steps] tokens; ``keep_logits`` (a list) receives each step's [rows, vocab] logits."""
